@@ -281,6 +281,68 @@ zl_status zl_embedding_backward_bf16(const int32_t *ids, const zl_bf16 *dx, floa
 zl_status zl_cross_entropy_fused_bf16(zl_bf16 *logits, const int32_t *targets, int rows, int vocab,
                                       float eps, float grad_scale, float *loss_rows, float *loss_out,
                                       zl_stream stream);
+/* ---- operators on next-token distributions (no reference counterpart: its loss works on softmax
+ *      probabilities, cross_entropy.cpp:23-79) ----
+ * Rows of logits are vocab elements long and row_stride >= vocab elements apart, at any element-aligned
+ * address (rows on 16-byte boundaries are the fastest); y = scale * x, scale in [1e-4, 1e4] an inverse
+ * temperature.  rows = 0 does nothing.  -inf masks a logit: its p is 0 and adds nothing to any sum; a row
+ * whose logits are all -inf has lse and every log probability -inf, entropy 0, no gradient.  A NaN or +inf
+ * logit makes its row's statistics NaN.  No entry allocates or waits; all can be captured into a graph.
+ * Results do not depend on the launch: every sum has a fixed order.
+ *
+ * Log probabilities of given tokens, entropy, log-sum-exp and top alternatives of each row:
+ *   lse[r] = ln sum_j e^{y_j},  logp[r] = y_t - lse with t = targets[r] (0 where t is not in [0, vocab)),
+ *   entropy[r] = -sum_j p_j ln p_j,
+ *   top_ids / top_logp [rows, top_k]: the top_k largest logits, largest first (equal ones by the lower index,
+ *   NaN last), and their log probabilities.
+ * logp, entropy, lse, top_logp may be NULL; targets may be NULL without logp.  top_k in [0, min(vocab, 128)]. */
+zl_status zl_token_logprobs_bf16(const zl_bf16 *logits, int64_t row_stride, const int32_t *targets, int rows,
+                                 int vocab, float scale, int top_k, float *logp, float *entropy, float *lse,
+                                 float *top_logp, int32_t *top_ids, zl_stream stream);
+zl_status zl_token_logprobs_f32(const float *logits, int64_t row_stride, const int32_t *targets, int rows, int vocab,
+                                float scale, int top_k, float *logp, float *entropy, float *lse, float *top_logp,
+                                int32_t *top_ids, zl_stream stream);
+/* Their gradient: d_logits[r, j] = scale ( g_logp[r] (1[j = t] - p_j) - g_entropy[r] p_j (ln p_j + entropy[r]) )
+ * with lse and entropy as the forward wrote them.  g_logp or g_entropy may be NULL (a zero gradient; entropy is
+ * then not read); rows without a target take nothing from g_logp, and rows masked wholly (lse below -1e30: all
+ * -inf, or all the type's lowest value) have none.  d_logits may be logits (with its row stride)
+ * but may not overlap it in any other way. */
+zl_status zl_token_logprobs_backward_bf16(const zl_bf16 *logits, int64_t row_stride, const int32_t *targets,
+                                          const float *lse, const float *entropy, const float *g_logp,
+                                          const float *g_entropy, int rows, int vocab, float scale,
+                                          zl_bf16 *d_logits, int64_t d_row_stride, zl_stream stream);
+zl_status zl_token_logprobs_backward_f32(const float *logits, int64_t row_stride, const int32_t *targets,
+                                         const float *lse, const float *entropy, const float *g_logp,
+                                         const float *g_entropy, int rows, int vocab, float scale, float *d_logits,
+                                         int64_t d_row_stride, zl_stream stream);
+/* Distillation from a teacher's top logits, with the hard targets' cross-entropy beside it where wanted:
+ *   q = softmax(teacher_scale * v) over a row's alternatives (normalize = 1), or e^{teacher_scale * v} as they are
+ *       (normalize = 0: recorded log probabilities, whose sum may be below 1),
+ *   KD = sum_i q_i (ln q_i - ln p_{id_i}) with p = softmax(scale * x),  CE = -ln softmax(x)_t,
+ *   loss_rows[r] = row_weight[r] (distill_weight KD + target_weight CE),
+ *   *loss_out = grad_scale * sum_r loss_rows[r],  d_logits = the gradient of *loss_out.
+ * teacher_ids / teacher_logits [rows, top_k], top_k in [0, 128]; an id not in [0, vocab) is no alternative (short
+ * lists end in -1), an id given twice counts twice.  targets may be NULL with target_weight 0; a target not in
+ * [0, vocab) adds nothing.  row_weight may be NULL (all 1); a row of weight 0 has loss and gradient 0 whatever
+ * it holds, as has a student row with nothing left.  d_logits may be NULL (the loss alone) or logits (with its
+ * row stride), but may not overlap it in any other way; loss_out may be NULL. */
+typedef struct {
+  float scale;           /* of the student's logits: 1 / temperature */
+  float teacher_scale;   /* of the teacher's, in [1e-4, 1e4] */
+  int normalize;
+  float distill_weight, target_weight;
+  float grad_scale;      /* e.g. 1 / rows */
+} zl_distill_options;
+zl_status zl_distill_topk_bf16(const zl_bf16 *logits, int64_t row_stride, const int32_t *teacher_ids,
+                               const float *teacher_logits, int top_k, const int32_t *targets,
+                               const float *row_weight, const zl_distill_options *opt, int rows, int vocab,
+                               zl_bf16 *d_logits, int64_t d_row_stride, float *loss_rows, float *loss_out,
+                               zl_stream stream);
+zl_status zl_distill_topk_f32(const float *logits, int64_t row_stride, const int32_t *teacher_ids,
+                              const float *teacher_logits, int top_k, const int32_t *targets,
+                              const float *row_weight, const zl_distill_options *opt, int rows, int vocab,
+                              float *d_logits, int64_t d_row_stride, float *loss_rows, float *loss_out,
+                              zl_stream stream);
 /* Column sums of a bf16 [M, N] matrix accumulated into db (fp32): bias gradients.  N a multiple of 8
  * (ZL_EUNSUPPORTED otherwise); dy 16-byte aligned (ZL_EINVAL otherwise). */
 zl_status zl_colsum_bf16(const zl_bf16 *dy, float *db, float *workspace, int64_t M, int N, zl_stream stream);

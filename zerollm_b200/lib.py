@@ -41,6 +41,11 @@ class AdamWConfig(C.Structure):
     _fields_ = [("beta1", f32), ("beta2", f32), ("eps", f32), ("weight_decay", f32)]
 
 
+class DistillOptions(C.Structure):
+    _fields_ = [("scale", f32), ("teacher_scale", f32), ("normalize", i32), ("distill_weight", f32),
+                ("target_weight", f32), ("grad_scale", f32)]
+
+
 # name -> (restype, argtypes); every zl_* returning zl_status uses i32
 SIGNATURES = {
     "zl_last_error": (C.c_char_p, []),
@@ -84,6 +89,11 @@ SIGNATURES = {
     "zl_embedding_forward_bf16": (i32, [vp, vp, vp, vp, i64, i32, i32, i32, vp]),
     "zl_embedding_backward_bf16": (i32, [vp, vp, vp, i64, i32, i32, vp]),
     "zl_cross_entropy_fused_bf16": (i32, [vp, vp, i32, i32, f32, f32, vp, vp, vp]),
+    **{f"zl_token_logprobs_{t}": (i32, [vp, i64, vp, i32, i32, f32, i32, vp, vp, vp, vp, vp, vp]) for t in ("bf16", "f32")},
+    **{f"zl_token_logprobs_backward_{t}": (i32, [vp, i64, vp, vp, vp, vp, vp, i32, i32, f32, vp, i64, vp])
+       for t in ("bf16", "f32")},
+    **{f"zl_distill_topk_{t}": (i32, [vp, i64, vp, vp, i32, vp, vp, C.POINTER(DistillOptions), i32, i32, vp, i64, vp, vp,
+                                      vp]) for t in ("bf16", "f32")},
     "zl_colsum_bf16": (i32, [vp, vp, vp, i64, i32, vp]),
     "zl_linear_forward_bf16": (i32, [vp, vp, vp, vp, i64, i64, i64, i32, vp]),
     "zl_linear_backward_bf16": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]),
