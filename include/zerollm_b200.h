@@ -343,6 +343,15 @@ zl_status zl_distill_topk_f32(const float *logits, int64_t row_stride, const int
                               const float *row_weight, const zl_distill_options *opt, int rows, int vocab,
                               float *d_logits, int64_t d_row_stride, float *loss_rows, float *loss_out,
                               zl_stream stream);
+/* Log probabilities, entropies and log-sum-exps of logits = hidden weight^T (hidden [rows, dim], weight
+ * [vocab, dim], packed, fp32 accumulation on tcgen05) that are never stored: for scoring.  Outputs as those of
+ * zl_token_logprobs_*, which also gives the gradient where logits are kept.  dim a multiple of 8
+ * (ZL_EUNSUPPORTED otherwise); hidden, weight and workspace (fp32, zl_linear_logprobs_workspace_floats()
+ * elements for the current device) 16-byte aligned.  The workspace serves one call in flight at a time. */
+zl_status zl_linear_logprobs_bf16(const zl_bf16 *hidden, const zl_bf16 *weight, const int32_t *targets, int rows,
+                                  int dim, int vocab, float scale, float *logp, float *entropy, float *lse,
+                                  float *workspace, zl_stream stream);
+int64_t zl_linear_logprobs_workspace_floats(int rows, int dim, int vocab);
 /* Column sums of a bf16 [M, N] matrix accumulated into db (fp32): bias gradients.  N a multiple of 8
  * (ZL_EUNSUPPORTED otherwise); dy 16-byte aligned (ZL_EINVAL otherwise). */
 zl_status zl_colsum_bf16(const zl_bf16 *dy, float *db, float *workspace, int64_t M, int N, zl_stream stream);

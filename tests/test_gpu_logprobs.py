@@ -566,3 +566,105 @@ def test_zero_rows(L):
         L.call(f"zl_distill_topk_{t}", None, 64, None, None, 4, lo.data_ptr(), None, C.byref(o), 0, 64, None, 0, None,
                lo.data_ptr(), stream())
         assert float(lo) == 0.0
+
+
+# ------------------------------------------------------------------ from hidden states
+def call_head(L, h, w, t, scale, st=None):
+    rows, dim = h.shape
+    vocab = w.shape[0]
+    out = {n: torch.full((rows + 3,), 7.0, device="cuda") for n in ("logp", "entropy", "lse")}
+    ws = torch.empty(max(1, L.load().zl_linear_logprobs_workspace_floats(rows, dim, vocab)), device="cuda")
+    L.call("zl_linear_logprobs_bf16", h.data_ptr(), w.data_ptr(), ptr(t), rows, dim, vocab, scale,
+           out["logp"].data_ptr() if t is not None else None, out["entropy"].data_ptr(), out["lse"].data_ptr(), ws.data_ptr(),
+           st if st is not None else stream())
+    torch.cuda.synchronize()
+    for v in out.values():
+        assert bool((v[rows:] == 7.0).all()), "wrote past its rows"
+    return {n: v[:rows] for n, v in out.items()}
+
+
+def check_head(L, h, w, scale=1.0, t=None):
+    """Beside the bounds above a logit is off by at most 2 (dim / 16 + 4) u sum |h w|: products are exact in fp32, and
+    each step of 16 adds one rounding (no better than truncation) of a partial sum.  lse and every ln p move by no
+    more than the row's largest such error, the entropy by that times (1 + ln vocab + its spread)."""
+    rows, dim = h.shape
+    vocab = w.shape[0]
+    scale = C.c_float(scale).value
+    t = targets_for(rows, vocab) if t is None else t
+    out = call_head(L, h, w, t, scale)
+    x = h.double() @ w.double().T
+    logp, lse = softmax64(x, scale)
+    off = scale * 2 * (dim / 16 + 4) * U * (h.double().abs() @ w.double().abs().T).amax(1)
+    # a thread's sums: chunks of 32 (8 additions to a chain), at most vocab / 64 chunks; 148 partials joined
+    E, lnv = (8 + math.ceil(vocab / 64) + 5 * 20) * U, math.log(vocab)
+    ymax = (x * scale).amax(1)
+    close(out["lse"], lse, off + E + 4 * U * (lnv + ymax.abs()), "lse")
+    spread = ((logp.exp() * (logp - (logp.exp() * logp).sum(1, keepdim=True)) ** 2).sum(1)).sqrt()
+    close(out["entropy"], entropy64(logp), 2 * off * (1 + spread) + E * (2 + lnv) + 4 * U * (lnv + 1), "entropy")
+    ok = (t >= 0) & (t < vocab)
+    at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
+    close(out["logp"], torch.where(ok, at, torch.zeros_like(at)), 2 * off + E + 4 * U * (lnv + at.abs()), "logp")
+
+
+@pytest.mark.parametrize("rows,dim,vocab", [(1, 8, 1), (1, 64, 2), (2, 512, 6400), (7, 72, 300), (8, 2048, 32000), (9, 520, 1000),
+                                            (33, 200, 257), (128, 128, 640), (129, 512, 255), (256, 64, 256), (257, 576, 513),
+                                            (300, 1032, 1025), (1000, 512, 6400), (5000, 64, 130), (40, 264, 20011), (1, 1000, 100003)])
+def test_linear_logprobs_sizes(L, rows, dim, vocab):
+    g = torch.Generator(device="cuda").manual_seed(rows + dim)
+    h = torch.randn(rows, dim, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(vocab, dim, device="cuda", generator=g) * (2.5 / math.sqrt(dim))).bfloat16()
+    check_head(L, h, w)
+    check_head(L, h, w, 0.6)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_linear_logprobs_values(L, rows):
+    """Large logits (every row nearly certain), equal logits, and targets at the edges of the tiles."""
+    dim, vocab = 136, 1500
+    g = torch.Generator(device="cuda").manual_seed(2)
+    h = torch.randn(rows, dim, device="cuda", generator=g).bfloat16()
+    w = torch.randn(vocab, dim, device="cuda", generator=g).bfloat16()
+    edges = torch.tensor([0, 31, 32, 127, 128, 255, 256, 1499, 1500, -5, 1023, 1024], device="cuda", dtype=torch.int32)
+    t = edges.repeat(rows // 12 + 1)[:rows].contiguous()
+    check_head(L, h * 4, w, t=t)
+    check_head(L, h * 0, w, t=t)
+    check_head(L, h, w[:1].repeat(vocab, 1).contiguous(), t=t)
+
+
+def test_linear_logprobs_agrees_with_the_stored_logits(L):
+    """On the fp32 logits that the GEMM stores from the same operands, the first operator gives the same."""
+    rows, dim, vocab = 70, 512, 6400
+    g = torch.Generator(device="cuda").manual_seed(8)
+    h = torch.randn(rows, dim, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(vocab, dim, device="cuda", generator=g) * 0.1).bfloat16()
+    x = torch.empty(rows, vocab, device="cuda")
+    e = L.Epilogue()
+    L.call("zl_gemm_bf16", h.data_ptr(), w.data_ptr(), x.data_ptr(), rows, vocab, dim, L.A_KMAJOR | L.B_KMAJOR, L.EPI_OUT_F32,
+           C.byref(e), None, stream())
+    t = targets_for(rows, vocab)
+    a, _, _ = call_logprobs(L, x, "f32", t, 1.0, 0)
+    b = call_head(L, h, w, t, 1.0)
+    off = 4 * (dim / 16 + 4) * U * float((h.double().abs() @ w.double().abs().T).amax())
+    for n in a:
+        assert float((a[n] - b[n]).abs().max()) < 12 * (off + err(vocab, "f32") + 40 * U)
+
+
+def test_linear_logprobs_graph_replay(L):
+    rows, dim, vocab = 200, 256, 5000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    hs = [torch.randn(rows, dim, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    w = (torch.randn(vocab, dim, device="cuda", generator=g) * 0.1).bfloat16()
+    t = targets_for(rows, vocab)
+    want = [call_head(L, h, w, t, 1.0) for h in hs]
+    h = hs[0].clone()
+    out = {n: torch.zeros(rows, device="cuda") for n in ("logp", "entropy", "lse")}
+    ws = torch.empty(L.load().zl_linear_logprobs_workspace_floats(rows, dim, vocab), device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        L.call("zl_linear_logprobs_bf16", h.data_ptr(), w.data_ptr(), t.data_ptr(), rows, dim, vocab, 1.0, out["logp"].data_ptr(),
+               out["entropy"].data_ptr(), out["lse"].data_ptr(), ws.data_ptr(), stream())
+    for z, a in zip(hs, want):
+        h.copy_(z)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out[n], a[n]) for n in out)

@@ -93,3 +93,33 @@ def test_distill_refusals(L, t):
     refused(L, n, bad, "element boundary", *args(d=A + 1))
     refused(L, n, bad, "row stride", *args(d=A, ds=104))
     refused(L, n, bad, "loss_rows", *args(lr=None))
+
+
+def test_linear_logprobs_refusals(L):
+    n = "zl_linear_logprobs_bf16"
+
+    def args(h=A, w=A, tg=A, rows=4, dim=64, vocab=100, scale=1.0, logp=A, ws=A):
+        return (h, w, tg, rows, dim, vocab, scale, logp, A, A, ws, None)
+
+    bad = L.ZL_EINVAL
+    refused(L, n, bad, "sizes", *args(rows=-1))
+    refused(L, n, bad, "sizes", *args(dim=0))
+    refused(L, n, bad, "sizes", *args(vocab=0))
+    refused(L, n, L.ZL_EUNSUPPORTED, "dim", *args(dim=60))
+    refused(L, n, bad, "scale", *args(scale=math.nan))
+    refused(L, n, bad, "targets", *args(tg=None))
+    refused(L, n, bad, "null", *args(ws=None))
+    refused(L, n, bad, "null", *args(h=None))
+    refused(L, n, bad, "aligned", *args(w=A + 8))
+    refused(L, n, bad, "aligned", *args(ws=A + 4))
+    assert getattr(L.load(), n)(*args(rows=0, h=None, w=None, ws=None)) == L.ZL_OK
+
+
+def test_linear_logprobs_workspace(L):
+    """A partial (four floats, two column halves) of every row for each pair that can meet its row tile: at least
+    one, no more than the vocabulary has tiles of 256 (one more where segments do not begin with the row tile)."""
+    f = L.load().zl_linear_logprobs_workspace_floats
+    for rows, vocab in [(1, 1), (1, 32000), (300, 6400), (32768, 6400), (16384, 32000)]:
+        n = f(rows, 512, vocab)
+        assert n % (rows * 8) == 0 and 1 <= n // (rows * 8) <= (vocab + 255) // 256 + 1
+    assert f(0, 512, 100) == 0

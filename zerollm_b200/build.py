@@ -18,13 +18,14 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-ccbin", "g++",
          "-I", os.path.join(ROOT, "include"), "-I", CSRC, "--expt-relaxed-constexpr"]
-SOURCES = ["kernels.cu", "logprobs.cu", "gemm.cu", "attention.cu", "attention_tc.cu", "model.cu", "dist.cu", "loader.cu"]
+SOURCES = ["kernels.cu", "logprobs.cu", "head_logprobs.cu", "gemm.cu", "attention.cu", "attention_tc.cu", "model.cu", "dist.cu", "loader.cu"]
 
 
 def _compile(src: str, verbose: bool) -> str:
     obj = os.path.join(OUT_DIR, os.path.splitext(src)[0] + ".o")
     srcp = os.path.join(CSRC, src)
-    deps = [srcp, os.path.join(CSRC, "common.cuh"), os.path.join(ROOT, "include", "zerollm_b200.h")]
+    deps = [srcp, os.path.join(ROOT, "include", "zerollm_b200.h"),
+            *(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh"))]
     if os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     cmd = [NVCC, *ARCH, *FLAGS, "-c", srcp, "-o", obj]

@@ -1,0 +1,310 @@
+// head_logprobs.cu -- log probabilities of given tokens straight from hidden states and the output head's
+// weight: logits = hidden weight^T stay in tensor memory, where each tile's epilogue folds them into the
+// running softmax statistics of its rows.  Neither logits nor probabilities reach device memory (the
+// reference's head writes them, zerollm.cpp:150-195).
+//
+// A CTA pair (cta_group::2) computes tiles of 256 rows x 256 vocabulary entries as the pair GEMM does
+// (gemm.cu): each CTA loads its 128 rows of hidden and its half of the weight tile by TMA, the even CTA
+// issues the products for both, each CTA's eight epilogue warps read their 128 x 256 half of the accumulator
+// (two in tensor memory, so products and epilogue overlap).  A thread keeps (m, S0, S1, target logit) of one
+// row and half of the tile's columns over the consecutive tiles of a work segment and writes them once, as a
+// partial; a second small kernel joins a row's partials in a fixed order.
+#include <algorithm>
+#include <atomic>
+#include <cstdio>
+
+#include "logprobs.cuh"
+
+namespace zl {
+int sm_count_current();  // gemm.cu
+bool make_tma_map(CUtensorMap* map, const void* ptr, bool is_f32, uint64_t inner, uint64_t rows, uint32_t box_inner,
+                  uint32_t box_rows, int swizzle_bytes, uint64_t row_stride);
+
+namespace {
+constexpr int BM = 128, BN = 256, BK = 64;   // rows of a CTA, vocabulary entries of a tile, reduction block
+constexpr int kEpiWarps = 8, kThreads = 64 + kEpiWarps * 32;
+constexpr int kStages = 6;
+constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of the weight, in one stage
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kBarOff = kStages * kStageBytes;
+constexpr int kSmem = kBarOff + 256 + 1024;  // barriers, alignment slack
+
+// Work: (row tile, vocabulary tile) steps, row tile by row tile; pair p takes the steps [p per, (p + 1) per).
+// A row tile's steps fall to the pairs first .. last, each of which writes one partial (slot p - first).
+int pair_slots();  // CTA pairs that the current device runs at once
+
+struct Plan {
+  int row_tiles, n_tiles, pairs, slots;
+  int64_t steps, per;
+};
+Plan make_plan(int rows, int vocab) {
+  Plan p;
+  p.row_tiles = (rows + 2 * BM - 1) / (2 * BM);
+  p.n_tiles = (vocab + BN - 1) / BN;
+  p.steps = (int64_t)p.row_tiles * p.n_tiles;
+  p.pairs = (int)std::min<int64_t>(p.steps, pair_slots());
+  p.per = p.pairs ? (p.steps + p.pairs - 1) / p.pairs : 0;
+  p.slots = p.per ? (int)std::min<int64_t>(p.pairs, (p.n_tiles - 1) / p.per + 2) : 0;
+  return p;
+}
+
+struct HeadArgs {
+  const int32_t* targets;
+  int rows, vocab, k_blocks, n_tiles, slots;
+  int64_t steps, per;
+  float c;  // scale * log2(e)
+  float4* partials;  // [row][slot][half] (m, S0, S1, target logit)
+};
+
+__global__ void __launch_bounds__(kThreads, 1)
+    head_logprobs_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
+                         const HeadArgs a) {
+  constexpr uint32_t IDESC = make_idesc(1, 2 * BM, BN, 0, 0);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int64_t s0 = (int64_t)(blockIdx.x >> 1) * a.per, s1 = min(a.steps, s0 + a.per);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kEpiWarps * 32); }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmH);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_holder, 2 * BN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();  // barriers of both CTAs initialised, tensor memory allocated in both
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t s = s0; s < s1 && ok; ++s) {
+        const int m0 = (int)(s / a.n_tiles) * (2 * BM) + (int)rank * BM;
+        const int n0 = (int)(s % a.n_tiles) * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < a.k_blocks; ++kb) {
+          if (!bounded_wait(&empty[stage], phase ^ 1u, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
+          uint8_t* sA = smem + stage * kStageBytes;
+          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);  // the even CTA's barrier
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kStageBytes);
+          tma_load_2d_pair(sA, &tmH, bar, kb * BK, m0);
+          tma_load_2d_pair(sA + kTileBytes, &tmW, bar, kb * BK, n0);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer (even CTA only)
+    if (leader) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t s = s0; s < s1 && ok; ++s) {
+        // both CTAs' epilogues have drained accumulator `acc`
+        if (!__all_sync(0xffffffffu, bounded_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, DEV_TIMEOUT_ACC))) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+        for (int kb = 0; kb < a.k_blocks; ++kb) {
+          if (!bounded_wait_warp(&full[stage], phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(smem + stage * kStageBytes), b_base = a_base + kTileBytes;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma_f16_pair_w(d_tmem, smem_desc_sw128(a_base + k * 32, 16, 1024), smem_desc_sw128(b_base + k * 32, 16, 1024),
+                            IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit_pair_w(&empty[stage], 0x3);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit_pair_w(&acc_full[acc], 0x3);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else {
+    // ------------------------------------------------ epilogue (both CTAs, own half of the rows)
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t acc_empty_leader[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    Stats st;
+    float xt = 0.f;
+    int row = 0, t = -1;
+    for (int64_t s = s0; s < s1; ++s) {
+      const int rt = (int)(s / a.n_tiles), nt = (int)(s % a.n_tiles);
+      if (s == s0 || nt == 0) {  // a segment begins
+        row = rt * (2 * BM) + (int)rank * BM + quarter * 32 + lane;
+        t = (a.targets && row < a.rows) ? a.targets[row] : -1;
+        st = Stats();
+        xt = 0.f;
+      }
+      if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
+#pragma unroll 1
+      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+        uint32_t u[32];
+        tmem_ld32(t_row + (uint32_t)c, u);
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
+        const int n = nt * BN + c;
+        if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
+        }
+        if (t >= n && t < n + 32 && t < a.vocab) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
+        }
+        st.add(v, a.c);
+      }
+      tc_fence_before();
+      mbar_arrive_cluster(acc_empty_leader[acc]);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      if ((s + 1 == s1 || nt + 1 == a.n_tiles) && row < a.rows) {  // it ends: this pair's partial of the row
+        const int slot = (int)((int64_t)(blockIdx.x >> 1) - (int64_t)rt * a.n_tiles / a.per);
+        a.partials[((int64_t)row * a.slots + slot) * 2 + half] = make_float4(st.m, st.s0, st.s1, xt);
+      }
+    }
+  }
+  // The even CTA's products read both CTAs' shared memory and write both tensor memories: neither CTA may
+  // leave (or free its tensor memory) before both are done.
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * BN);
+  }
+}
+
+cudaLaunchConfig_t pair_config(int pairs, cudaStream_t st, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = 2;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+int pair_slots() {
+  static std::atomic<int> found[64];
+  const int sms = std::max(1, sm_count_current() / 2);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return sms;  // no device: the plan of a full one
+  }
+  int n = found[dev].load();
+  if (n == 0) {
+    cudaLaunchAttribute attr;
+    cudaLaunchConfig_t cfg = pair_config(sms, nullptr, &attr);
+    if (cudaFuncSetAttribute(head_logprobs_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, head_logprobs_kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return sms;
+    }
+    n = std::min(n, sms);
+    found[dev].store(n);
+  }
+  return n;
+}
+
+// One warp per row: its partials joined in a fixed order.
+__global__ void __launch_bounds__(256) head_join_kernel(const HeadArgs a, float scale, float* __restrict__ logp,
+                                                        float* __restrict__ entropy, float* __restrict__ lse) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  const int64_t rt = row / (2 * BM);
+  const int n = 2 * (int)(((rt + 1) * a.n_tiles - 1) / a.per - rt * a.n_tiles / a.per + 1);
+  Stats s;
+  float xt = 0.f;
+  for (int i = lane; i < n; i += 32) {
+    const float4 p = a.partials[(int64_t)row * a.slots * 2 + i];
+    Stats o;
+    o.m = p.x; o.s0 = p.y; o.s1 = p.z;
+    s.join(o, a.c);
+    xt += p.w;
+  }
+  s.join_warp(a.c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) xt += __shfl_xor_sync(0xffffffffu, xt, o);
+  if (lane) return;
+  const float ln_s0 = logf(s.s0), h = fmaf(-kLn2, s.s1 / s.s0, ln_s0);
+  const int t = a.targets ? a.targets[row] : -1;
+  if (lse) lse[row] = s.s0 == 0.f ? -INFINITY : fmaf(s.m, scale, ln_s0);
+  if (entropy) entropy[row] = (s.s0 == 0.f || h < 0.f) ? 0.f : h;
+  if (logp) logp[row] = (t >= 0 && t < a.vocab) ? log_prob(xt, s, ln_s0, scale) : 0.f;
+}
+}  // namespace
+
+int head_dev_error_read_and_clear() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, zl_dev_error, sizeof(int));
+  if (v) {
+    int z = 0;
+    cudaMemcpyToSymbol(zl_dev_error, &z, sizeof(int));
+  }
+  return v;
+}
+}  // namespace zl
+
+// ============================================================== C ABI
+using namespace zl;
+
+extern "C" int64_t zl_linear_logprobs_workspace_floats(int rows, int dim, int vocab) {
+  if (rows <= 0 || dim <= 0 || vocab <= 0) return 0;
+  return (int64_t)rows * make_plan(rows, vocab).slots * 8;
+}
+
+extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf16* weight, const int32_t* targets, int rows,
+                                             int dim, int vocab, float scale, float* logp, float* entropy, float* lse,
+                                             float* workspace, zl_stream stream) {
+  const char* what = "linear_logprobs";
+  if (rows < 0 || dim <= 0 || vocab <= 0) return set_error(ZL_EINVAL, "%s: sizes must be positive", what);
+  if (dim % 8) return set_error(ZL_EUNSUPPORTED, "%s: dim %% 8 != 0", what);
+  if (bad_scale(scale)) return set_error(ZL_EINVAL, "%s: scale must be in [1e-4, 1e4]", what);
+  if (logp && !targets) return set_error(ZL_EINVAL, "%s: log probabilities need targets", what);
+  if (rows == 0) return ZL_OK;
+  if (!hidden || !weight || !workspace) return set_error(ZL_EINVAL, "%s: null hidden, weight or workspace", what);
+  if ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(workspace)) & 15)
+    return set_error(ZL_EINVAL, "%s: hidden, weight and workspace must be 16-byte aligned", what);
+  const Plan p = make_plan(rows, vocab);
+  CUtensorMap mh, mw;
+  if (!make_tma_map(&mh, hidden, false, dim, rows, BK, BM, 128, 0) ||
+      !make_tma_map(&mw, weight, false, dim, vocab, BK, BN / 2, 128, 0))
+    return set_error(ZL_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
+  HeadArgs a{targets, rows, vocab, (dim + BK - 1) / BK, p.n_tiles, p.slots, p.steps, p.per, scale * kLog2e,
+             reinterpret_cast<float4*>(workspace)};
+  cudaLaunchAttribute attr;
+  const cudaLaunchConfig_t cfg = pair_config(p.pairs, (cudaStream_t)stream, &attr);  // (make_plan has set the kernel's attribute)
+  cudaError_t e = cudaLaunchKernelEx(&cfg, head_logprobs_kernel, mh, mw, a);
+  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  head_join_kernel<<<(rows + 7) / 8, 256, 0, (cudaStream_t)stream>>>(a, scale, logp, entropy, lse);
+  return check_launch(what);
+}

@@ -12,7 +12,7 @@
 #include <cmath>
 #include <cstdint>
 
-#include "common.cuh"
+#include "logprobs.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -23,8 +23,6 @@ namespace {
 constexpr int kTopMax = 128;   // most alternatives of a row
 constexpr int kCand = 512;     // candidates ranked at once; more (long runs of equal values) go the slow way
 constexpr int kMaxParts = 8;   // blocks of a cluster that share a row
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kFloor = -1000.f;  // a log2 probability this low has p = 0; stands for -inf in products
 
 // ------------------------------------------------------------------ elements
 template <typename T> struct Elt;
@@ -62,12 +60,6 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
   return u;
 }
-__device__ __forceinline__ float ex2(float t) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
-  return r;
-}
-
 // A row as elements [0, head) before its first 16-byte boundary, nv whole vectors, and the rest [tail, V).
 // Block `part` of the `parts` that share the row takes the vectors [lo, hi); the first block takes the
 // head and the last one the rest, one element per thread.
@@ -98,57 +90,6 @@ template <typename T> struct Span {
     return v >= lo && v < hi;
   }
 };
-
-// ------------------------------------------------------------------ running softmax statistics
-// c = scale * log2(e).  A masked logit (-inf) has e = 0; its exponent is kept off -inf before it is
-// multiplied with e.  A NaN or +inf logit makes s0 and s1 NaN.
-struct Stats {
-  float m = -INFINITY, s0 = 0.f, s1 = 0.f;
-  // statistics of the same elements about the larger maximum M
-  __device__ __forceinline__ void rebase(float M, float c) {
-    const float d = m == -INFINITY ? kFloor : fmaxf((m - M) * c, kFloor);
-    const float f = ex2(d);
-    s1 = f * fmaf(d, s0, s1);
-    s0 *= f;
-    m = M;
-  }
-  template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
-    float b = v[0];
-#pragma unroll
-    for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
-    if (b > m) rebase(b, c);
-    const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float t = (v[j] - base) * c, e = ex2(t);
-      s0 += e;
-      s1 = fmaf(e, fmaxf(t, kFloor), s1);
-    }
-  }
-  __device__ __forceinline__ void join(const Stats& o, float c) {
-    Stats a = o;
-    const float M = fmaxf(m, o.m);
-    rebase(M, c);
-    a.rebase(M, c);
-    s0 += a.s0;
-    s1 += a.s1;
-  }
-  __device__ __forceinline__ void join_warp(float c) {
-    float M = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    rebase(M, c);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-    }
-  }
-};
-// ln p of a logit from a row's statistics; a row without a finite logit (s0 = 0) has ln p = -inf everywhere.
-__device__ __forceinline__ float log_prob(float x, const Stats& s, float ln_s0, float scale) {
-  return s.s0 == 0.f ? -INFINITY : fmaf(x - s.m, scale, -ln_s0);
-}
 
 // Statistics of this block's part of a row, the same in every thread (two block barriers).
 template <typename T, int NT>
@@ -677,7 +618,6 @@ zl_status launch_parts(const char* what, K kern, int64_t blocks, int threads, in
   return ZL_OK;
 }
 
-bool bad_scale(float s) { return !(s >= 1e-4f && s <= 1e4f); }
 template <typename T> bool off_element(const void* p) { return (reinterpret_cast<uintptr_t>(p) % sizeof(T)) != 0; }
 
 template <typename T>

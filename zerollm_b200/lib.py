@@ -94,6 +94,8 @@ SIGNATURES = {
        for t in ("bf16", "f32")},
     **{f"zl_distill_topk_{t}": (i32, [vp, i64, vp, vp, i32, vp, vp, C.POINTER(DistillOptions), i32, i32, vp, i64, vp, vp,
                                       vp]) for t in ("bf16", "f32")},
+    "zl_linear_logprobs_bf16": (i32, [vp, vp, vp, i32, i32, i32, f32, vp, vp, vp, vp, vp]),
+    "zl_linear_logprobs_workspace_floats": (i64, [i32, i32, i32]),
     "zl_colsum_bf16": (i32, [vp, vp, vp, i64, i32, vp]),
     "zl_linear_forward_bf16": (i32, [vp, vp, vp, vp, i64, i64, i64, i32, vp]),
     "zl_linear_backward_bf16": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]),
