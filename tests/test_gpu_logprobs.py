@@ -165,7 +165,8 @@ def check_logprobs(L, x, dtype, scale, k, targets):
 
 
 SIZES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 64), (3, 257), (6, 1000), (2, 2048), (3, 4099), (5, 6400), (2, 8193),
-         (300, 640), (1, 32000), (2, 50001), (400, 20001), (1, 150001)]
+         (300, 640), (1, 32000), (2, 50001), (400, 20001), (1, 150001),
+         (1200, 3), (1301, 100), (1200, 2049), (5000, 130), (1250, 6401), (1190, 16000), (1184, 30000), (1300, 40000)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -178,7 +179,8 @@ def test_token_logprobs_sizes(L, rows, vocab, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("kind", ["masked", "few", "lowest", "constant", "ties", "sorted", "sharp", "column"])
-@pytest.mark.parametrize("rows,vocab,k", [(3, 900, 20), (3, 6400, 16), (7, 6400, 128), (1, 33333, 50), (2, 140000, 64)])
+@pytest.mark.parametrize("rows,vocab,k", [(3, 900, 20), (3, 6400, 16), (7, 6400, 128), (1, 33333, 50), (2, 140000, 64),
+                                          (1200, 900, 20), (1201, 6400, 64), (2500, 5003, 1)])
 def test_token_logprobs_values(L, rows, vocab, k, kind, dtype):
     check_logprobs(L, make(kind, rows, vocab, dtype), dtype, 1.0, k, targets_for(rows, vocab))
 
@@ -186,7 +188,7 @@ def test_token_logprobs_values(L, rows, vocab, k, kind, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("pad,offset,scale", [(0, 1, 1.0), (8, 0, 0.7), (13, 3, 1.3), (1, 5, 0.25)])
 def test_token_logprobs_strides(L, pad, offset, scale, dtype):
-    for rows, vocab in [(4, 6), (5, 1001), (3, 6400), (2, 20000)]:
+    for rows, vocab in [(4, 6), (5, 1001), (3, 6400), (2, 20000), (1300, 1001)]:
         check_logprobs(L, make("normal", rows, vocab, dtype, pad, offset), dtype, scale, min(vocab, 9), targets_for(rows, vocab))
 
 

@@ -1040,12 +1040,13 @@ namespace zl {
 int gemm_dev_error_read_and_clear();
 int attn_tc_dev_error_read_and_clear();
 int head_dev_error_read_and_clear();
+int logprobs_dev_error_read_and_clear();
 }
 extern "C" zl_status zl_device_error(int* code_out) {
-  int v = zl::gemm_dev_error_read_and_clear();
-  const int a = zl::attn_tc_dev_error_read_and_clear();
-  const int h = zl::head_dev_error_read_and_clear();
-  if (!v) v = a ? a : h;
+  int v = 0;
+  for (const int e : {zl::gemm_dev_error_read_and_clear(), zl::attn_tc_dev_error_read_and_clear(),
+                      zl::head_dev_error_read_and_clear(), zl::logprobs_dev_error_read_and_clear()})
+    if (!v) v = e;
   if (code_out) *code_out = v;
   return v ? set_error(ZL_ETIMEOUT, "device wait timed out (code %d)", v) : ZL_OK;
 }

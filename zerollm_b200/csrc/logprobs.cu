@@ -8,6 +8,7 @@
 // over a block and, where there are few rows, over the cluster of blocks that shares a row.
 // The reference has no counterpart: its loss takes softmax probabilities (cross_entropy.cpp:23-79).
 #include <cooperative_groups.h>
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -21,7 +22,6 @@ int sm_count_current();  // gemm.cu
 
 namespace {
 constexpr int kTopMax = 128;   // most alternatives of a row
-constexpr int kCand = 512;     // candidates ranked at once; more (long runs of equal values) go the slow way
 constexpr int kMaxParts = 8;   // blocks of a cluster that share a row
 
 // ------------------------------------------------------------------ elements
@@ -74,9 +74,8 @@ template <typename T> struct Span {
     hi = (int)((int64_t)nv * (part + 1) / parts);
     tail = head + nv * VEC;
   }
-  // the element outside whole vectors that this thread has, or -1
-  __device__ int single(int V, int part, int parts) const {
-    const int t = threadIdx.x;
+  // the element outside whole vectors that thread t has, or -1
+  __device__ int single(int V, int part, int parts, int t) const {
     if (part == 0 && t < head) return t;
     if (part == parts - 1 && t >= 8 && t < 16 && tail + t - 8 < V) return tail + t - 8;
     return -1;
@@ -125,6 +124,122 @@ __device__ __forceinline__ Stats block_stats(const T* x, const Span<T>& sp, int 
   return s;
 }
 
+// ------------------------------------------------------------------ rows through shared memory
+// A row's vectors are cut into pieces of 128 (four to a lane).  A warp takes every NW-th piece and has up to
+// kDepth of them on the way from device memory (cp.async.bulk into its own ring), so that loads run on while
+// it computes, and into its next row.
+constexpr int kPieceVecs = 128, kPieceBytes = kPieceVecs * 16, kDepth = 4;
+
+// The source of a warp's pieces: rows r, r + step, ... of the matrix, of each the pieces first, first + NW, ...
+// of the part [lo, hi) of its vectors.
+template <typename T, int NW> struct Feed {
+  const T* base;
+  int64_t stride;
+  int rows, V, part, parts, first, row_step;
+  int64_t row;
+  const uint8_t* src;
+  int left;  // vectors from src to the end of the part
+  uint32_t issued;
+  uint8_t* buf;
+  uint64_t* bar;
+  __device__ void open() {
+    for (left = 0; row < rows; row += row_step) {
+      const T* x = base + row * stride;
+      const Span<T> sp(x, V, part, parts);
+      left = sp.hi - sp.lo - first * kPieceVecs;
+      src = reinterpret_cast<const uint8_t*>(x + sp.head) + (int64_t)(sp.lo + first * kPieceVecs) * 16;
+      if (left > 0) return;
+    }
+    left = 0;
+  }
+  // the next piece on its way (one lane copies); nothing once the rows are through
+  __device__ __forceinline__ void issue(int lane) {
+    if (left <= 0) return;
+    const uint32_t s = issued % kDepth;
+    const uint32_t bytes = min(left, kPieceVecs) * 16;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bar[s], bytes);
+      bulk_copy_g2s(buf + s * kPieceBytes, src, bytes, &bar[s]);
+    }
+    ++issued;
+    left -= NW * kPieceVecs;
+    src += NW * kPieceBytes;
+    if (left <= 0) {
+      row += row_step;
+      open();
+    }
+  }
+};
+
+// A lane's four vectors of a consumed piece; those past its end are -inf.
+template <typename T, int NW>
+__device__ __forceinline__ void take_piece(Feed<T, NW>& feed, uint32_t n, int vecs, int lane, uint4 (&u)[4]) {
+  const uint32_t s = n % kDepth;
+  bounded_wait(&feed.bar[s], (n / kDepth) & 1u, DEV_TIMEOUT_FULL);  // (a lost copy: its error is recorded, nobody hangs)
+  const uint4* p = reinterpret_cast<const uint4*>(feed.buf + s * kPieceBytes) + lane;
+  constexpr uint32_t NI = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) u[j] = j * 32 + lane < vecs ? p[j * 32] : make_uint4(NI, NI, NI, NI);
+  __syncwarp();
+  feed.issue(lane);
+}
+
+// Maxima of a lane's four vectors, NaN aside.
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T> struct Maxima;
+template <> struct Maxima<__nv_bfloat16> {
+  using Store = uint2;
+  uint2 m{0xff80ff80u, 0xff80ff80u};
+  __device__ __forceinline__ Store take(const uint4 (&u)[4]) {
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = max2(max2(u[j].x, u[j].y), max2(u[j].z, u[j].w));
+    const uint2 v = make_uint2(max2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[0], h[1], 0x7632)),
+                               max2(__byte_perm(h[2], h[3], 0x5410), __byte_perm(h[2], h[3], 0x7632)));
+    m.x = max2(m.x, v.x);
+    m.y = max2(m.y, v.y);
+    return v;
+  }
+  static __device__ __forceinline__ float4 values(const Store& v) {
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                       __uint_as_float(v.y & 0xffff0000u));
+  }
+  __device__ __forceinline__ float4 all() const { return values(m); }
+};
+template <> struct Maxima<float> {
+  using Store = float4;
+  float4 m{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  static __device__ __forceinline__ float of(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  __device__ __forceinline__ Store take(const uint4 (&u)[4]) {
+    const float4 v = make_float4(of(u[0]), of(u[1]), of(u[2]), of(u[3]));
+    m = make_float4(fmaxf(m.x, v.x), fmaxf(m.y, v.y), fmaxf(m.z, v.z), fmaxf(m.w, v.w));
+    return v;
+  }
+  static __device__ __forceinline__ float4 values(const Store& v) { return v; }
+  __device__ __forceinline__ float4 all() const { return m; }
+};
+// A lane's four vectors, their maximum known.
+template <typename T> __device__ __forceinline__ void add_piece(Stats& s, const uint4 (&u)[4], float most, float c) {
+  constexpr int VEC = Elt<T>::VEC;
+  if (most > s.m) s.rebase(most, c);
+  float f[4 * VEC];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float e[VEC];
+    Elt<T>::unpack(u[j], e);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[j * VEC + i] = e[i];
+  }
+  s.add_below(f, c);
+}
+__device__ __forceinline__ float max_of(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+
 // ------------------------------------------------------------------ top alternatives
 // Order-preserving key: larger values have larger keys, -0 and +0 the same one, NaN the lowest (0).
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -136,199 +251,308 @@ constexpr uint32_t kKeyMasked = 0x007fffffu;  // of -inf
 __device__ __forceinline__ float key_value(uint32_t k) {
   return k == 0u ? __uint_as_float(0x7fffffffu) : __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
+// key of a maximum: -inf may stand for -inf, for NaN or for no element at all, so it is below every bound
+__device__ __forceinline__ uint32_t max_key(float m) { return m == -INFINITY ? 0u : order_key(m); }
 // A candidate: larger key first, then the lower index.
 __device__ __forceinline__ unsigned long long candidate(uint32_t key, int i) {
   return ((unsigned long long)key << 32) | (0xffffffffu - (uint32_t)i);
 }
 
-struct TopShared {
-  unsigned long long cand[kCand];
-  uint32_t group[256];
-  int col[256];
-  int n, ncol;
-  uint32_t tau;
+// Threads of the NW warps that share a row (or a part of one).
+template <int NW> __device__ __forceinline__ void team_sync() {
+  if (NW == 1) __syncwarp();
+  else __syncthreads();
+}
+template <int NW> __device__ __forceinline__ int team_thread() { return NW == 1 ? (threadIdx.x & 31) : threadIdx.x; }
+
+template <int NW> struct TopShared {
+  static constexpr int CAP = NW == 1 ? 256 : 512;  // candidates ranked at once; more go the slow way
+  static constexpr int GROUPS = NW == 1 ? 128 : 256;
+  unsigned long long cand[CAP];
+  int vec[CAP];
+  uint32_t group[NW == 1 ? 1 : GROUPS];
+  int slots[NW];
+  int n, nvec;
 };
 
-// Count of the row's elements with key >= k, the same in every thread (one block, the whole row).
-template <typename T, int NT>
-__device__ int count_from(const T* x, int V, uint32_t k, int* slots) {
-  int n = 0;
-  for (int i = threadIdx.x; i < V; i += NT) n += order_key(Elt<T>::get(x + i)) >= k;
+// The largest t whose bits below bit LO are those of `low` such that at least k of the warp's keys (R to a lane)
+// are >= t, given that at least k are >= t0 (whose bits from HI down are 0).
+template <int R> __device__ __forceinline__ uint32_t kth_key(const uint32_t (&g)[R], int k, uint32_t t0, int hi, int lo) {
+  uint32_t tau = t0;
+#pragma unroll 1
+  for (int b = hi; b >= lo; --b) {
+    const uint32_t t = tau | (1u << b);
+    int n = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    for (int i = 0; i < R; ++i) n += g[i] >= t;
+    if (__reduce_add_sync(0xffffffffu, n) >= k) tau = t;
+  }
+  return tau;
+}
+
+// Appends a value of each lane that has one; n counts them all, those past CAP are dropped.
+template <typename V> __device__ __forceinline__ void push(bool yes, V v, V* list, int* n, int cap) {
+  const uint32_t vote = __ballot_sync(0xffffffffu, yes);
+  if (vote == 0) return;
+  const int lane = threadIdx.x & 31, first = __ffs(vote) - 1;
+  int at = 0;
+  if (lane == first) at = atomicAdd(n, __popc(vote));
+  at = __shfl_sync(0xffffffffu, at, first) + __popc(vote & ((1u << lane) - 1u));
+  if (yes && at < cap) list[at] = v;
+}
+
+// Count of the row's elements with key >= t, the same in every thread of the team.
+template <typename T, int NW> __device__ int count_from(const T* x, int V, uint32_t t, TopShared<NW>& sh) {
+  int n = 0;
+#pragma unroll 4
+  for (int i = team_thread<NW>(); i < V; i += NW * 32) n += order_key(Elt<T>::get(x + i)) >= t;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (NW == 1) return n;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = n;
+  if ((threadIdx.x & 31) == 0) sh.slots[threadIdx.x >> 5] = n;
   __syncthreads();
   n = 0;
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) n += slots[w];
+  for (int w = 0; w < NW; ++w) n += sh.slots[w];
   return n;
 }
 
-// The candidates of a row in which more than kCand elements are at least tau (long runs of equal values:
-// masked vocabularies, constant rows): the exact key K of the k-th largest element, every element above it
-// (fewer than k) and the lowest-indexed ones equal to it.
-template <typename T, int NT>
-__device__ void select_slow(const T* x, int V, int k, uint32_t tau, TopShared& sh, int* slots) {
-  if (tau == 0 && count_from<T, NT>(x, V, kKeyMasked, slots) >= k) tau = kKeyMasked;
-  uint32_t K = tau;
-  if (tau != 0xffffffffu && count_from<T, NT>(x, V, tau + 1, slots) >= k) {
-    K = 0;
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t t = K | (1u << b);
-      if (count_from<T, NT>(x, V, t, slots) >= k) K = t;
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < V; i += NT) {
-    const uint32_t q = order_key(Elt<T>::get(x + i));
-    if (q > K) sh.cand[atomicAdd(&sh.n, 1)] = candidate(q, i);
-  }
-  __syncthreads();
-  int n = sh.n;  // < k <= kTopMax
-  // equal ones in index order, NT elements at a time
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int i0 = 0; i0 < V && n < k; i0 += NT) {
-    const int i = i0 + threadIdx.x;
+// Appends to the n candidates the lowest-indexed elements of key K, up to k candidates; returns their number.
+template <typename T, int NW> __device__ int append_equal(const T* x, int V, uint32_t K, int n, int k, TopShared<NW>& sh) {
+  const int tid = team_thread<NW>(), lane = tid & 31, w = tid >> 5;
+  for (int i0 = 0; i0 < V && n < k; i0 += NW * 32) {
+    const int i = i0 + tid;
     const bool eq = i < V && order_key(Elt<T>::get(x + i)) == K;
     const uint32_t vote = __ballot_sync(0xffffffffu, eq);
-    __syncthreads();
-    if (lane == 0) slots[w] = __popc(vote);
-    __syncthreads();
-    int at = n, all = 0;
+    int at = n, all = __popc(vote);
+    if (NW > 1) {
+      __syncthreads();
+      if (lane == 0) sh.slots[w] = all;
+      __syncthreads();
+      all = 0;
 #pragma unroll
-    for (int j = 0; j < NT / 32; ++j) {
-      if (j < w) at += slots[j];
-      all += slots[j];
+      for (int j = 0; j < NW; ++j) {
+        if (j < w) at += sh.slots[j];
+        all += sh.slots[j];
+      }
     }
     at += __popc(vote & ((1u << lane) - 1u));
     if (eq && at < k) sh.cand[at] = candidate(K, i);
     n = min(k, n + all);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.n = n;
-  __syncthreads();
+  team_sync<NW>();
+  return n;
+}
+
+// The candidates of a row in which more than CAP elements reach the bound (long runs of equal values, as in
+// constant rows and rows masked with a finite value): every element above the key K of the k-th largest one
+// (fewer than k), then the lowest-indexed ones equal to it.  tau: the k-th largest group maximum, so K >= tau,
+// and K = tau unless k elements are above it.
+template <typename T, int NW> __device__ int select_slow(const T* x, int V, int k, uint32_t tau, TopShared<NW>& sh) {
+  uint32_t K = tau;
+  if (count_from<T, NW>(x, V, tau + 1, sh) >= k) {
+    K = 0;
+#pragma unroll 1
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t t = K | (1u << b);
+      if (count_from<T, NW>(x, V, t, sh) >= k) K = t;
+    }
+  }
+  team_sync<NW>();
+  if (team_thread<NW>() == 0) sh.n = 0;
+  team_sync<NW>();
+#pragma unroll 4
+  for (int i = team_thread<NW>(); i < V; i += NW * 32) {
+    const uint32_t q = order_key(Elt<T>::get(x + i));
+    if (q > K) sh.cand[atomicAdd(&sh.n, 1)] = candidate(q, i);
+  }
+  team_sync<NW>();
+  const int n = sh.n;
+  team_sync<NW>();
+  return append_equal<T, NW>(x, V, K, n, k, sh);
 }
 
 struct LogprobArgs {
   const void* logits;
   int64_t stride;
   const int32_t* targets;
-  int rows, vocab, k, groups, parts;
+  int rows, vocab, k, parts, pieces;  // pieces: most of a part
   float scale;
   float *logp, *entropy, *lse, *top_logp;
   int32_t* top_ids;
 };
+// dynamic shared memory: rings, then per team the vectors' maxima
+template <typename T, int NW, int TEAMS> size_t logprobs_smem(const LogprobArgs& a) {
+  return (size_t)NW * TEAMS * kDepth * kPieceBytes +
+         (a.k ? (size_t)TEAMS * a.pieces * 32 * sizeof(typename Maxima<T>::Store) : 0);
+}
 
-// One row per block, or per cluster of `parts` blocks.  Top alternatives: the k-th largest of the maxima of
-// `groups` disjoint sets of elements (a thread's elements, or those of some neighbouring threads) is a bound
-// tau that at least k elements reach; only threads whose own maximum reaches it have candidates, and a warp
-// reads such a thread's elements again (from L2).  For values in any order about k * 1.15 elements reach tau.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobArgs a) {
-  constexpr int VEC = Elt<T>::VEC, NW = NT / 32;
-  __shared__ Stats red[NW];
-  __shared__ Stats parts_st[kMaxParts];
-  __shared__ int slots[NW];
-  __shared__ TopShared sh;
+// NW warps to a row (TEAMS rows to a block), or a cluster of `parts` blocks of NW warps.  Top alternatives: the
+// k-th largest of the maxima of 128 (one warp) or 256 disjoint sets of elements is a bound that at least k
+// elements reach, about 1.15 k of them where values come in any order; the maxima of the single vectors, kept
+// in shared memory, say which vectors to read again (from L2).  Few candidates are left, whose ranks are counted.
+template <typename T, int NW, int TEAMS>
+__global__ void __launch_bounds__(NW * TEAMS * 32) logprobs_kernel(const LogprobArgs a) {
+  constexpr int VEC = Elt<T>::VEC, GROUPS = TopShared<NW>::GROUPS, CAP = TopShared<NW>::CAP;
+  using Store = typename Maxima<T>::Store;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ TopShared<NW> top[TEAMS];
+  __shared__ Stats red[NW], parts_st[kMaxParts];
+  __shared__ uint64_t bars[NW * TEAMS * kDepth];
+  static_assert(NW == 1 || TEAMS == 1, "a block barrier serves one team");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = NW == 1 ? warp : 0, tid = team_thread<NW>();
   const int parts = a.parts, part = parts > 1 ? (int)(blockIdx.x % parts) : 0;
-  const int64_t r = blockIdx.x / parts;
-  const int V = a.vocab, tid = threadIdx.x, lane = tid & 31;
-  const T* x = static_cast<const T*>(a.logits) + r * a.stride;
+  const int V = a.vocab, k = a.k;
   const float c = a.scale * kLog2e;
-  const Span<T> sp(x, V, part, parts);
-  const int single = sp.single(V, part, parts);
-  if (tid == 0) { sh.n = 0; sh.ncol = 0; }
-  if (parts > 1) cg::this_cluster().barrier_arrive();
-  float tmax;
-  Stats s = block_stats<T, NT>(x, sp, single, c, tmax, red);
-  // a maximum of -inf may stand for -inf, for NaN or for no element at all: below every bound
-  const uint32_t tkey = tmax == -INFINITY ? 0u : order_key(tmax);
-  if (parts > 1) cg::this_cluster().barrier_wait();  // every block of the cluster runs: its shared memory may be written
-  if (a.k > 0) {
-    // NT * parts / groups threads to a group (a power of two, at most 32)
-    const int per = NT * parts / a.groups;
-    uint32_t g = tkey;
-    for (int o = per >> 1; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if ((tid & (per - 1)) == 0) {
-      const int at = part * (a.groups / parts) + tid / per;
-      if (parts == 1) sh.group[at] = g;
-      else
-        for (int q = 0; q < parts; ++q) *cg::this_cluster().map_shared_rank(&sh.group[at], q) = g;
-    }
-  }
-  if (parts > 1) {
-    if (tid < parts) *cg::this_cluster().map_shared_rank(&parts_st[part], tid) = s;
-    cg::this_cluster().sync();
-    s = parts_st[0];
-    for (int q = 1; q < parts; ++q) s.join(parts_st[q], c);
-  } else {
-    __syncthreads();
-  }
-  const float ln_s0 = logf(s.s0);
-  if (part == 0 && tid == 0) {
-    const int t = a.targets ? a.targets[r] : -1;
-    const float h = fmaf(-kLn2, s.s1 / s.s0, ln_s0);
-    if (a.lse) a.lse[r] = s.s0 == 0.f ? -INFINITY : fmaf(s.m, a.scale, ln_s0);
-    if (a.entropy) a.entropy[r] = (s.s0 == 0.f || h < 0.f) ? 0.f : h;
-    if (a.logp) a.logp[r] = (t >= 0 && t < V) ? log_prob(Elt<T>::get(x + t), s, ln_s0, a.scale) : 0.f;
-  }
-  if (a.k == 0) return;
+  TopShared<NW>& sh = top[team];
+  Store* vmax = reinterpret_cast<Store*>(dyn + NW * TEAMS * kDepth * kPieceBytes) + (int64_t)team * a.pieces * 32;
+  const int64_t row0 = parts > 1 ? blockIdx.x / parts : (int64_t)blockIdx.x * TEAMS + team;
+  const int row_step = parts > 1 ? (int)(gridDim.x / parts) : (int)gridDim.x * TEAMS;
 
-  // tau: the k-th largest group maximum, bit by bit over one warp's ballots
-  if (tid < 32) {
-    uint32_t g[8], tau = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = i * 32 + lane < a.groups ? sh.group[i * 32 + lane] : 0u;
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t t = tau | (1u << b);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i * 32 < a.groups) n += __popc(__ballot_sync(0xffffffffu, g[i] >= t));
-      if (n >= a.k) tau = t;
-    }
-    if (lane == 0) sh.tau = tau;
+  Feed<T, NW> feed;
+  feed.base = static_cast<const T*>(a.logits);
+  feed.stride = a.stride;
+  feed.rows = a.rows; feed.V = V; feed.part = part; feed.parts = parts;
+  feed.first = NW == 1 ? 0 : warp;
+  feed.row_step = row_step; feed.row = row0; feed.issued = 0;
+  feed.buf = dyn + warp * kDepth * kPieceBytes;
+  feed.bar = bars + warp * kDepth;
+  if (lane == 0) {
+    for (int i = 0; i < kDepth; ++i) mbar_init(&feed.bar[i], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
   }
-  __syncthreads();
-  const uint32_t tau = sh.tau;
-  if (tkey >= tau) sh.col[atomicAdd(&sh.ncol, 1)] = tid;
-  TopShared& first = parts > 1 ? *cg::this_cluster().map_shared_rank(&sh, 0) : sh;
-  auto offer = [&](float f, int i) {
-    const uint32_t q = order_key(f);
-    if (q >= tau) {
-      const int n = atomicAdd(&first.n, 1);
-      if (n < kCand) first.cand[n] = candidate(q, i);
+  __syncwarp();
+  feed.open();
+  for (int i = 0; i < kDepth; ++i) feed.issue(lane);
+  if (parts > 1) cg::this_cluster().barrier_arrive();
+  uint32_t taken = 0;
+  bool entered = parts == 1;
+
+  for (int64_t r = row0; r < a.rows; r += row_step) {
+    const T* x = feed.base + r * a.stride;
+    const Span<T> sp(x, V, part, parts);
+    // the target's logit, asked for early
+    int t = -1;
+    float xt = 0.f;
+    if (a.logp && part == 0 && tid == 0) {
+      t = a.targets[r];
+      if (t >= V) t = -1;
+      if (t >= 0) xt = Elt<T>::get(x + t);
     }
-  };
-  if (single >= 0) offer(Elt<T>::get(x + single), single);
-  __syncthreads();
-  const int ncol = sh.ncol;
-  for (int i = tid >> 5; i < ncol; i += NW) {
-    for (int v = sp.lo + sh.col[i] + lane * NT; v < sp.hi; v += 32 * NT) {
-      float f[VEC];
-      Elt<T>::unpack(load16(x + sp.head + (int64_t)v * VEC), f);
+    const int single = (NW == 1 || tid < 32) ? sp.single(V, part, parts, tid) : -1;
+    const float xs = single >= 0 ? Elt<T>::get(x + single) : -INFINITY;
+    if (k > 0 && tid == 0) { sh.n = 0; sh.nvec = 0; }
+
+    Stats s;
+    Maxima<T> mx;
+    for (int v = sp.lo + (NW == 1 ? 0 : warp) * kPieceVecs, i = NW == 1 ? 0 : warp; v < sp.hi; v += NW * kPieceVecs, i += NW) {
+      uint4 u[4];
+      take_piece(feed, taken++, sp.hi - v, lane, u);
+      const Store m = mx.take(u);
+      if (k > 0) vmax[i * 32 + lane] = m;
+      add_piece<T>(s, u, max_of(Maxima<T>::values(m)), c);
+    }
+    if (single >= 0) {
+      const float f[1] = {xs};
+      s.add(f, c);
+    }
+    float4 g4 = mx.all();
+    g4.x = fmaxf(g4.x, xs);
+    s.join_warp(c);
+    if constexpr (NW > 1) {
+      if (k > 0) {  // 32 / parts groups to a warp
+        uint32_t g = max_key(max_of(g4));
+        for (int o = parts >> 1; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (!entered) { cg::this_cluster().barrier_wait(); entered = true; }  // the other blocks run: their memory may be written
+        if ((lane & (parts - 1)) == 0) {
+          const int at = (part * NW + warp) * (32 / parts) + lane / parts;
+          if (parts == 1) sh.group[at] = g;
+          else
+            for (int q = 0; q < parts; ++q) *cg::this_cluster().map_shared_rank(&sh.group[at], q) = g;
+        }
+      }
+      if (lane == 0) red[warp] = s;
+      __syncthreads();
+      s = lane < NW ? red[lane] : Stats();
+      s.join_warp(c);
+      if (parts > 1) {
+        if (!entered) { cg::this_cluster().barrier_wait(); entered = true; }
+        if (tid < parts) *cg::this_cluster().map_shared_rank(&parts_st[part], tid) = s;
+        cg::this_cluster().sync();
+        s = lane < parts ? parts_st[lane] : Stats();
+        s.join_warp(c);
+      }
+    }
+    const float ln_s0 = logf(s.s0);
+    if (part == 0 && tid == 0) {
+      const float h = fmaf(-kLn2, s.s1 / s.s0, ln_s0);
+      if (a.lse) a.lse[r] = s.s0 == 0.f ? -INFINITY : fmaf(s.m, a.scale, ln_s0);
+      if (a.entropy) a.entropy[r] = (s.s0 == 0.f || h < 0.f) ? 0.f : h;
+      if (a.logp) a.logp[r] = t >= 0 ? log_prob(xt, s, ln_s0, a.scale) : 0.f;
+    }
+    if (k > 0) {
+      if (NW == 1) __syncwarp();
+      // every warp finds the bound; fp32 keys are cut to their upper half first, a slightly lower bound
+      uint32_t g[GROUPS / 32];
+      if constexpr (NW == 1) {
+        g[0] = max_key(g4.x); g[1] = max_key(g4.y); g[2] = max_key(g4.z); g[3] = max_key(g4.w);
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) offer(f[j], sp.head + v * VEC + j);
+        for (int i = 0; i < GROUPS / 32; ++i) g[i] = sh.group[i * 32 + lane];
+      }
+      const uint32_t tau = kth_key(g, k, 0u, 31, 16);
+      const float least = tau == 0 ? -FLT_MAX : key_value(tau);  // tau = 0: every finite logit is a candidate
+      TopShared<NW>& first = parts > 1 ? *cg::this_cluster().map_shared_rank(&sh, 0) : sh;
+      push(xs >= least, candidate(order_key(xs), single), first.cand, &first.n, CAP);
+      for (int v = sp.lo + (NW == 1 ? 0 : warp) * kPieceVecs, i = NW == 1 ? 0 : warp; v < sp.hi; v += NW * kPieceVecs, i += NW) {
+        const float4 m = Maxima<T>::values(vmax[i * 32 + lane]);
+        if (__any_sync(0xffffffffu, max_of(m) >= least)) {
+          push(m.x >= least, v + lane, sh.vec, &sh.nvec, CAP);
+          push(m.y >= least, v + 32 + lane, sh.vec, &sh.nvec, CAP);
+          push(m.z >= least, v + 64 + lane, sh.vec, &sh.nvec, CAP);
+          push(m.w >= least, v + 96 + lane, sh.vec, &sh.nvec, CAP);
+        }
+      }
+      team_sync<NW>();
+      const int nvec = sh.nvec;
+      for (int i0 = warp * 32 * (NW > 1); i0 < min(nvec, CAP); i0 += NW * 32) {
+        float f[VEC];
+        int at = -1;
+        if (i0 + lane < nvec) {
+          at = sp.head + sh.vec[i0 + lane] * VEC;
+          Elt<T>::unpack(load16(x + at), f);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) push(at >= 0 && f[j] >= least, candidate(order_key(f[j]), at + j), first.cand, &first.n, CAP);
+      }
+      if (nvec > CAP && tid == 0) atomicAdd(&first.n, CAP);  // vectors were dropped: the slow way
+      if (parts > 1) cg::this_cluster().sync();
+      else team_sync<NW>();
+      if (part == 0) {
+        int n = sh.n;
+        team_sync<NW>();
+        if (n > CAP) {
+          n = select_slow<T, NW>(x, V, k, kth_key(g, k, tau, 15, 0), sh);
+        } else if (n < k) {  // (tau = 0) masked logits, then NaN ones, by their index
+          n = append_equal<T, NW>(x, V, kKeyMasked, n, k, sh);
+          n = append_equal<T, NW>(x, V, 0u, n, k, sh);
+        }
+        for (int i = tid; i < n; i += NW * 32) {
+          const unsigned long long me = sh.cand[i];
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += sh.cand[j] > me;
+          if (rank < k) {
+            const int64_t o = r * k + rank;
+            if (a.top_logp) a.top_logp[o] = log_prob(key_value((uint32_t)(me >> 32)), s, ln_s0, a.scale);
+            a.top_ids[o] = (int32_t)(0xffffffffu - (uint32_t)me);
+          }
+        }
+        team_sync<NW>();
+      }
     }
   }
-  if (parts > 1) cg::this_cluster().sync();
-  else __syncthreads();
-  if (part != 0) return;
-  if (sh.n > kCand) select_slow<T, NT>(x, V, a.k, tau, sh, slots);
-  const int n = sh.n;
-  for (int i = tid; i < n; i += NT) {
-    const unsigned long long me = sh.cand[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.cand[j] > me;
-    if (rank < a.k) {
-      const int64_t o = r * a.k + rank;
-      if (a.top_logp) a.top_logp[o] = log_prob(key_value((uint32_t)(me >> 32)), s, ln_s0, a.scale);
-      a.top_ids[o] = (int32_t)(0xffffffffu - (uint32_t)me);
-    }
-  }
+  if (!entered) cg::this_cluster().barrier_wait();
 }
 
 // ------------------------------------------------------------------ gradient of the log probabilities
@@ -373,7 +597,7 @@ __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a
   };
   if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
     const Span<T> sp(x, V, part, slices);
-    const int single = sp.single(V, part, slices);
+    const int single = sp.single(V, part, slices, tid);
     for (int v = sp.lo + tid; v < sp.hi; v += NT) {
       float f[VEC];
       const int i0 = sp.head + v * VEC;
@@ -437,7 +661,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
   const float w = a.row_weight ? a.row_weight[r] : 1.f;
   const bool same = d && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
   const Span<T> sp(x, V, part, parts);
-  const int single = sp.single(V, part, parts);
+  const int single = sp.single(V, part, parts, tid);
   // d[i] = f(x[i], i) over this block's part of the row
   auto fill = [&](auto f) {
     for (int v = sp.lo + tid; v < sp.hi; v += NT) {
@@ -597,12 +821,24 @@ int row_parts(int rows, int vocab) {
   return p;
 }
 
+// `blocks` blocks in clusters of `parts`; resident: at most as many as the device runs at once, each of which
+// goes on to further rows.
 template <typename K, typename... A>
-zl_status launch_parts(const char* what, K kern, int64_t blocks, int threads, int parts, zl_stream s, A... args) {
+zl_status launch_rows(const char* what, K kern, int64_t blocks, int threads, int parts, size_t smem, bool resident,
+                      zl_stream s, A... args) {
+  cudaError_t e = cudaSuccess;
+  if (smem > 0) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && resident) {
+    int per_sm = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
+    blocks = std::min<int64_t>(blocks, (int64_t)std::max(1, per_sm) * sm_count_current());
+  }
+  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
   if (blocks > 0x7fffffff) return set_error(ZL_EUNSUPPORTED, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)s;
   cudaLaunchAttribute attr[1];
   if (parts > 1) {
@@ -613,7 +849,7 @@ zl_status launch_parts(const char* what, K kern, int64_t blocks, int threads, in
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
   return ZL_OK;
 }
@@ -641,11 +877,23 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   if (top_k > kTopMax) return set_error(ZL_EUNSUPPORTED, "token_logprobs: top_k is at most %d", kTopMax);
   if (top_k > 0 && !top_ids) return set_error(ZL_EINVAL, "token_logprobs: null top_ids");
   if (rows == 0) return ZL_OK;
-  constexpr int NT = 256;
-  LogprobArgs a{logits, stride, targets, rows, vocab, top_k, 0, row_parts(rows, vocab), scale,
-                logp, entropy, lse, top_logp, top_ids};
-  a.groups = NT;
-  return launch_parts("token_logprobs", logprobs_kernel<T, NT>, (int64_t)rows * a.parts, NT, a.parts, s, a);
+  LogprobArgs a{logits, stride, targets, rows, vocab, top_k, 1, 0, scale, logp, entropy, lse, top_logp, top_ids};
+  const int vecs = vocab / Elt<T>::VEC + 1;
+  if (top_k <= 64 && rows >= 8 * sm_count_current() && vecs <= 4096) {
+    // a warp to a row
+    constexpr int TEAMS = 4;
+    a.pieces = (vecs + kPieceVecs - 1) / kPieceVecs;
+    return launch_rows("token_logprobs", logprobs_kernel<T, 1, TEAMS>, (rows + TEAMS - 1) / TEAMS, TEAMS * 32, 1,
+                       logprobs_smem<T, 1, TEAMS>(a), true, s, a);
+  }
+  a.parts = row_parts(rows, vocab);
+  for (;; a.parts *= 2) {  // (the maxima of a part fit into shared memory)
+    a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
+    if (logprobs_smem<T, 8, 1>(a) <= 200 * 1024) break;
+    if (a.parts == kMaxParts) return set_error(ZL_EUNSUPPORTED, "token_logprobs: vocab too large for top alternatives");
+  }
+  return launch_rows("token_logprobs", logprobs_kernel<T, 8, 1>, (int64_t)rows * a.parts, 256, a.parts,
+                     logprobs_smem<T, 8, 1>(a), false, s, a);
 }
 
 template <typename T>
@@ -667,7 +915,7 @@ zl_status token_logprobs_backward(const T* logits, int64_t stride, const int32_t
   const int per = NT * Elt<T>::VEC * 4;
   const int slices = (vocab + per - 1) / per;
   LogprobBwdArgs a{logits, stride, targets, lse, entropy, g_logp, g_entropy, rows, vocab, scale, d, d_stride};
-  return launch_parts(what, logprobs_bwd_kernel<T, NT>, (int64_t)rows * slices, NT, 1, s, a, slices);
+  return launch_rows(what, logprobs_bwd_kernel<T, NT>, (int64_t)rows * slices, NT, 1, 0, false, s, a, slices);
 }
 
 template <typename T>
@@ -694,13 +942,26 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
     constexpr int NT = 256;
     DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, row_parts(rows, vocab), *opt, d,
                   d_stride, loss_rows};
-    st = launch_parts(what, distill_kernel<T, NT>, (int64_t)rows * a.parts, NT, a.parts, s, a);
+    st = launch_rows(what, distill_kernel<T, NT>, (int64_t)rows * a.parts, NT, a.parts, 0, false, s, a);
     if (st != ZL_OK) return st;
   }
   if (!loss_out) return ZL_OK;
   scaled_sum_kernel<<<1, 1024, 0, (cudaStream_t)s>>>(loss_rows, rows, opt->grad_scale, loss_out);
   return check_launch("distill_topk loss");
 }
+}  // namespace
+
+int logprobs_dev_error_read_and_clear() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, zl_dev_error, sizeof(int));
+  if (v) {
+    int z = 0;
+    cudaMemcpyToSymbol(zl_dev_error, &z, sizeof(int));
+  }
+  return v;
+}
+
+namespace {
 const __nv_bfloat16* B(const zl_bf16* p) { return reinterpret_cast<const __nv_bfloat16*>(p); }
 __nv_bfloat16* B(zl_bf16* p) { return reinterpret_cast<__nv_bfloat16*>(p); }
 }  // namespace

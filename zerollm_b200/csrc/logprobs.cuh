@@ -36,6 +36,10 @@ struct Stats {
 #pragma unroll
     for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
     if (b > m) rebase(b, c);
+    add_below(v, c);
+  }
+  // elements none of which is above m
+  template <int N> __device__ __forceinline__ void add_below(const float (&v)[N], float c) {
     const float base = m == -INFINITY ? 0.f : m;
     if constexpr (N % 4 == 0) {
       // two pairs of partial sums: four chains of N / 4 additions, paired fp32 instructions
