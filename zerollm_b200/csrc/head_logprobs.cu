@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t acc_empty_leader[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
     int acc = 0;
     uint32_t acc_phase = 0;
-    Stats st;
+    Running run;
     float xt = 0.f;
     int row = 0, t = -1;
     for (int64_t s = s0; s < s1; ++s) {
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (s == s0 || nt == 0) {  // a segment begins
         row = rt * (2 * BM) + (int)rank * BM + quarter * 32 + lane;
         t = (a.targets && row < a.rows) ? a.targets[row] : -1;
-        st = Stats();
+        run = Running();
         xt = 0.f;
       }
       if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) break;
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
         const int n = nt * BN + c;
+        if (n >= a.vocab) break;
         if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
@@ -175,13 +176,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
         }
-        st.add(v, a.c);
+        run.add_any(v, a.c);
       }
       tc_fence_before();
       mbar_arrive_cluster(acc_empty_leader[acc]);
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       if ((s + 1 == s1 || nt + 1 == a.n_tiles) && row < a.rows) {  // it ends: this pair's partial of the row
         const int slot = (int)((int64_t)(blockIdx.x >> 1) - (int64_t)rt * a.n_tiles / a.per);
+        const Stats st = run.sums(a.c);
         a.partials[((int64_t)row * a.slots + slot) * 2 + half] = make_float4(st.m, st.s0, st.s1, xt);
       }
     }

@@ -9,6 +9,7 @@
 // The reference has no counterpart: its loss takes softmax probabilities (cross_entropy.cpp:23-79).
 #include <cooperative_groups.h>
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -28,6 +29,7 @@ constexpr int kMaxParts = 8;   // blocks of a cluster that share a row
 template <typename T> struct Elt;
 template <> struct Elt<float> {
   static constexpr int VEC = 4;
+  static constexpr float MAX = FLT_MAX;
   static __device__ __forceinline__ float get(const float* p) { return *p; }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
   static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[4]) {
@@ -39,6 +41,7 @@ template <> struct Elt<float> {
 };
 template <> struct Elt<__nv_bfloat16> {
   static constexpr int VEC = 8;
+  static constexpr float MAX = 0x1.fep127f;
   static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
   static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
@@ -61,7 +64,7 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   return u;
 }
 // A row as elements [0, head) before its first 16-byte boundary, nv whole vectors, and the rest [tail, V).
-// Block `part` of the `parts` that share the row takes the vectors [lo, hi); the first block takes the
+// Block `part` of the `parts` (a power of two) that share the row takes the vectors [lo, hi); the first block takes the
 // head and the last one the rest, one element per thread.
 template <typename T> struct Span {
   int head, lo, hi, tail;
@@ -70,8 +73,13 @@ template <typename T> struct Span {
     const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     head = mis ? min(VEC - mis, V) : 0;
     const int nv = (V - head) / VEC;
-    lo = (int)((int64_t)nv * part / parts);
-    hi = (int)((int64_t)nv * (part + 1) / parts);
+    lo = 0;
+    hi = nv;
+    if (parts > 1) {
+      const int sh = __ffs(parts) - 1;
+      lo = (int)(((int64_t)nv * part) >> sh);
+      hi = (int)(((int64_t)nv * (part + 1)) >> sh);
+    }
     tail = head + nv * VEC;
   }
   // the element outside whole vectors that thread t has, or -1
@@ -95,7 +103,7 @@ template <typename T, int NT>
 __device__ __forceinline__ Stats block_stats(const T* x, const Span<T>& sp, int single, float c, float& thread_max,
                                              Stats* red) {
   constexpr int VEC = Elt<T>::VEC, U = 4;
-  Stats s;
+  Running run;
   for (int v = sp.lo + (int)threadIdx.x; v < sp.hi; v += NT * U) {
     uint4 u[U];
 #pragma unroll
@@ -106,14 +114,12 @@ __device__ __forceinline__ Stats block_stats(const T* x, const Span<T>& sp, int 
       if (v + i * NT < sp.hi) {
         float f[VEC];
         Elt<T>::unpack(u[i], f);
-        s.add(f, c);
+        run.add_any(f, c);
       }
   }
-  if (single >= 0) {
-    const float f[1] = {Elt<T>::get(x + single)};
-    s.add(f, c);
-  }
-  thread_max = s.m;
+  if (single >= 0) run.add_one(Elt<T>::get(x + single), c);
+  thread_max = run.m;
+  Stats s = run.sums(c);
   s.join_warp(c);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
@@ -128,7 +134,8 @@ __device__ __forceinline__ Stats block_stats(const T* x, const Span<T>& sp, int 
 // A row's vectors are cut into pieces of 128 (four to a lane).  A warp takes every NW-th piece and has up to
 // kDepth of them on the way from device memory (cp.async.bulk into its own ring), so that loads run on while
 // it computes, and into its next row.
-constexpr int kPieceVecs = 128, kPieceBytes = kPieceVecs * 16, kDepth = 4;
+constexpr int kLaneVecs = 4, kPieceVecs = 32 * kLaneVecs, kPieceBytes = kPieceVecs * 16, kDepth = 2;
+constexpr int kRowBlocks = 6;  // blocks of four single-warp teams on an SM
 
 // The source of a warp's pieces: rows r, r + step, ... of the matrix, of each the pieces first, first + NW, ...
 // of the part [lo, hi) of its vectors.
@@ -145,7 +152,7 @@ template <typename T, int NW> struct Feed {
   __device__ void open() {
     for (left = 0; row < rows; row += row_step) {
       const T* x = base + row * stride;
-      const Span<T> sp(x, V, part, parts);
+      const Span<T> sp(x, V, NW == 1 ? 0 : part, NW == 1 ? 1 : parts);
       left = sp.hi - sp.lo - first * kPieceVecs;
       src = reinterpret_cast<const uint8_t*>(x + sp.head) + (int64_t)(sp.lo + first * kPieceVecs) * 16;
       if (left > 0) return;
@@ -171,74 +178,138 @@ template <typename T, int NW> struct Feed {
   }
 };
 
-// A lane's four vectors of a consumed piece; those past its end are -inf.
+// A lane's vectors of a consumed piece (every 32nd one); those past its end are -inf.
 template <typename T, int NW>
-__device__ __forceinline__ void take_piece(Feed<T, NW>& feed, uint32_t n, int vecs, int lane, uint4 (&u)[4]) {
+__device__ __forceinline__ void take_piece(Feed<T, NW>& feed, uint32_t n, int vecs, int lane, uint4 (&u)[kLaneVecs]) {
   const uint32_t s = n % kDepth;
   bounded_wait(&feed.bar[s], (n / kDepth) & 1u, DEV_TIMEOUT_FULL);  // (a lost copy: its error is recorded, nobody hangs)
   const uint4* p = reinterpret_cast<const uint4*>(feed.buf + s * kPieceBytes) + lane;
   constexpr uint32_t NI = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  if (vecs >= kPieceVecs) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) u[j] = j * 32 + lane < vecs ? p[j * 32] : make_uint4(NI, NI, NI, NI);
+    for (int j = 0; j < kLaneVecs; ++j) u[j] = p[j * 32];
+  } else {
+#pragma unroll
+    for (int j = 0; j < kLaneVecs; ++j) u[j] = j * 32 + lane < vecs ? p[j * 32] : make_uint4(NI, NI, NI, NI);
+  }
   __syncwarp();
   feed.issue(lane);
 }
 
-// Maxima of a lane's four vectors, NaN aside.
+// Maxima of a lane's vectors, NaN aside: of each for the piece, and of four classes over all its pieces.
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+__device__ __forceinline__ float lo_bf16(uint32_t a) { return __uint_as_float(a << 16); }
+__device__ __forceinline__ float hi_bf16(uint32_t a) { return __uint_as_float(a & 0xffff0000u); }
+__device__ __forceinline__ float max_of(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
 template <typename T> struct Maxima;
 template <> struct Maxima<__nv_bfloat16> {
-  using Store = uint2;
-  uint2 m{0xff80ff80u, 0xff80ff80u};
-  __device__ __forceinline__ Store take(const uint4 (&u)[4]) {
-    uint32_t h[4];
+  struct __align__(kLaneVecs * 2) Store {
+    uint32_t v[kLaneVecs / 2];
+    __device__ __forceinline__ float most() const {
+      uint32_t a = v[0];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = max2(max2(u[j].x, u[j].y), max2(u[j].z, u[j].w));
-    const uint2 v = make_uint2(max2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[0], h[1], 0x7632)),
-                               max2(__byte_perm(h[2], h[3], 0x5410), __byte_perm(h[2], h[3], 0x7632)));
-    m.x = max2(m.x, v.x);
-    m.y = max2(m.y, v.y);
-    return v;
+      for (int j = 1; j < kLaneVecs / 2; ++j) a = max2(a, v[j]);
+      return fmaxf(lo_bf16(a), hi_bf16(a));
+    }
+    // which of them are >= least (a bf16 value), a bit each
+    __device__ __forceinline__ uint32_t reaching(float least) const {
+      const __nv_bfloat162 l = __float2bfloat162_rn(least);
+      uint32_t b = 0;
+#pragma unroll
+      for (int j = 0; j < kLaneVecs / 2; ++j)
+        b |= __hge2_mask(reinterpret_cast<const __nv_bfloat162&>(v[j]), l) & (0x00020001u << (2 * j));
+      return (b | (b >> 16)) & ((1u << kLaneVecs) - 1u);
+    }
+  };
+  uint32_t m[2] = {0xff80ff80u, 0xff80ff80u};
+  __device__ __forceinline__ Store take(const uint4 (&u)[kLaneVecs]) {
+    uint32_t h[kLaneVecs];
+    Store s;
+#pragma unroll
+    for (int j = 0; j < kLaneVecs; ++j) h[j] = max2(max2(u[j].x, u[j].y), max2(u[j].z, u[j].w));
+#pragma unroll
+    for (int j = 0; j < kLaneVecs / 2; ++j) {
+      s.v[j] = max2(__byte_perm(h[2 * j], h[2 * j + 1], 0x5410), __byte_perm(h[2 * j], h[2 * j + 1], 0x7632));
+      m[j & 1] = max2(m[j & 1], s.v[j]);
+    }
+    return s;
   }
-  static __device__ __forceinline__ float4 values(const Store& v) {
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
-                       __uint_as_float(v.y & 0xffff0000u));
-  }
-  __device__ __forceinline__ float4 all() const { return values(m); }
+  __device__ __forceinline__ float4 all() const { return make_float4(lo_bf16(m[0]), hi_bf16(m[0]), lo_bf16(m[1]), hi_bf16(m[1])); }
 };
 template <> struct Maxima<float> {
-  using Store = float4;
-  float4 m{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  static __device__ __forceinline__ float of(const uint4& u) {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
-  }
-  __device__ __forceinline__ Store take(const uint4 (&u)[4]) {
-    const float4 v = make_float4(of(u[0]), of(u[1]), of(u[2]), of(u[3]));
-    m = make_float4(fmaxf(m.x, v.x), fmaxf(m.y, v.y), fmaxf(m.z, v.z), fmaxf(m.w, v.w));
-    return v;
-  }
-  static __device__ __forceinline__ float4 values(const Store& v) { return v; }
-  __device__ __forceinline__ float4 all() const { return m; }
-};
-// A lane's four vectors, their maximum known.
-template <typename T> __device__ __forceinline__ void add_piece(Stats& s, const uint4 (&u)[4], float most, float c) {
-  constexpr int VEC = Elt<T>::VEC;
-  if (most > s.m) s.rebase(most, c);
-  float f[4 * VEC];
+  struct __align__(16) Store {
+    float v[kLaneVecs];
+    __device__ __forceinline__ float most() const {
+      float a = v[0];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+      for (int j = 1; j < kLaneVecs; ++j) a = fmaxf(a, v[j]);
+      return a;
+    }
+    __device__ __forceinline__ uint32_t reaching(float least) const {
+      uint32_t b = 0;
+#pragma unroll
+      for (int j = 0; j < kLaneVecs; ++j) b |= v[j] >= least ? 1u << j : 0u;
+      return b;
+    }
+  };
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  __device__ __forceinline__ Store take(const uint4 (&u)[kLaneVecs]) {
+    Store s;
+#pragma unroll
+    for (int j = 0; j < kLaneVecs; ++j) {
+      s.v[j] = fmaxf(fmaxf(__uint_as_float(u[j].x), __uint_as_float(u[j].y)), fmaxf(__uint_as_float(u[j].z), __uint_as_float(u[j].w)));
+      m[j & 3] = fmaxf(m[j & 3], s.v[j]);
+    }
+    return s;
+  }
+  __device__ __forceinline__ float4 all() const { return make_float4(m[0], m[1], m[2], m[3]); }
+};
+
+// N of a lane's vectors, none of whose elements is above the running maximum.
+template <typename T, int N, bool E> __device__ __forceinline__ void add_vecs(RunningT<E>& s, const uint4* u, float c) {
+  constexpr int VEC = Elt<T>::VEC;
+  float f[N * VEC];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
     float e[VEC];
-    Elt<T>::unpack(u[j], e);
+    if constexpr (sizeof(T) == 2) {
+      Elt<T>::unpack(make_uint4(max2_nan(u[j].x, kClampBf16), max2_nan(u[j].y, kClampBf16), max2_nan(u[j].z, kClampBf16),
+                                max2_nan(u[j].w, kClampBf16)), e);
+    } else {
+      Elt<T>::unpack(u[j], e);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = max_nan(e[i], kClamp);
+    }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) f[j * VEC + i] = e[i];
   }
-  s.add_below(f, c);
+  s.add(f, c);
 }
-__device__ __forceinline__ float max_of(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+// A lane's vectors of a piece, the maximum of which is known.
+template <typename T, bool E>
+__device__ __forceinline__ void add_piece(RunningT<E>& s, const uint4 (&u)[kLaneVecs], int vecs, float most, float c) {
+  constexpr int VEC = Elt<T>::VEC;
+  if (most > s.m) s.raise(most, c);
+  if (__any_sync(0xffffffffu, s.deep())) {
+#pragma unroll
+    for (int j = 0; j < kLaneVecs; ++j) {
+      float e[VEC];
+      Elt<T>::unpack(u[j], e);
+#pragma unroll 1
+      for (int i = 0; i < VEC; ++i) s.add_one(e[i], c);
+    }
+  } else if (vecs >= kPieceVecs) {
+    add_vecs<T, kLaneVecs>(s, u, c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kLaneVecs; j += 2)
+      if (vecs > j * 32) add_vecs<T, 2>(s, u + j, c);
+  }
+}
 
 // ------------------------------------------------------------------ top alternatives
 // Order-preserving key: larger values have larger keys, -0 and +0 the same one, NaN the lowest (0).
@@ -266,17 +337,35 @@ template <int NW> __device__ __forceinline__ void team_sync() {
 template <int NW> __device__ __forceinline__ int team_thread() { return NW == 1 ? (threadIdx.x & 31) : threadIdx.x; }
 
 template <int NW> struct TopShared {
-  static constexpr int CAP = NW == 1 ? 256 : 512;  // candidates ranked at once; more go the slow way
-  static constexpr int GROUPS = NW == 1 ? 128 : 256;
+  static constexpr int CAP = NW == 1 ? 192 : 512;  // candidates ranked at once; more go the slow way
   unsigned long long cand[CAP];
   int vec[CAP];
-  uint32_t group[NW == 1 ? 1 : GROUPS];
+  float group[NW == 1 ? 1 : 256];
   int slots[NW];
   int n, nvec;
 };
 
-// The largest t whose bits below bit LO are those of `low` such that at least k of the warp's keys (R to a lane)
-// are >= t, given that at least k are >= t0 (whose bits from HI down are 0).
+// Disjoint sets of elements whose maxima bound the top k: with G of them about -G ln(1 - k / G) elements reach the
+// k-th largest maximum (1.1 to 2 k here).
+__host__ __device__ inline int group_count(int k, int least) {
+  const int g = k <= 24 ? 32 : k <= 48 ? 64 : k <= 96 ? 128 : 256;
+  return g < least ? least : g;
+}
+
+// The k-th largest of a warp's 32 values, one to a lane (none NaN): a bitonic sort.
+__device__ __forceinline__ float kth_of_32(float v, int k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int d = size / 2; d > 0; d /= 2) {
+      const float o = __shfl_xor_sync(0xffffffffu, v, d);
+      v = ((lane & size) == 0) == ((lane & d) == 0) ? fmaxf(v, o) : fminf(v, o);
+    }
+  return __shfl_sync(0xffffffffu, v, k - 1);
+}
+// The largest t, its bits from hi to lo beside those of t0, such that at least k of a warp's keys (R to a lane) are
+// >= t, given that at least k are >= t0.
 template <int R> __device__ __forceinline__ uint32_t kth_key(const uint32_t (&g)[R], int k, uint32_t t0, int hi, int lo) {
   uint32_t tau = t0;
 #pragma unroll 1
@@ -289,8 +378,21 @@ template <int R> __device__ __forceinline__ uint32_t kth_key(const uint32_t (&g)
   }
   return tau;
 }
+template <int R> __device__ __forceinline__ uint32_t kth_key(const float* group, int k, uint32_t t0, int hi, int lo) {
+  uint32_t g[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) g[i] = max_key(group[i * 32 + (threadIdx.x & 31)]);
+  return kth_key(g, k, t0, hi, lo);
+}
 
-// Appends a value of each lane that has one; n counts them all, those past CAP are dropped.
+// Appends a value of each lane that has one; n counts them all, those past CAP are dropped.  The counter of a
+// single warp's list is a register of all lanes, that of several warps (or blocks) is in shared memory.
+template <typename V> __device__ __forceinline__ void push(bool yes, V v, V* list, int& n, int cap) {
+  const uint32_t vote = __ballot_sync(0xffffffffu, yes);
+  const int at = n + __popc(vote & ((1u << (threadIdx.x & 31)) - 1u));
+  if (yes && at < cap) list[at] = v;
+  n += __popc(vote);
+}
 template <typename V> __device__ __forceinline__ void push(bool yes, V v, V* list, int* n, int cap) {
   const uint32_t vote = __ballot_sync(0xffffffffu, yes);
   if (vote == 0) return;
@@ -346,8 +448,9 @@ template <typename T, int NW> __device__ int append_equal(const T* x, int V, uin
 
 // The candidates of a row in which more than CAP elements reach the bound (long runs of equal values, as in
 // constant rows and rows masked with a finite value): every element above the key K of the k-th largest one
-// (fewer than k), then the lowest-indexed ones equal to it.  tau: the k-th largest group maximum, so K >= tau,
-// and K = tau unless k elements are above it.
+// (fewer than k), then the lowest-indexed ones equal to it.  K is at least the bound tau, and where runs of equal
+// values fill the row usually the least value above which fewer than k elements lie: tau, or for a bound cut to its
+// upper half one of a few steps more.
 template <typename T, int NW> __device__ int select_slow(const T* x, int V, int k, uint32_t tau, TopShared<NW>& sh) {
   uint32_t K = tau;
   if (count_from<T, NW>(x, V, tau + 1, sh) >= k) {
@@ -388,12 +491,12 @@ template <typename T, int NW, int TEAMS> size_t logprobs_smem(const LogprobArgs&
 }
 
 // NW warps to a row (TEAMS rows to a block), or a cluster of `parts` blocks of NW warps.  Top alternatives: the
-// k-th largest of the maxima of 128 (one warp) or 256 disjoint sets of elements is a bound that at least k
-// elements reach, about 1.15 k of them where values come in any order; the maxima of the single vectors, kept
-// in shared memory, say which vectors to read again (from L2).  Few candidates are left, whose ranks are counted.
+// k-th largest of the maxima of 32 to 256 disjoint sets of elements is a bound that at least k elements reach, and
+// few more where values come in any order; the maxima of the single vectors, kept in shared memory, say which
+// vectors to read again (from L2).  The candidates' ranks are counted.
 template <typename T, int NW, int TEAMS>
-__global__ void __launch_bounds__(NW * TEAMS * 32) logprobs_kernel(const LogprobArgs a) {
-  constexpr int VEC = Elt<T>::VEC, GROUPS = TopShared<NW>::GROUPS, CAP = TopShared<NW>::CAP;
+__global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / NW) logprobs_kernel(const LogprobArgs a) {
+  constexpr int VEC = Elt<T>::VEC, CAP = TopShared<NW>::CAP;
   using Store = typename Maxima<T>::Store;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ TopShared<NW> top[TEAMS];
@@ -401,8 +504,8 @@ __global__ void __launch_bounds__(NW * TEAMS * 32) logprobs_kernel(const Logprob
   __shared__ uint64_t bars[NW * TEAMS * kDepth];
   static_assert(NW == 1 || TEAMS == 1, "a block barrier serves one team");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = NW == 1 ? warp : 0, tid = team_thread<NW>();
-  const int parts = a.parts, part = parts > 1 ? (int)(blockIdx.x % parts) : 0;
-  const int V = a.vocab, k = a.k;
+  const int parts = NW == 1 ? 1 : a.parts, part = parts > 1 ? (int)(blockIdx.x & (parts - 1)) : 0;
+  const int V = a.vocab, k = a.k, groups = group_count(k, NW * parts);
   const float c = a.scale * kLog2e;
   TopShared<NW>& sh = top[team];
   Store* vmax = reinterpret_cast<Store*>(dyn + NW * TEAMS * kDepth * kPieceBytes) + (int64_t)team * a.pieces * 32;
@@ -444,32 +547,38 @@ __global__ void __launch_bounds__(NW * TEAMS * 32) logprobs_kernel(const Logprob
     const float xs = single >= 0 ? Elt<T>::get(x + single) : -INFINITY;
     if (k > 0 && tid == 0) { sh.n = 0; sh.nvec = 0; }
 
-    Stats s;
+    Running run;
     Maxima<T> mx;
     for (int v = sp.lo + (NW == 1 ? 0 : warp) * kPieceVecs, i = NW == 1 ? 0 : warp; v < sp.hi; v += NW * kPieceVecs, i += NW) {
-      uint4 u[4];
+      uint4 u[kLaneVecs];
       take_piece(feed, taken++, sp.hi - v, lane, u);
       const Store m = mx.take(u);
       if (k > 0) vmax[i * 32 + lane] = m;
-      add_piece<T>(s, u, max_of(Maxima<T>::values(m)), c);
+      add_piece<T>(run, u, sp.hi - v, m.most(), c);
     }
-    if (single >= 0) {
-      const float f[1] = {xs};
-      s.add(f, c);
-    }
+    if (single >= 0) run.add_one(xs, c);
+    Stats s = run.sums(c);
     float4 g4 = mx.all();
     g4.x = fmaxf(g4.x, xs);
     s.join_warp(c);
     if constexpr (NW > 1) {
-      if (k > 0) {  // 32 / parts groups to a warp
-        uint32_t g = max_key(max_of(g4));
-        for (int o = parts >> 1; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if (k > 0) {
         if (!entered) { cg::this_cluster().barrier_wait(); entered = true; }  // the other blocks run: their memory may be written
-        if ((lane & (parts - 1)) == 0) {
-          const int at = (part * NW + warp) * (32 / parts) + lane / parts;
-          if (parts == 1) sh.group[at] = g;
+        const int mine = groups / (NW * parts), at = (part * NW + warp) * mine;  // this warp's groups
+        auto put = [&](int i, float v) {
+          if (parts == 1) sh.group[i] = v;
           else
-            for (int q = 0; q < parts; ++q) *cg::this_cluster().map_shared_rank(&sh.group[at], q) = g;
+            for (int q = 0; q < parts; ++q) *cg::this_cluster().map_shared_rank(&sh.group[i], q) = v;
+        };
+        if (mine == 128) {
+          put(at + lane, g4.x); put(at + 32 + lane, g4.y); put(at + 64 + lane, g4.z); put(at + 96 + lane, g4.w);
+        } else if (mine == 64) {
+          put(at + lane, fmaxf(g4.x, g4.y)); put(at + 32 + lane, fmaxf(g4.z, g4.w));
+        } else {
+          float g = max_of(g4);
+          const int per = 32 / mine;
+          for (int o = per >> 1; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+          if ((lane & (per - 1)) == 0) put(at + lane / per, g);
         }
       }
       if (lane == 0) red[warp] = s;
@@ -493,47 +602,77 @@ __global__ void __launch_bounds__(NW * TEAMS * 32) logprobs_kernel(const Logprob
     }
     if (k > 0) {
       if (NW == 1) __syncwarp();
-      // every warp finds the bound; fp32 keys are cut to their upper half first, a slightly lower bound
-      uint32_t g[GROUPS / 32];
-      if constexpr (NW == 1) {
-        g[0] = max_key(g4.x); g[1] = max_key(g4.y); g[2] = max_key(g4.z); g[3] = max_key(g4.w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < GROUPS / 32; ++i) g[i] = sh.group[i * 32 + lane];
-      }
-      const uint32_t tau = kth_key(g, k, 0u, 31, 16);
-      const float least = tau == 0 ? -FLT_MAX : key_value(tau);  // tau = 0: every finite logit is a candidate
+      // every warp finds the bound: a value that at least k elements reach (0: fewer than k groups have a finite
+      // maximum, and every finite logit is a candidate).  Keys are cut to their upper half at first.
+      auto bound = [&](uint32_t t0, int hi, int lo) -> uint32_t {
+        if constexpr (NW == 1) {
+          if (groups == 64) {
+            const uint32_t g[2] = {max_key(fmaxf(g4.x, g4.y)), max_key(fmaxf(g4.z, g4.w))};
+            return kth_key(g, k, t0, hi, lo);
+          }
+          const uint32_t g[4] = {max_key(g4.x), max_key(g4.y), max_key(g4.z), max_key(g4.w)};
+          return kth_key(g, k, t0, hi, lo);
+        } else {
+          return groups == 64 ? kth_key<2>(sh.group, k, t0, hi, lo)
+                 : groups == 128 ? kth_key<4>(sh.group, k, t0, hi, lo) : kth_key<8>(sh.group, k, t0, hi, lo);
+        }
+      };
+      const uint32_t tau = groups == 32 ? max_key(kth_of_32(NW == 1 ? max_of(g4) : sh.group[lane % 256], k)) : bound(0u, 31, 16);
+      const float least = tau == 0 ? -Elt<T>::MAX : key_value(tau);
       TopShared<NW>& first = parts > 1 ? *cg::this_cluster().map_shared_rank(&sh, 0) : sh;
-      push(xs >= least, candidate(order_key(xs), single), first.cand, &first.n, CAP);
-      for (int v = sp.lo + (NW == 1 ? 0 : warp) * kPieceVecs, i = NW == 1 ? 0 : warp; v < sp.hi; v += NW * kPieceVecs, i += NW) {
-        const float4 m = Maxima<T>::values(vmax[i * 32 + lane]);
-        if (__any_sync(0xffffffffu, max_of(m) >= least)) {
-          push(m.x >= least, v + lane, sh.vec, &sh.nvec, CAP);
-          push(m.y >= least, v + 32 + lane, sh.vec, &sh.nvec, CAP);
-          push(m.z >= least, v + 64 + lane, sh.vec, &sh.nvec, CAP);
-          push(m.w >= least, v + 96 + lane, sh.vec, &sh.nvec, CAP);
+      int own_n = 0, own_vec = 0;  // the counters of a single warp
+      auto push_cand = [&](bool yes, float v, int i) {
+        if constexpr (NW == 1) push(yes, candidate(order_key(v), i), sh.cand, own_n, CAP);
+        else push(yes, candidate(order_key(v), i), first.cand, &first.n, CAP);
+      };
+      if (__any_sync(0xffffffffu, xs >= least)) push_cand(xs >= least, xs, single);
+      // the vectors that reach it, as many pieces at a time as a lane's word has bits for
+      constexpr int PW = 32 / kLaneVecs;
+      const int p0 = NW == 1 ? 0 : warp;
+      for (int v0 = sp.lo + p0 * kPieceVecs, i0 = p0; v0 < sp.hi; v0 += PW * NW * kPieceVecs, i0 += PW * NW) {
+        uint32_t bits = 0;
+        const int n = min(PW, (sp.hi - v0 + NW * kPieceVecs - 1) / (NW * kPieceVecs));
+        for (int i = 0; i < n; ++i) bits |= vmax[(i0 + i * NW) * 32 + lane].reaching(least) << (kLaneVecs * i);
+        while (__any_sync(0xffffffffu, bits != 0)) {
+          const int b = __ffs(bits) - 1;
+          const int v = v0 + b / kLaneVecs * NW * kPieceVecs + b % kLaneVecs * 32 + lane;
+          if constexpr (NW == 1) push(bits != 0, v, sh.vec, own_vec, CAP);
+          else push(bits != 0, v, sh.vec, &sh.nvec, CAP);
+          bits &= bits - 1;
         }
       }
       team_sync<NW>();
-      const int nvec = sh.nvec;
+      const int nvec = NW == 1 ? own_vec : sh.nvec;
       for (int i0 = warp * 32 * (NW > 1); i0 < min(nvec, CAP); i0 += NW * 32) {
         float f[VEC];
-        int at = -1;
-        if (i0 + lane < nvec) {
+        int at = 0;
+        uint32_t bits = 0;
+        if (i0 + lane < min(nvec, CAP)) {
           at = sp.head + sh.vec[i0 + lane] * VEC;
           Elt<T>::unpack(load16(x + at), f);
-        }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) push(at >= 0 && f[j] >= least, candidate(order_key(f[j]), at + j), first.cand, &first.n, CAP);
+          for (int j = 0; j < VEC; ++j) bits |= f[j] >= least ? 1u << j : 0u;
+        }
+        while (__any_sync(0xffffffffu, bits != 0)) {
+          const int b = __ffs(bits) - 1;
+          float v = 0.f;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v = b == j ? f[j] : v;
+          push_cand(bits != 0, v, at + b);
+          bits &= bits - 1;
+        }
       }
-      if (nvec > CAP && tid == 0) atomicAdd(&first.n, CAP);  // vectors were dropped: the slow way
+      if (nvec > CAP) {  // vectors were dropped: the slow way
+        own_n += CAP;
+        if (NW > 1 && tid == 0) atomicAdd(&first.n, CAP);
+      }
       if (parts > 1) cg::this_cluster().sync();
       else team_sync<NW>();
       if (part == 0) {
-        int n = sh.n;
+        int n = NW == 1 ? own_n : sh.n;
         team_sync<NW>();
         if (n > CAP) {
-          n = select_slow<T, NW>(x, V, k, kth_key(g, k, tau, 15, 0), sh);
+          n = select_slow<T, NW>(x, V, k, groups == 32 || tau == 0 ? tau : bound(tau, 15, 0), sh);
         } else if (n < k) {  // (tau = 0) masked logits, then NaN ones, by their index
           n = append_equal<T, NW>(x, V, kKeyMasked, n, k, sh);
           n = append_equal<T, NW>(x, V, 0u, n, k, sh);
@@ -541,6 +680,7 @@ __global__ void __launch_bounds__(NW * TEAMS * 32) logprobs_kernel(const Logprob
         for (int i = tid; i < n; i += NW * 32) {
           const unsigned long long me = sh.cand[i];
           int rank = 0;
+#pragma unroll 4
           for (int j = 0; j < n; ++j) rank += sh.cand[j] > me;
           if (rank < k) {
             const int64_t o = r * k + rank;
@@ -596,9 +736,10 @@ __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a
     return v * scale;
   };
   if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0) {
-    const Span<T> sp(x, V, part, slices);
-    const int single = sp.single(V, part, slices, tid);
-    for (int v = sp.lo + tid; v < sp.hi; v += NT) {
+    const Span<T> sp(x, V, 0, 1);
+    const int lo = (int)((int64_t)sp.hi * part / slices), hi = (int)((int64_t)sp.hi * (part + 1) / slices);
+    const int single = part == 0 ? sp.single(V, 0, 1, tid) : -1;
+    for (int v = lo + tid; v < hi; v += NT) {
       float f[VEC];
       const int i0 = sp.head + v * VEC;
       Elt<T>::unpack(load16(x + i0), f);
@@ -821,19 +962,18 @@ int row_parts(int rows, int vocab) {
   return p;
 }
 
-// `blocks` blocks in clusters of `parts`; resident: at most as many as the device runs at once, each of which
-// goes on to further rows.
+constexpr size_t kMaxDynamic = 200 * 1024;
+// Lets a kernel have that much dynamic shared memory, once per device.
+template <typename K> cudaError_t allow_dynamic(K kern, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load() >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxDynamic);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+  return e;
+}
 template <typename K, typename... A>
-zl_status launch_rows(const char* what, K kern, int64_t blocks, int threads, int parts, size_t smem, bool resident,
-                      zl_stream s, A... args) {
-  cudaError_t e = cudaSuccess;
-  if (smem > 0) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && resident) {
-    int per_sm = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
-    blocks = std::min<int64_t>(blocks, (int64_t)std::max(1, per_sm) * sm_count_current());
-  }
-  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+zl_status launch(const char* what, K kern, int64_t blocks, int threads, int parts, size_t smem, zl_stream s, A... args) {
   if (blocks > 0x7fffffff) return set_error(ZL_EUNSUPPORTED, "%s: too many rows", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
@@ -849,9 +989,24 @@ zl_status launch_rows(const char* what, K kern, int64_t blocks, int threads, int
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  e = cudaLaunchKernelEx(&cfg, kern, args...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
   return ZL_OK;
+}
+// Teams of NW warps to a row, or clusters of `parts` blocks; single warps go on to further rows, no more blocks of
+// them than run at once.
+template <typename T, int NW, int TEAMS, typename K>
+zl_status launch_rows(const char* what, K kern, int rows, int parts, zl_stream s, const LogprobArgs& a) {
+  static std::atomic<uint64_t> done{0};
+  const size_t smem = logprobs_smem<T, NW, TEAMS>(a);
+  const cudaError_t e = allow_dynamic(kern, done);
+  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  int64_t blocks = ((int64_t)rows + TEAMS - 1) / TEAMS * parts;
+  if (NW == 1) {
+    const int64_t per_sm = std::min<int64_t>(kRowBlocks, (227 * 1024) / (smem + sizeof(TopShared<NW>) * TEAMS + 2048));
+    blocks = std::min(blocks, per_sm * sm_count_current());
+  }
+  return launch(what, kern, blocks, NW * TEAMS * 32, parts, smem, s, a);
 }
 
 template <typename T> bool off_element(const void* p) { return (reinterpret_cast<uintptr_t>(p) % sizeof(T)) != 0; }
@@ -878,22 +1033,33 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   if (top_k > 0 && !top_ids) return set_error(ZL_EINVAL, "token_logprobs: null top_ids");
   if (rows == 0) return ZL_OK;
   LogprobArgs a{logits, stride, targets, rows, vocab, top_k, 1, 0, scale, logp, entropy, lse, top_logp, top_ids};
-  const int vecs = vocab / Elt<T>::VEC + 1;
-  if (top_k <= 64 && rows >= 8 * sm_count_current() && vecs <= 4096) {
-    // a warp to a row
-    constexpr int TEAMS = 4;
-    a.pieces = (vecs + kPieceVecs - 1) / kPieceVecs;
-    return launch_rows("token_logprobs", logprobs_kernel<T, 1, TEAMS>, (rows + TEAMS - 1) / TEAMS, TEAMS * 32, 1,
-                       logprobs_smem<T, 1, TEAMS>(a), true, s, a);
-  }
-  a.parts = row_parts(rows, vocab);
-  for (;; a.parts *= 2) {  // (the maxima of a part fit into shared memory)
+  const int vecs = vocab / Elt<T>::VEC + 1, sms = sm_count_current();
+  a.pieces = (vecs + kPieceVecs - 1) / kPieceVecs;
+  // Warps to a row: as many as let all rows run at once (24 warps on an SM), if each has a piece of its own; with
+  // more rows than that one warp where a row is short, four where it is 16 pieces or longer, whose rows would
+  // leave SMs idle at the end (measured: 2400 x 6400 17 us with one, 22 / 25 / 41 us with 2 / 4 / 8; 1021 x 50001
+  // 35 us with two, 39 / 41 us with 4 / 8; 600 x 50001 25 us with four, 29 us with 2 or 8; 2048 x 32000 45 us with
+  // four, 56 us with one).
+  const int64_t room = 24 * (int64_t)sms;
+  int nw = 1;
+  if (rows > room / 2) nw = a.pieces >= 16 ? 4 : 1;
+  else
+    while (nw < 8 && rows * 2 * nw <= room && a.pieces >= 2 * nw) nw *= 2;
+  // the vectors' maxima of a row fit beside the rings, and a single warp has 128 groups
+  while (nw < 8 && (vecs > 4096 * nw || (nw == 1 && top_k > 96))) nw *= 2;
+  if (nw == 1) return launch_rows<T, 1, 4>("token_logprobs", logprobs_kernel<T, 1, 4>, rows, 1, s, a);
+  if (nw == 2) return launch_rows<T, 2, 1>("token_logprobs", logprobs_kernel<T, 2, 1>, rows, 1, s, a);
+  if (nw == 4) return launch_rows<T, 4, 1>("token_logprobs", logprobs_kernel<T, 4, 1>, rows, 1, s, a);
+  // blocks to a row: while all still run at once and each warp has a piece (64 x 131072: 21 / 15 / 13 / 22 us with
+  // 1 / 2 / 4 / 8; 1 x 131072: 19 / 15 / 13 / 11 us)
+  const int pieces = a.pieces;
+  while (a.parts < kMaxParts && rows * 2 * (int64_t)a.parts * 8 <= room && pieces >= 14 * a.parts) a.parts *= 2;
+  for (;; a.parts *= 2) {
     a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
-    if (logprobs_smem<T, 8, 1>(a) <= 200 * 1024) break;
+    if (logprobs_smem<T, 8, 1>(a) <= kMaxDynamic) break;
     if (a.parts == kMaxParts) return set_error(ZL_EUNSUPPORTED, "token_logprobs: vocab too large for top alternatives");
   }
-  return launch_rows("token_logprobs", logprobs_kernel<T, 8, 1>, (int64_t)rows * a.parts, 256, a.parts,
-                     logprobs_smem<T, 8, 1>(a), false, s, a);
+  return launch_rows<T, 8, 1>("token_logprobs", logprobs_kernel<T, 8, 1>, rows, a.parts, s, a);
 }
 
 template <typename T>
@@ -915,7 +1081,7 @@ zl_status token_logprobs_backward(const T* logits, int64_t stride, const int32_t
   const int per = NT * Elt<T>::VEC * 4;
   const int slices = (vocab + per - 1) / per;
   LogprobBwdArgs a{logits, stride, targets, lse, entropy, g_logp, g_entropy, rows, vocab, scale, d, d_stride};
-  return launch_rows(what, logprobs_bwd_kernel<T, NT>, (int64_t)rows * slices, NT, 1, 0, false, s, a, slices);
+  return launch(what, logprobs_bwd_kernel<T, NT>, (int64_t)rows * slices, NT, 1, 0, s, a, slices);
 }
 
 template <typename T>
@@ -942,7 +1108,7 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
     constexpr int NT = 256;
     DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, row_parts(rows, vocab), *opt, d,
                   d_stride, loss_rows};
-    st = launch_rows(what, distill_kernel<T, NT>, (int64_t)rows * a.parts, NT, a.parts, 0, false, s, a);
+    st = launch(what, distill_kernel<T, NT>, (int64_t)rows * a.parts, NT, a.parts, 0, s, a);
     if (st != ZL_OK) return st;
   }
   if (!loss_out) return ZL_OK;

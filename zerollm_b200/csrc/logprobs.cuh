@@ -19,53 +19,34 @@ __device__ __forceinline__ float ex2(float t) {
 }
 
 // ------------------------------------------------------------------ running softmax statistics
-// c = scale * log2(e).  A masked logit (-inf) has e = 0; its exponent is kept off -inf before it is
-// multiplied with e.  A NaN or +inf logit makes s0 and s1 NaN.
+// c = scale * log2(e).  Sums of e = 2^((x - m) c) and e (x - m) c about the running maximum m.  A masked logit
+// (-inf) has e = 0; it is kept off -inf before anything is multiplied with e.  A NaN or +inf logit makes s0 and
+// s1 NaN.  While m >= kDeep the exponent is one fused product x c - fl(m c); the rounding of m c is taken out of
+// the sums again when they leave the thread or m rises.
+constexpr float kDeep = -0x1p90f;    // logits below it only occur as masks
+constexpr float kClamp = -0x1p96f;   // masked logits in products: e = 0 beside any m >= kDeep
+constexpr uint32_t kClampBf16 = 0xef80ef80u;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Statistics of some elements, exact about m.
 struct Stats {
   float m = -INFINITY, s0 = 0.f, s1 = 0.f;
-  // statistics of the same elements about the larger maximum M
+  // the same about the larger maximum M
   __device__ __forceinline__ void rebase(float M, float c) {
     const float d = m == -INFINITY ? kFloor : fmaxf((m - M) * c, kFloor);
     const float f = ex2(d);
     s1 = f * fmaf(d, s0, s1);
     s0 *= f;
     m = M;
-  }
-  template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
-    float b = v[0];
-#pragma unroll
-    for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
-    if (b > m) rebase(b, c);
-    add_below(v, c);
-  }
-  // elements none of which is above m
-  template <int N> __device__ __forceinline__ void add_below(const float (&v)[N], float c) {
-    const float base = m == -INFINITY ? 0.f : m;
-    if constexpr (N % 4 == 0) {
-      // two pairs of partial sums: four chains of N / 4 additions, paired fp32 instructions
-      const uint64_t nb = f2_pack(-base, -base), c2 = f2_pack(c, c);
-      uint64_t a0[2] = {0, 0}, a1[2] = {0, 0};
-#pragma unroll
-      for (int j = 0; j < N; j += 2) {
-        float t0, t1;
-        f2_unpack(mul2(add2(f2_pack(v[j], v[j + 1]), nb), c2), t0, t1);
-        const uint64_t e = f2_pack(ex2(t0), ex2(t1));
-        a0[j / 2 & 1] = add2(a0[j / 2 & 1], e);
-        a1[j / 2 & 1] = fma2(e, f2_pack(fmaxf(t0, kFloor), fmaxf(t1, kFloor)), a1[j / 2 & 1]);
-      }
-      float x, y;
-      f2_unpack(add2(a0[0], a0[1]), x, y);
-      s0 += x + y;
-      f2_unpack(add2(a1[0], a1[1]), x, y);
-      s1 += x + y;
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float t = (v[j] - base) * c, e = ex2(t);
-        s0 += e;
-        s1 = fmaf(e, fmaxf(t, kFloor), s1);
-      }
-    }
   }
   __device__ __forceinline__ void join(const Stats& o, float c) {
     Stats a = o;
@@ -87,6 +68,74 @@ struct Stats {
     }
   }
 };
+
+// A thread's running statistics.
+template <bool ENTROPY> struct RunningT {
+  float m = -INFINITY, mc = 0.f, s0 = 0.f, s1 = 0.f;
+  // whether m is a finite mask: add() does not hold for its elements then, add_one() does
+  __device__ __forceinline__ bool deep() const { return m < kDeep && m != -INFINITY; }
+  __device__ __forceinline__ Stats sums(float c) const {
+    Stats s;
+    s.m = m; s.s0 = s0; s.s1 = s1;
+    if (m >= kDeep) {  // m c - fl(m c), exact
+      const float off = fmaf(m, c, -mc), f = fmaf(-off, kLn2, 1.f);
+      s.s1 = f * fmaf(-off, s.s0, s.s1);
+      s.s0 *= f;
+    }
+    return s;
+  }
+  // a maximum above m of elements to come
+  __device__ __forceinline__ void raise(float most, float c) {
+    Stats s = sums(c);
+    s.rebase(most, c);
+    m = most; mc = m * c;
+    s0 = s.s0; s1 = s.s1;
+  }
+  // N elements, none above m and none below kClamp: pairs of partial sums (paired fp32 instructions)
+  template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
+    const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(-mc, -mc);
+    uint64_t a0[2] = {0, 0}, a1[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const uint64_t t = fma2(f2_pack(v[j], v[j + 1]), c2, n2);
+      float t0, t1;
+      f2_unpack(t, t0, t1);
+      const uint64_t e = f2_pack(ex2(t0), ex2(t1));
+      a0[j / 2 & 1] = add2(a0[j / 2 & 1], e);
+      if (ENTROPY) a1[j / 2 & 1] = fma2(e, t, a1[j / 2 & 1]);
+    }
+    float x, y;
+    f2_unpack(add2(a0[0], a0[1]), x, y);
+    s0 += x + y;
+    if (ENTROPY) {
+      f2_unpack(add2(a1[0], a1[1]), x, y);
+      s1 += x + y;
+    }
+  }
+  // one element of any value
+  __device__ __forceinline__ void add_one(float v, float c) {
+    if (v > m) raise(v, c);
+    const float t = m >= kDeep ? fmaf(v, c, -mc) : (v - (m == -INFINITY ? 0.f : m)) * c, e = ex2(t);
+    s0 += e;
+    if (ENTROPY) s1 = fmaf(e, fmaxf(t, kFloor), s1);
+  }
+  // N elements of any values
+  template <int N> __device__ __forceinline__ void add_any(float (&v)[N], float c) {
+    float b = v[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
+    if (b > m) raise(b, c);
+    if (deep()) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) add_one(v[j], c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = max_nan(v[j], kClamp);
+      add(v, c);
+    }
+  }
+};
+using Running = RunningT<true>;
 // ln p of a logit from a row's statistics; a row without a finite logit (s0 = 0) has ln p = -inf everywhere.
 __device__ __forceinline__ float log_prob(float x, const Stats& s, float ln_s0, float scale) {
   return s.s0 == 0.f ? -INFINITY : fmaf(x - s.m, scale, -ln_s0);
