@@ -13,6 +13,8 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
+#include <type_traits>
 
 #include "logprobs.cuh"
 
@@ -97,38 +99,6 @@ template <typename T> struct Span {
     return v >= lo && v < hi;
   }
 };
-
-// Statistics of this block's part of a row, the same in every thread (two block barriers).
-template <typename T, int NT>
-__device__ __forceinline__ Stats block_stats(const T* x, const Span<T>& sp, int single, float c, float& thread_max,
-                                             Stats* red) {
-  constexpr int VEC = Elt<T>::VEC, U = 4;
-  Running run;
-  for (int v = sp.lo + (int)threadIdx.x; v < sp.hi; v += NT * U) {
-    uint4 u[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (v + i * NT < sp.hi) u[i] = load16(x + sp.head + (int64_t)(v + i * NT) * VEC);
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (v + i * NT < sp.hi) {
-        float f[VEC];
-        Elt<T>::unpack(u[i], f);
-        run.add_any(f, c);
-      }
-  }
-  if (single >= 0) run.add_one(Elt<T>::get(x + single), c);
-  thread_max = run.m;
-  Stats s = run.sums(c);
-  s.join_warp(c);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = red[0];
-#pragma unroll
-  for (int w = 1; w < NT / 32; ++w) s.join(red[w], c);
-  __syncthreads();
-  return s;
-}
 
 // ------------------------------------------------------------------ rows through shared memory
 // A row's vectors are cut into pieces of 128 (four to a lane).  A warp takes every NW-th piece and has up to
@@ -269,6 +239,22 @@ template <> struct Maxima<float> {
   __device__ __forceinline__ float4 all() const { return make_float4(m[0], m[1], m[2], m[3]); }
 };
 
+// Maximum of a lane's vectors, NaN aside.
+template <typename T> __device__ __forceinline__ float max_vecs(const uint4 (&u)[kLaneVecs]) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t a = max2(max2(u[0].x, u[0].y), max2(u[0].z, u[0].w));
+#pragma unroll
+    for (int j = 1; j < kLaneVecs; ++j) a = max2(a, max2(max2(u[j].x, u[j].y), max2(u[j].z, u[j].w)));
+    return fmaxf(lo_bf16(a), hi_bf16(a));
+  } else {
+    float a = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kLaneVecs; ++j)
+      a = fmaxf(a, fmaxf(fmaxf(__uint_as_float(u[j].x), __uint_as_float(u[j].y)), fmaxf(__uint_as_float(u[j].z), __uint_as_float(u[j].w))));
+    return a;
+  }
+}
+
 // N of a lane's vectors, none of whose elements is above the running maximum.
 template <typename T, int N, bool E> __device__ __forceinline__ void add_vecs(RunningT<E>& s, const uint4* u, float c) {
   constexpr int VEC = Elt<T>::VEC;
@@ -295,12 +281,15 @@ __device__ __forceinline__ void add_piece(RunningT<E>& s, const uint4 (&u)[kLane
   constexpr int VEC = Elt<T>::VEC;
   if (most > s.m) s.raise(most, c);
   if (__any_sync(0xffffffffu, s.deep())) {
-#pragma unroll
-    for (int j = 0; j < kLaneVecs; ++j) {
-      float e[VEC];
-      Elt<T>::unpack(u[j], e);
 #pragma unroll 1
-      for (int i = 0; i < VEC; ++i) s.add_one(e[i], c);
+    for (int i = 0; i < kLaneVecs * VEC; ++i) {
+      uint32_t word = 0;  // (selected, not indexed: the vectors stay in registers)
+#pragma unroll
+      for (int j = 0; j < kLaneVecs * 4; ++j) {
+        const uint4& v = u[j / 4];
+        word = i * (int)sizeof(T) / 4 == j ? (j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w) : word;
+      }
+      s.add_one(sizeof(T) == 4 ? __uint_as_float(word) : i % 2 ? hi_bf16(word) : lo_bf16(word), c);
     }
   } else if (vecs >= kPieceVecs) {
     add_vecs<T, kLaneVecs>(s, u, c);
@@ -500,7 +489,7 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
   using Store = typename Maxima<T>::Store;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ TopShared<NW> top[TEAMS];
-  __shared__ Stats red[NW], parts_st[kMaxParts];
+  __shared__ float3 red[NW], parts_st[kMaxParts];  // (Stats)
   __shared__ uint64_t bars[NW * TEAMS * kDepth];
   static_assert(NW == 1 || TEAMS == 1, "a block barrier serves one team");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = NW == 1 ? warp : 0, tid = team_thread<NW>();
@@ -581,15 +570,15 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
           if ((lane & (per - 1)) == 0) put(at + lane / per, g);
         }
       }
-      if (lane == 0) red[warp] = s;
+      if (lane == 0) red[warp] = s.pack();
       __syncthreads();
-      s = lane < NW ? red[lane] : Stats();
+      s = lane < NW ? Stats(red[lane]) : Stats();
       s.join_warp(c);
       if (parts > 1) {
         if (!entered) { cg::this_cluster().barrier_wait(); entered = true; }
-        if (tid < parts) *cg::this_cluster().map_shared_rank(&parts_st[part], tid) = s;
+        if (tid < parts) *cg::this_cluster().map_shared_rank(&parts_st[part], tid) = s.pack();
         cg::this_cluster().sync();
-        s = lane < parts ? parts_st[lane] : Stats();
+        s = lane < parts ? Stats(parts_st[lane]) : Stats();
         s.join_warp(c);
       }
     }
@@ -762,178 +751,476 @@ struct DistillArgs {
   const float* values;
   const int32_t* targets;
   const float* row_weight;
-  int rows, vocab, k, parts;
+  int rows, vocab, k, parts, pieces;  // pieces: most of a part
   zl_distill_options opt;
   void* d;
   int64_t d_stride;
   float* loss_rows;
 };
 
-__device__ __forceinline__ float block_sum(float v, float* slots, int warps) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < warps; ++w) v += slots[w];
-  return v;
-}
+#ifndef DW
+#define DW 16
+#endif
+// Blocks of that many warps which an SM runs at once: 16 warps, whose registers suffice.
+constexpr int distill_blocks(int warps) { return DW / warps > 0 ? DW / warps : 1; }
 
-// Loss and gradient of one row per block (or cluster): the statistics of s x (and of x, for the hard target,
-// where s != 1) in one pass, then the dense part p of the gradient in a second one over the row (from L2),
-// then the at most k + 1 elements that also have a teacher's or target's share.  The logits are read before
-// any of this row's gradient is written, so the gradient may take their place.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
-  constexpr int VEC = Elt<T>::VEC, NW = NT / 32;
-  __shared__ Stats red[NW];
-  __shared__ Stats parts_st[kMaxParts], parts_st1[kMaxParts];
-  __shared__ float slots[NW];
-  __shared__ int s_id[kTopMax + 1];
-  __shared__ float s_q[kTopMax + 1];
-  __shared__ float s_sum[2];  // sum q, sum q ln q
-  __shared__ float part_loss[kMaxParts];
-  const int parts = a.parts, part = parts > 1 ? (int)(blockIdx.x % parts) : 0;
-  const int64_t r = blockIdx.x / parts;
-  const int V = a.vocab, tid = threadIdx.x, lane = tid & 31, k = a.k;
-  const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-  T* d = a.d ? static_cast<T*>(a.d) + r * a.d_stride : nullptr;
-  const float w = a.row_weight ? a.row_weight[r] : 1.f;
-  const bool same = d && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
-  const Span<T> sp(x, V, part, parts);
-  const int single = sp.single(V, part, parts, tid);
-  // d[i] = f(x[i], i) over this block's part of the row
-  auto fill = [&](auto f) {
-    for (int v = sp.lo + tid; v < sp.hi; v += NT) {
-      float e[VEC];
-      const int i0 = sp.head + v * VEC;
-      Elt<T>::unpack(load16(x + i0), e);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) e[j] = f(e[j]);
-      if (same) {
-        *reinterpret_cast<uint4*>(d + i0) = Elt<T>::pack(e);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) Elt<T>::put(d + i0 + j, e[j]);
-      }
-    }
-    if (single >= 0) Elt<T>::put(d + single, f(Elt<T>::get(x + single)));
-  };
-  if (w == 0.f) {  // a row without weight has no part in the loss, whatever its logits hold
-    if (d) fill([](float) { return 0.f; });
-    if (part == 0 && tid == 0) a.loss_rows[r] = 0.f;
-    return;
+// How a row's second exponential, e1 = 2^((x - m) log2 e) beside e = 2^((x - m) s log2 e), is had: not at all (no
+// hard target, or s = 1), as the square of the first (s = 1/2), as the fourth power (s = 1/4), or by itself.
+enum Second { kNone, kSquare, kFourth, kOwn };
+
+// Sums of both exponentials about a maximum.
+struct Sums2 {
+  float m = -INFINITY, s = 0.f, h = 0.f;
+  __device__ Sums2() {}
+  __device__ explicit Sums2(const float3& v) : m(v.x), s(v.y), h(v.z) {}
+  __device__ float3 pack() const { return make_float3(m, s, h); }
+  __device__ __forceinline__ void rebase(float M, float c) {
+    const float d = m == -INFINITY ? kFloor : m - M;
+    s *= ex2(fmaxf(d * c, kFloor));
+    h *= ex2(fmaxf(d * kLog2e, kFloor));
+    m = M;
   }
-  const float s = a.opt.scale, c = s * kLog2e, kd = a.opt.distill_weight;
-  int t = a.targets ? a.targets[r] : -1;
-  if (t >= V || a.opt.target_weight == 0.f) t = -1;
-  const float ce = t >= 0 ? a.opt.target_weight : 0.f;
-  const bool hard = t >= 0 && s != 1.f;  // needs the statistics at scale 1 too
-
-  // the teacher's distribution, four alternatives to a lane
-  if (tid < 32) {
-    float y[kTopMax / 32], mx = -INFINITY;
-    int id[kTopMax / 32];
-#pragma unroll
-    for (int i = 0; i < kTopMax / 32; ++i) {
-      const int j = i * 32 + lane;
-      id[i] = j < k ? a.ids[r * k + j] : -1;
-      if (id[i] >= V) id[i] = -1;
-      y[i] = id[i] >= 0 ? a.values[r * k + j] * a.opt.teacher_scale : -INFINITY;
-      if (id[i] < 0) id[i] = -1;
-      mx = fmaxf(mx, y[i]);
-    }
-    float ln_n = 0.f;
-    if (a.opt.normalize) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (mx == -INFINITY) mx = 0.f;
-      float n = 0.f;
-#pragma unroll
-      for (int i = 0; i < kTopMax / 32; ++i) n += expf(y[i] - mx);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-      ln_n = n == 0.f ? 0.f : mx + logf(n);
-    }
-    float sum = 0.f, ent = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTopMax / 32; ++i) {
-      const int j = i * 32 + lane;
-      const float lq = y[i] - ln_n, q = id[i] >= 0 ? expf(lq) : 0.f;
-      sum += q;
-      ent += q == 0.f ? 0.f : q * lq;
-      s_id[j] = id[i];
-      s_q[j] = q;
-    }
+  __device__ __forceinline__ void join_warp(float c) {
+    rebase(max_warp(m), c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      ent += __shfl_xor_sync(0xffffffffu, ent, o);
-    }
-    if (lane == 0) {
-      s_sum[0] = sum; s_sum[1] = ent;
-      s_id[kTopMax] = t; s_q[kTopMax] = 0.f;
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      h += __shfl_xor_sync(0xffffffffu, h, o);
     }
   }
-  if (parts > 1) cg::this_cluster().barrier_arrive();
-  float tmax;
-  Stats st = block_stats<T, NT>(x, sp, single, c, tmax, red), st1 = st;
-  if (hard) st1 = block_stats<T, NT>(x, sp, single, kLog2e, tmax, red);
-  if (parts > 1) {
-    cg::this_cluster().barrier_wait();  // every block of the cluster runs: its shared memory may be written
-    if (tid < parts) {
-      *cg::this_cluster().map_shared_rank(&parts_st[part], tid) = st;
-      *cg::this_cluster().map_shared_rank(&parts_st1[part], tid) = st1;
-    }
-    cg::this_cluster().sync();
-    st = parts_st[0];
-    st1 = parts_st1[0];
-    for (int q = 1; q < parts; ++q) { st.join(parts_st[q], c); if (hard) st1.join(parts_st1[q], kLog2e); }
-    if (!hard) st1 = st;
-  }
-  const bool none = st.s0 == 0.f;  // nothing left of the student's row: no loss, no gradient
-  const float ln_s0 = logf(st.s0), ln_s1 = hard ? logf(st1.s0) : ln_s0;
-  // this thread's alternative (or the hard target), where it lies in this block's part of the row
-  float ej = 0.f, xj = 0.f;
-  const int idx = tid <= kTopMax ? s_id[tid] : -1;
-  static_assert(NT > kTopMax, "a thread for each alternative and the target");
-  const bool mine = idx >= 0 && sp.has(idx, part, parts);
-  if (mine) {
-    xj = Elt<T>::get(x + idx);
-    const float q = s_q[tid];
-    if (tid < kTopMax && q != 0.f && kd != 0.f) ej = -kd * q * log_prob(xj, st, ln_s0, s);
-    if (tid == kTopMax) ej = -ce * log_prob(xj, st1, ln_s1, hard ? 1.f : s);
-  }
-  const float loss = block_sum(ej, slots, NW);
-  if (parts > 1 && tid == 0) *cg::this_cluster().map_shared_rank(&part_loss[part], 0) = loss;
+};
 
-  if (d) {
-    const float gs = a.opt.grad_scale * w;
-    const float wp = gs * kd * s * s_sum[0], wq = gs * kd * s, wc = gs * ce;
-    const float is0 = 1.f / st.s0, is1 = 1.f / st1.s0;
-    const float m = st.m;
-    auto dense = [&](float f) {
-      if (none) return 0.f;
-      const float p = ex2((f - m) * c) * is0;
-      const float p1 = hard ? ex2((f - m) * kLog2e) * is1 : p;
-      return fmaf(wp, p, wc * p1);
-    };
-    fill(dense);
-    __syncthreads();  // the elements below are written a second time, by other threads
-    if (mine && !none) {
-      float q = 0.f;
-      for (int j = 0; j < k; ++j) q += s_id[j] == idx ? s_q[j] : 0.f;
-      Elt<T>::put(d + idx, dense(xj) - wq * q - (idx == t ? wc : 0.f));
+// A thread's exponentials about a maximum m: x c - fl(m c), the rounding of m c taken out by settle() (as in RunningT);
+// below kDeep (masks only) (x - m) c.
+template <int SECOND> struct Exponent {
+  float m, c, mc, mc1;
+  __device__ __forceinline__ void at(float M, float scale_c) {
+    m = M; c = scale_c;
+    mc = m == -INFINITY ? 0.f : m * c;
+    mc1 = m == -INFINITY ? 0.f : m * kLog2e;
+  }
+  __device__ __forceinline__ bool deep() const { return m < kDeep && m != -INFINITY; }
+  // factors that make sums of e and e1 exact about m
+  __device__ __forceinline__ void settle(float& f, float& f1) const {
+    f = f1 = 1.f;
+    if (m >= kDeep) {
+      const float off = fmaf(m, c, -mc) * kLn2;
+      f = 1.f - off;
+      f1 = SECOND == kSquare ? fmaf(-2.f, off, 1.f) : SECOND == kFourth ? fmaf(-4.f, off, 1.f)
+           : SECOND == kOwn ? fmaf(-kLn2, fmaf(m, kLog2e, -mc1), 1.f) : 1.f;
     }
   }
-  float all = loss;
-  if (parts > 1) {
-    cg::this_cluster().sync();
-    all = 0.f;
-    for (int q = 0; q < parts; ++q) all += part_loss[q];
+  __device__ __forceinline__ uint64_t first2(uint64_t x) const {
+    float a, b;
+    f2_unpack(fma2(x, f2_pack(c, c), f2_pack(-mc, -mc)), a, b);
+    return f2_pack(ex2(a), ex2(b));
   }
-  if (part == 0 && tid == 0) a.loss_rows[r] = none ? 0.f : w * fmaf(kd, s_sum[1], all);
+  __device__ __forceinline__ uint64_t second2(uint64_t x, uint64_t e) const {
+    if (SECOND == kSquare) return mul2(e, e);
+    if (SECOND == kFourth) { const uint64_t q = mul2(e, e); return mul2(q, q); }
+    float a, b;
+    f2_unpack(fma2(x, f2_pack(kLog2e, kLog2e), f2_pack(-mc1, -mc1)), a, b);
+    return f2_pack(ex2(a), ex2(b));
+  }
+  // one element of any value
+  __device__ __forceinline__ void one(float x, float& e, float& e1) const {
+    const bool dp = deep();
+    e = ex2(dp ? (x - m) * c : fmaf(x, c, -mc));
+    if (SECOND == kSquare) e1 = e * e;
+    else if (SECOND == kFourth) e1 = (e * e) * (e * e);
+    else if (SECOND == kOwn) e1 = ex2(dp ? (x - m) * kLog2e : fmaf(x, kLog2e, -mc1));
+    else e1 = 0.f;
+  }
+  // wf e + wc e1, of a pair (m not below kDeep) and of one element, rounded alike
+  __device__ __forceinline__ uint64_t grad2(uint64_t x, uint64_t wf, uint64_t wc) const {
+    const uint64_t e = first2(x);
+    if (SECOND == kNone) return mul2(e, wf);
+    if (SECOND == kSquare) return mul2(e, fma2(e, wc, wf));
+    return fma2(wc, second2(x, e), mul2(wf, e));
+  }
+  __device__ __forceinline__ float grad(float x, float wf, float wc) const {
+    float e, e1;
+    one(x, e, e1);
+    if (SECOND == kNone) return __fmul_rn(e, wf);
+    if (SECOND == kSquare) return __fmul_rn(e, fmaf(e, wc, wf));
+    return fmaf(wc, e1, __fmul_rn(wf, e));
+  }
+};
+
+// A row's part lies in shared memory, piece by piece, from its statistics to its gradient; the piece of the next
+// row takes its place as soon as its gradient is written.
+template <int NW> struct DistillShared {
+  __align__(16) int id[kTopMax + 4];  // the teacher's alternatives, then the hard target
+  __align__(16) float q[kTopMax + 4];
+  float single[16];  // the elements outside whole vectors
+  float sum, ent;    // sum q, sum q ln q
+  float slots[NW];
+  float3 red[NW], part[kMaxParts];  // (Sums2)
+  float loss[kMaxParts];
+};
+
+template <typename T, int NW> struct DistillWarp {
+  static constexpr int VEC = Elt<T>::VEC;
+  const DistillArgs& a;
+  uint8_t* buf;    // the team's pieces
+  uint64_t* bar;   // one to a piece
+  uint32_t phase;  // of this warp's pieces, a bit each
+  int warp, lane, part, parts;
+
+  __device__ __forceinline__ Span<T> span(int64_t r) const {
+    return Span<T>(static_cast<const T*>(a.logits) + r * a.stride, a.vocab, part, parts);
+  }
+  // piece i of row r on its way
+  __device__ __forceinline__ void issue(int64_t r, const Span<T>& sp, int i) {
+    const int left = sp.hi - sp.lo - i * kPieceVecs;
+    if (left <= 0 || lane != 0) return;
+    const uint32_t bytes = min(left, kPieceVecs) * 16;
+    mbar_arrive_expect_tx(&bar[i], bytes);
+    bulk_copy_g2s(buf + (int64_t)i * kPieceBytes,
+                  static_cast<const T*>(a.logits) + r * a.stride + sp.head + (int64_t)(sp.lo + i * kPieceVecs) * VEC, bytes, &bar[i]);
+  }
+  __device__ __forceinline__ void read(int i, int vecs, uint4 (&u)[kLaneVecs]) const {
+    const uint4* p = reinterpret_cast<const uint4*>(buf + (int64_t)i * kPieceBytes) + lane;
+    constexpr uint32_t NI = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+    if (vecs >= kPieceVecs) {
+#pragma unroll
+      for (int j = 0; j < kLaneVecs; ++j) u[j] = p[j * 32];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLaneVecs; ++j) u[j] = j * 32 + lane < vecs ? p[j * 32] : make_uint4(NI, NI, NI, NI);
+    }
+  }
+  // this warp's sums of its pieces and its single element xs
+  template <int SECOND> __device__ __forceinline__ Sums2 sums(const Span<T>& sp, float xs, bool single, float c) {
+    Sums2 t;
+    Exponent<SECOND> ex;
+    ex.at(-INFINITY, c);
+    float s = 0.f, h = 0.f;  // about ex
+    auto raise = [&](float most) {
+      float f, f1;
+      ex.settle(f, f1);
+      t.m = ex.m; t.s = s * f; t.h = h * f1;
+      t.rebase(most, c);
+      s = t.s; h = t.h;
+      ex.at(most, c);
+    };
+    auto one = [&](float x) {
+      if (x > ex.m) raise(x);
+      float e, e1;
+      ex.one(x, e, e1);
+      s += e;
+      h += e1;
+    };
+    int n = 0;
+    for (int i = warp; sp.lo + i * kPieceVecs < sp.hi; i += NW, ++n) {
+      bounded_wait(&bar[i], phase >> n & 1u, DEV_TIMEOUT_FULL);
+      phase ^= 1u << n;
+      const int vecs = sp.hi - sp.lo - i * kPieceVecs;
+      uint4 u[kLaneVecs];
+      read(i, vecs, u);
+      const float most = max_vecs<T>(u);
+      if (most > ex.m) raise(most);
+      if (__any_sync(0xffffffffu, ex.deep())) {
+        const T* e = reinterpret_cast<const T*>(buf + (int64_t)i * kPieceBytes);
+#pragma unroll 1
+        for (int l = lane; l < min(vecs, kPieceVecs) * VEC; l += 32) one(Elt<T>::get(e + l));
+        continue;
+      }
+      uint64_t b0[2] = {0, 0}, b1[2] = {0, 0};
+      auto add = [&](const uint4& v) {
+        float f[VEC];
+        Elt<T>::unpack(v, f);
+#pragma unroll
+        for (int l = 0; l < VEC; l += 2) {
+          const uint64_t x = f2_pack(f[l], f[l + 1]), e = ex.first2(x);
+          b0[l / 2 & 1] = add2(b0[l / 2 & 1], e);
+          if (SECOND == kSquare) b1[l / 2 & 1] = fma2(e, e, b1[l / 2 & 1]);
+          else if (SECOND != kNone) b1[l / 2 & 1] = add2(b1[l / 2 & 1], ex.second2(x, e));
+        }
+      };
+      if (vecs > kPieceVecs - 32) {
+#pragma unroll
+        for (int j = 0; j < kLaneVecs; ++j) add(u[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kLaneVecs - 1; ++j)
+          if (vecs > j * 32) add(u[j]);
+      }
+      float p, q;
+      f2_unpack(add2(b0[0], b0[1]), p, q);
+      s += p + q;
+      if (SECOND != kNone) {
+        f2_unpack(add2(b1[0], b1[1]), p, q);
+        h += p + q;
+      }
+    }
+    if (single) one(xs);
+    float f, f1;
+    ex.settle(f, f1);
+    t.m = ex.m; t.s = s * f; t.h = h * f1;
+    return t;
+  }
+  // d = wf e + wc e1 over this warp's pieces, each replaced by the next row's once it is read
+  template <int SECOND>
+  __device__ __forceinline__ void gradient(const Span<T>& sp, const T* x, T* d, bool zero, const Exponent<SECOND>& ex, float wf,
+                                           float wc, int64_t next, const Span<T>& nsp) {
+    const bool plain = d && !zero && !ex.deep() && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+    const uint64_t wf2 = f2_pack(wf, wf), wc2 = f2_pack(wc, wc);
+    const int most = max(sp.hi - sp.lo, nsp.hi - nsp.lo);
+    T* o = d + sp.head + (int64_t)(sp.lo + warp * kPieceVecs + lane) * VEC;
+    for (int i = warp; i * kPieceVecs < most; i += NW, o += NW * kPieceVecs * VEC) {
+      const int vecs = sp.hi - sp.lo - i * kPieceVecs;
+      if (plain && vecs > 0) {
+        uint4 u[kLaneVecs];
+        read(i, vecs, u);
+        auto put = [&](int j) {
+          float f[VEC];
+          Elt<T>::unpack(u[j], f);
+#pragma unroll
+          for (int l = 0; l < VEC; l += 2) {
+            f2_unpack(ex.grad2(f2_pack(f[l], f[l + 1]), wf2, wc2), f[l], f[l + 1]);
+          }
+          *reinterpret_cast<uint4*>(o + j * 32 * VEC) = Elt<T>::pack(f);
+        };
+        if (vecs >= kPieceVecs) {
+#pragma unroll
+          for (int j = 0; j < kLaneVecs; ++j) put(j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kLaneVecs; ++j)
+            if (j * 32 + lane < vecs) put(j);
+        }
+        __syncwarp();
+      } else if (d && vecs > 0) {
+        // one element at a time: rows without part in the loss, of masks only, or of another place within 16 bytes
+        const T* e = reinterpret_cast<const T*>(buf + (int64_t)i * kPieceBytes);
+        T* to = d + sp.head + (int64_t)(sp.lo + i * kPieceVecs) * VEC;
+#pragma unroll 4
+        for (int l = lane; l < min(vecs, kPieceVecs) * VEC; l += 32) {
+          Elt<T>::put(to + l, zero ? 0.f : ex.grad(Elt<T>::get(e + l), wf, wc));
+        }
+        __syncwarp();
+      }
+      if (next < a.rows) issue(next, nsp, i);
+    }
+  }
+};
+
+// Loss and gradient, a row to NW warps (TEAMS rows to a block) or to a cluster of `parts` blocks: the sums of both
+// exponentials from one reading of the row into shared memory, the dense part of the gradient from there, then the at
+// most k + 1 elements with a teacher's or target's share.  The row is read before its gradient is written, so the
+// gradient may take its place.
+template <typename T, int NW, int TEAMS>
+__global__ void __launch_bounds__(NW * TEAMS * 32, distill_blocks(NW * TEAMS)) distill_kernel(const DistillArgs a) {
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ DistillShared<NW> shared[TEAMS];
+  constexpr int ROUNDS = (kTopMax + NW * 32) / (NW * 32), LR = kTopMax / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = NW == 1 ? warp : 0, tid = team_thread<NW>();
+  const int parts = NW == 1 ? 1 : a.parts, part = parts > 1 ? (int)(blockIdx.x & (parts - 1)) : 0;
+  const int V = a.vocab, k = a.k;
+  DistillShared<NW>& sh = shared[team];
+  uint8_t* buf = dyn + (int64_t)team * a.pieces * kPieceBytes;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(dyn + (int64_t)TEAMS * a.pieces * kPieceBytes) + team * a.pieces;
+  DistillWarp<T, NW> w{a, buf, bar, 0u, NW == 1 ? 0 : warp, lane, part, parts};
+  if (lane == 0) {
+    for (int i = w.warp; i < a.pieces; i += NW) mbar_init(&bar[i], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  __syncwarp();
+  const int64_t row0 = parts > 1 ? blockIdx.x / parts : (int64_t)blockIdx.x * TEAMS + team;
+  const int64_t step = parts > 1 ? gridDim.x / parts : (int64_t)gridDim.x * TEAMS;
+  Span<T> sp = w.span(min(row0, (int64_t)a.rows - 1));
+  if (row0 < a.rows)
+    for (int i = w.warp; i < a.pieces; i += NW) w.issue(row0, sp, i);
+  if (parts > 1) cg::this_cluster().barrier_arrive();
+  bool entered = parts == 1;
+
+  const float s = a.opt.scale, c = s * kLog2e, kd = a.opt.distill_weight;
+  // What a row needs beside its logits is asked for one row ahead: the teacher's alternatives (LR to a lane of the
+  // first warp), weight and target.
+  int id[LR], t;
+  float val[LR], weight;
+  auto fetch = [&](int64_t r, int (&id)[LR], float (&val)[LR], int& t, float& weight) {
+    const bool row = r < a.rows;
+#pragma unroll
+    for (int i = 0; i < LR; ++i) {
+      const int j = i * 32 + lane;
+      const bool in = row && w.warp == 0 && j < k;
+      id[i] = in ? a.ids[r * k + j] : -1;
+      val[i] = in ? a.values[r * k + j] : 0.f;
+    }
+    t = row && a.targets && a.opt.target_weight != 0.f ? a.targets[r] : -1;
+    weight = row && a.row_weight ? a.row_weight[r] : 1.f;
+  };
+  fetch(row0, id, val, t, weight);
+  for (int64_t r = row0; r < a.rows; r += step) {
+    const T* x = static_cast<const T*>(a.logits) + r * a.stride;
+    T* d = a.d ? static_cast<T*>(a.d) + r * a.d_stride : nullptr;
+    const int64_t next = r + step;
+    const Span<T> nsp = w.span(min(next, (int64_t)a.rows - 1));
+    const int single = (NW == 1 || tid < 32) ? sp.single(V, part, parts, tid) : -1;
+    const float xs = single >= 0 ? Elt<T>::get(x + single) : -INFINITY;
+    if (single >= 0) sh.single[tid & 15] = xs;
+    if (t >= V) t = -1;
+    const float ce = t >= 0 ? a.opt.target_weight : 0.f;
+    const Second second = t < 0 || s == 1.f ? kNone : s == 0.5f ? kSquare : s == 0.25f ? kFourth : kOwn;
+    int id_n[LR], t_n;
+    float val_n[LR], weight_n;
+    fetch(next, id_n, val_n, t_n, weight_n);
+    // the teacher's distribution
+    if (w.warp == 0) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < LR; ++i) {
+        if (i * 32 >= k) break;
+        if (id[i] < 0 || id[i] >= V) id[i] = -1;
+        val[i] = id[i] >= 0 ? val[i] * a.opt.teacher_scale : -INFINITY;
+        mx = fmaxf(mx, val[i]);
+      }
+      // normalised: q = e^(y - mx) / n and ln q = y - mx - ln n; as given: mx = ln n = 0, n = 1
+      mx = a.opt.normalize ? max_warp(mx) : 0.f;
+      if (mx == -INFINITY) mx = 0.f;
+      float e[LR], n = 0.f, dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < LR; ++i) {
+        e[i] = 0.f;
+        if (i * 32 >= k) continue;
+        e[i] = id[i] >= 0 ? expf(val[i] - mx) : 0.f;
+        n += e[i];
+        dot += e[i] == 0.f ? 0.f : e[i] * (val[i] - mx);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      }
+      const float inv = !a.opt.normalize ? 1.f : n == 0.f ? 0.f : 1.f / n;
+#pragma unroll
+      for (int i = 0; i < LR; ++i) {
+        if (i * 32 >= k) break;
+        sh.id[i * 32 + lane] = id[i];
+        sh.q[i * 32 + lane] = e[i] * inv;
+      }
+      __syncwarp();
+      if (lane < 4) {  // the entry after the last is the hard target; then none, up to a multiple of four
+        sh.id[k + lane] = lane == 0 ? t : -1;
+        sh.q[k + lane] = 0.f;
+      }
+      if (lane == 0) {
+        sh.sum = a.opt.normalize ? (n == 0.f ? 0.f : n * inv) : n;
+        sh.ent = a.opt.normalize ? (n == 0.f ? 0.f : fmaf(dot, inv, -logf(n))) : dot;
+      }
+    }
+
+    Sums2 st = second == kNone ? w.template sums<kNone>(sp, xs, single >= 0, c)
+               : second == kSquare ? w.template sums<kSquare>(sp, xs, single >= 0, c)
+               : second == kFourth ? w.template sums<kFourth>(sp, xs, single >= 0, c)
+                                   : w.template sums<kOwn>(sp, xs, single >= 0, c);
+    st.join_warp(c);
+    if constexpr (NW > 1) {
+      if (lane == 0) sh.red[warp] = st.pack();
+      __syncthreads();
+      st = lane < NW ? Sums2(sh.red[lane]) : Sums2();
+      st.join_warp(c);
+      if (parts > 1) {
+        if (!entered) { cg::this_cluster().barrier_wait(); entered = true; }  // the other blocks run: their memory may be written
+        if (tid < parts) *cg::this_cluster().map_shared_rank(&sh.part[part], tid) = st.pack();
+        cg::this_cluster().sync();
+        st = lane < parts ? Sums2(sh.part[lane]) : Sums2();
+        st.join_warp(c);
+      }
+    } else {
+      __syncwarp();
+    }
+    // the alternatives and the target that lie in this block's part of the row, and their logits
+    int idx[ROUNDS];
+    float xj[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int j = i * NW * 32 + tid;
+      idx[i] = -1;
+      xj[i] = 0.f;
+      if (i * NW * 32 > k) continue;
+      if (j <= k) idx[i] = sh.id[j];
+      if (idx[i] >= 0 && !sp.has(idx[i], part, parts)) idx[i] = -1;
+      if (idx[i] >= 0) {
+        const int v = idx[i] - sp.head;
+        xj[i] = v < 0 ? sh.single[idx[i]] : idx[i] >= sp.tail ? sh.single[8 + idx[i] - sp.tail]
+                : Elt<T>::get(reinterpret_cast<const T*>(buf) + (v - sp.lo * Elt<T>::VEC));
+      }
+    }
+    // a row without weight, or with nothing left, has no part in the loss, whatever else it holds
+    const bool none = weight == 0.f || st.s == 0.f;
+    if (second == kNone) st.h = st.s;
+    const float ln_s = logf(st.s), ln_h = second == kNone ? ln_s : logf(st.h);
+    auto log_p = [&](float v, float scale, float ln) { return fmaf(v - st.m, scale, -ln); };
+    float loss = 0.f;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int j = i * NW * 32 + tid;
+      if (idx[i] < 0) continue;
+      if (j == k) loss -= ce * log_p(xj[i], second == kNone ? s : 1.f, ln_h);
+      else if (sh.q[j] != 0.f && kd != 0.f) loss -= kd * sh.q[j] * log_p(xj[i], s, ln_s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    if constexpr (NW > 1) {
+      if (lane == 0) sh.slots[warp] = loss;
+      __syncthreads();  // (also: every thread has read its logits)
+      loss = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) loss += sh.slots[i];
+      if (parts > 1 && tid == 0) *cg::this_cluster().map_shared_rank(&sh.loss[part], 0) = loss;
+    } else {
+      __syncwarp();
+    }
+    const float gs = a.opt.grad_scale * weight, wq = gs * kd * s, wc = gs * ce;
+    auto write = [&](auto tag) {
+      constexpr int SECOND = decltype(tag)::value;
+      Exponent<SECOND> ex;
+      ex.at(st.m, c);
+      float f, f1;
+      ex.settle(f, f1);
+      const float ff = (SECOND == kNone ? fmaf(wq, sh.sum, wc) : wq * sh.sum) * f / st.s, fc = SECOND == kNone ? 0.f : wc * f1 / st.h;
+      w.template gradient<SECOND>(sp, x, d, none, ex, ff, fc, next, nsp);
+      if (!d) return;
+      if (single >= 0) Elt<T>::put(d + single, none ? 0.f : ex.grad(xs, ff, fc));
+      team_sync<NW>();  // the elements below are written a second time, by other threads
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        if (i * NW * 32 > k) break;
+        if (idx[i] < 0 || none) continue;
+        float q = 0.f;
+        for (int j = 0; j < k; j += 4) {  // (the target's q is 0)
+          const int4 ids = *reinterpret_cast<const int4*>(&sh.id[j]);
+          const float4 qs = *reinterpret_cast<const float4*>(&sh.q[j]);
+          q += (ids.x == idx[i] ? qs.x : 0.f) + (ids.y == idx[i] ? qs.y : 0.f) + (ids.z == idx[i] ? qs.z : 0.f) +
+               (ids.w == idx[i] ? qs.w : 0.f);
+        }
+        Elt<T>::put(d + idx[i], ex.grad(xj[i], ff, fc) - wq * q - (idx[i] == t ? wc : 0.f));
+      }
+    };
+    if (second == kNone) write(std::integral_constant<int, kNone>());
+    else if (second == kSquare) write(std::integral_constant<int, kSquare>());
+    else if (second == kFourth) write(std::integral_constant<int, kFourth>());
+    else write(std::integral_constant<int, kOwn>());
+    if (parts > 1) {
+      cg::this_cluster().sync();
+      if (part == 0 && tid == 0) {
+        loss = 0.f;
+        for (int q = 0; q < parts; ++q) loss += sh.loss[q];
+      }
+    }
+    if (part == 0 && tid == 0) a.loss_rows[r] = none ? 0.f : weight * fmaf(kd, sh.ent, loss);
+    sp = nsp;
+    t = t_n;
+    weight = weight_n;
+#pragma unroll
+    for (int i = 0; i < LR; ++i) { id[i] = id_n[i]; val[i] = val_n[i]; }
+    team_sync<NW>();
+  }
+  if (!entered) cg::this_cluster().barrier_wait();
 }
 
 // *out = scale * sum(v), summed in 64 bits in a fixed order (one block).
@@ -1007,6 +1294,18 @@ zl_status launch_rows(const char* what, K kern, int rows, int parts, zl_stream s
     blocks = std::min(blocks, per_sm * sm_count_current());
   }
   return launch(what, kern, blocks, NW * TEAMS * 32, parts, smem, s, a);
+}
+
+// Teams (or clusters) that run at once, each of which goes on to further rows.
+template <typename T, int NW, int TEAMS, typename K>
+zl_status launch_distill(const char* what, K kern, zl_stream s, const DistillArgs& a) {
+  static std::atomic<uint64_t> done{0};
+  const size_t smem = (size_t)TEAMS * a.pieces * (kPieceBytes + 8);
+  const cudaError_t e = allow_dynamic(kern, done);
+  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(distill_blocks(NW * TEAMS), (227 * 1024) / (smem + sizeof(DistillShared<NW>) * TEAMS + 2048)));
+  const int64_t rows = ((int64_t)a.rows + TEAMS - 1) / TEAMS, room = std::max<int64_t>(1, per_sm * sm_count_current() / a.parts);
+  return launch(what, kern, std::min(rows, room) * a.parts, NW * TEAMS * 32, a.parts, smem, s, a);
 }
 
 template <typename T> bool off_element(const void* p) { return (reinterpret_cast<uintptr_t>(p) % sizeof(T)) != 0; }
@@ -1105,10 +1404,22 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
     return set_error(ZL_EINVAL, "%s: a gradient in the logits' place has their row stride", what);
   if (rows > 0 && !loss_rows) return set_error(ZL_EINVAL, "%s: null loss_rows", what);
   if (rows > 0) {
-    constexpr int NT = 256;
-    DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, row_parts(rows, vocab), *opt, d,
-                  d_stride, loss_rows};
-    st = launch(what, distill_kernel<T, NT>, (int64_t)rows * a.parts, NT, a.parts, 0, s, a);
+    DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, 1, 0, *opt, d, d_stride, loss_rows};
+    const int vecs = vocab / Elt<T>::VEC + 1;
+    int nw = getenv("ZL_DI_NW") ? atoi(getenv("ZL_DI_NW")) : 8;
+    a.parts = getenv("ZL_DI_PARTS") ? atoi(getenv("ZL_DI_PARTS")) : 1;
+    for (;; a.parts *= 2) {
+      a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
+      if ((size_t)a.pieces * (kPieceBytes + 8) <= kMaxDynamic) break;
+      if (a.parts == kMaxParts) return set_error(ZL_EUNSUPPORTED, "%s: vocab too large", what);
+    }
+    if (a.parts > 1 && nw < 8) nw = 8;
+    while (nw < 4 && a.pieces > 24 * nw) nw *= 2;
+    if (nw == 1) st = launch_distill<T, 1, 4>(what, distill_kernel<T, 1, 4>, s, a);
+    else if (nw == 2) st = launch_distill<T, 2, 1>(what, distill_kernel<T, 2, 1>, s, a);
+    else if (nw == 4) st = launch_distill<T, 4, 1>(what, distill_kernel<T, 4, 1>, s, a);
+    else if (nw == 8) st = launch_distill<T, 8, 1>(what, distill_kernel<T, 8, 1>, s, a);
+    else st = launch_distill<T, 16, 1>(what, distill_kernel<T, 16, 1>, s, a);
     if (st != ZL_OK) return st;
   }
   if (!loss_out) return ZL_OK;

@@ -37,9 +37,19 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
   return r;
 }
 
+// Maximum over a warp, NaN aside (-inf where every lane has NaN or -inf).
+__device__ __forceinline__ float max_warp(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Statistics of some elements, exact about m.
 struct Stats {
   float m = -INFINITY, s0 = 0.f, s1 = 0.f;
+  __device__ Stats() {}
+  __device__ explicit Stats(const float3& v) : m(v.x), s0(v.y), s1(v.z) {}
+  __device__ float3 pack() const { return make_float3(m, s0, s1); }
   // the same about the larger maximum M
   __device__ __forceinline__ void rebase(float M, float c) {
     const float d = m == -INFINITY ? kFloor : fmaxf((m - M) * c, kFloor);
@@ -57,10 +67,7 @@ struct Stats {
     s1 += a.s1;
   }
   __device__ __forceinline__ void join_warp(float c) {
-    float M = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    rebase(M, c);
+    rebase(max_warp(m), c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       s0 += __shfl_xor_sync(0xffffffffu, s0, o);
