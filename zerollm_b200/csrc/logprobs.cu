@@ -13,7 +13,6 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
-#include <cstdlib>
 #include <type_traits>
 
 #include "logprobs.cuh"
@@ -116,6 +115,7 @@ template <typename T, int NW> struct Feed {
   int64_t row;
   const uint8_t* src;
   int left;  // vectors from src to the end of the part
+  bool twice, again;  // every row comes twice; this is the second time
   uint32_t issued;
   uint8_t* buf;
   uint64_t* bar;
@@ -142,18 +142,37 @@ template <typename T, int NW> struct Feed {
     left -= NW * kPieceVecs;
     src += NW * kPieceBytes;
     if (left <= 0) {
-      row += row_step;
+      again = twice && !again;
+      if (!again) row += row_step;
       open();
     }
+  }
+  __device__ void init(const T* x, int64_t x_stride, int n_rows, int vocab, int p, int ps, int warp, int64_t row0, int step,
+                       bool both, uint8_t* ring, uint64_t* bars, int lane) {
+    base = x; stride = x_stride; rows = n_rows; V = vocab; part = p; parts = ps;
+    first = warp; row = row0; row_step = step; twice = both; again = false; issued = 0;
+    buf = ring; bar = bars;
+    if (lane == 0) {
+      for (int i = 0; i < kDepth; ++i) mbar_init(&bar[i], 1);
+      fence_mbar_init();
+      fence_proxy_async_smem();
+    }
+    __syncwarp();
+    open();
+    for (int i = 0; i < kDepth; ++i) issue(lane);
+  }
+  // piece n (of those issued) has arrived, in the slot returned
+  __device__ __forceinline__ const uint8_t* wait(uint32_t n) {
+    const uint32_t s = n % kDepth;
+    bounded_wait(&bar[s], (n / kDepth) & 1u, DEV_TIMEOUT_FULL);  // (a lost copy: its error is recorded, nobody hangs)
+    return buf + s * kPieceBytes;
   }
 };
 
 // A lane's vectors of a consumed piece (every 32nd one); those past its end are -inf.
 template <typename T, int NW>
 __device__ __forceinline__ void take_piece(Feed<T, NW>& feed, uint32_t n, int vecs, int lane, uint4 (&u)[kLaneVecs]) {
-  const uint32_t s = n % kDepth;
-  bounded_wait(&feed.bar[s], (n / kDepth) & 1u, DEV_TIMEOUT_FULL);  // (a lost copy: its error is recorded, nobody hangs)
-  const uint4* p = reinterpret_cast<const uint4*>(feed.buf + s * kPieceBytes) + lane;
+  const uint4* p = reinterpret_cast<const uint4*>(feed.wait(n)) + lane;
   constexpr uint32_t NI = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
   if (vecs >= kPieceVecs) {
 #pragma unroll
@@ -255,6 +274,17 @@ template <typename T> __device__ __forceinline__ float max_vecs(const uint4 (&u)
   }
 }
 
+// Element i of a lane's vectors (selected, not indexed: the vectors stay in registers).
+template <typename T> __device__ __forceinline__ float pick(const uint4 (&u)[kLaneVecs], int i) {
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < kLaneVecs * 4; ++j) {
+    const uint4& v = u[j / 4];
+    word = i * (int)sizeof(T) / 4 == j ? (j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w) : word;
+  }
+  return sizeof(T) == 4 ? __uint_as_float(word) : i % 2 ? hi_bf16(word) : lo_bf16(word);
+}
+
 // N of a lane's vectors, none of whose elements is above the running maximum.
 template <typename T, int N, bool E> __device__ __forceinline__ void add_vecs(RunningT<E>& s, const uint4* u, float c) {
   constexpr int VEC = Elt<T>::VEC;
@@ -282,15 +312,7 @@ __device__ __forceinline__ void add_piece(RunningT<E>& s, const uint4 (&u)[kLane
   if (most > s.m) s.raise(most, c);
   if (__any_sync(0xffffffffu, s.deep())) {
 #pragma unroll 1
-    for (int i = 0; i < kLaneVecs * VEC; ++i) {
-      uint32_t word = 0;  // (selected, not indexed: the vectors stay in registers)
-#pragma unroll
-      for (int j = 0; j < kLaneVecs * 4; ++j) {
-        const uint4& v = u[j / 4];
-        word = i * (int)sizeof(T) / 4 == j ? (j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w) : word;
-      }
-      s.add_one(sizeof(T) == 4 ? __uint_as_float(word) : i % 2 ? hi_bf16(word) : lo_bf16(word), c);
-    }
+    for (int i = 0; i < kLaneVecs * VEC; ++i) s.add_one(pick<T>(u, i), c);
   } else if (vecs >= kPieceVecs) {
     add_vecs<T, kLaneVecs>(s, u, c);
   } else {
@@ -502,21 +524,8 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
   const int row_step = parts > 1 ? (int)(gridDim.x / parts) : (int)gridDim.x * TEAMS;
 
   Feed<T, NW> feed;
-  feed.base = static_cast<const T*>(a.logits);
-  feed.stride = a.stride;
-  feed.rows = a.rows; feed.V = V; feed.part = part; feed.parts = parts;
-  feed.first = NW == 1 ? 0 : warp;
-  feed.row_step = row_step; feed.row = row0; feed.issued = 0;
-  feed.buf = dyn + warp * kDepth * kPieceBytes;
-  feed.bar = bars + warp * kDepth;
-  if (lane == 0) {
-    for (int i = 0; i < kDepth; ++i) mbar_init(&feed.bar[i], 1);
-    fence_mbar_init();
-    fence_proxy_async_smem();
-  }
-  __syncwarp();
-  feed.open();
-  for (int i = 0; i < kDepth; ++i) feed.issue(lane);
+  feed.init(static_cast<const T*>(a.logits), a.stride, a.rows, V, part, parts, NW == 1 ? 0 : warp, row0, row_step, false,
+            dyn + warp * kDepth * kPieceBytes, bars + warp * kDepth, lane);
   if (parts > 1) cg::this_cluster().barrier_arrive();
   uint32_t taken = 0;
   bool entered = parts == 1;
@@ -751,18 +760,12 @@ struct DistillArgs {
   const float* values;
   const int32_t* targets;
   const float* row_weight;
-  int rows, vocab, k, parts, pieces;  // pieces: most of a part
+  int rows, vocab, k, parts;
   zl_distill_options opt;
   void* d;
   int64_t d_stride;
   float* loss_rows;
 };
-
-#ifndef DW
-#define DW 16
-#endif
-// Blocks of that many warps which an SM runs at once: 16 warps, whose registers suffice.
-constexpr int distill_blocks(int warps) { return DW / warps > 0 ? DW / warps : 1; }
 
 // How a row's second exponential, e1 = 2^((x - m) log2 e) beside e = 2^((x - m) s log2 e), is had: not at all (no
 // hard target, or s = 1), as the square of the first (s = 1/2), as the fourth power (s = 1/4), or by itself.
@@ -847,276 +850,218 @@ template <int SECOND> struct Exponent {
   }
 };
 
-// A row's part lies in shared memory, piece by piece, from its statistics to its gradient; the piece of the next
-// row takes its place as soon as its gradient is written.
 template <int NW> struct DistillShared {
   __align__(16) int id[kTopMax + 4];  // the teacher's alternatives, then the hard target
   __align__(16) float q[kTopMax + 4];
-  float single[16];  // the elements outside whole vectors
+  float x[kTopMax + 4];     // the student's logits there
+  int next_id[kTopMax];     // as given, of the next row
+  float next_val[kTopMax];
   float sum, ent;    // sum q, sum q ln q
-  float slots[NW];
   float3 red[NW], part[kMaxParts];  // (Sums2)
-  float loss[kMaxParts];
 };
+// 4 bytes on their way to shared memory; all of the thread's have arrived
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-template <typename T, int NW> struct DistillWarp {
-  static constexpr int VEC = Elt<T>::VEC;
-  const DistillArgs& a;
-  uint8_t* buf;    // the team's pieces
-  uint64_t* bar;   // one to a piece
-  uint32_t phase;  // of this warp's pieces, a bit each
-  int warp, lane, part, parts;
-
-  __device__ __forceinline__ Span<T> span(int64_t r) const {
-    return Span<T>(static_cast<const T*>(a.logits) + r * a.stride, a.vocab, part, parts);
-  }
-  // piece i of row r on its way
-  __device__ __forceinline__ void issue(int64_t r, const Span<T>& sp, int i) {
-    const int left = sp.hi - sp.lo - i * kPieceVecs;
-    if (left <= 0 || lane != 0) return;
-    const uint32_t bytes = min(left, kPieceVecs) * 16;
-    mbar_arrive_expect_tx(&bar[i], bytes);
-    bulk_copy_g2s(buf + (int64_t)i * kPieceBytes,
-                  static_cast<const T*>(a.logits) + r * a.stride + sp.head + (int64_t)(sp.lo + i * kPieceVecs) * VEC, bytes, &bar[i]);
-  }
-  __device__ __forceinline__ void read(int i, int vecs, uint4 (&u)[kLaneVecs]) const {
-    const uint4* p = reinterpret_cast<const uint4*>(buf + (int64_t)i * kPieceBytes) + lane;
-    constexpr uint32_t NI = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
-    if (vecs >= kPieceVecs) {
-#pragma unroll
-      for (int j = 0; j < kLaneVecs; ++j) u[j] = p[j * 32];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kLaneVecs; ++j) u[j] = j * 32 + lane < vecs ? p[j * 32] : make_uint4(NI, NI, NI, NI);
-    }
-  }
-  // this warp's sums of its pieces and its single element xs
-  template <int SECOND> __device__ __forceinline__ Sums2 sums(const Span<T>& sp, float xs, bool single, float c) {
-    Sums2 t;
-    Exponent<SECOND> ex;
-    ex.at(-INFINITY, c);
-    float s = 0.f, h = 0.f;  // about ex
-    auto raise = [&](float most) {
-      float f, f1;
-      ex.settle(f, f1);
-      t.m = ex.m; t.s = s * f; t.h = h * f1;
-      t.rebase(most, c);
-      s = t.s; h = t.h;
-      ex.at(most, c);
-    };
-    auto one = [&](float x) {
-      if (x > ex.m) raise(x);
-      float e, e1;
-      ex.one(x, e, e1);
-      s += e;
-      h += e1;
-    };
-    int n = 0;
-    for (int i = warp; sp.lo + i * kPieceVecs < sp.hi; i += NW, ++n) {
-      bounded_wait(&bar[i], phase >> n & 1u, DEV_TIMEOUT_FULL);
-      phase ^= 1u << n;
-      const int vecs = sp.hi - sp.lo - i * kPieceVecs;
-      uint4 u[kLaneVecs];
-      read(i, vecs, u);
-      const float most = max_vecs<T>(u);
-      if (most > ex.m) raise(most);
-      if (__any_sync(0xffffffffu, ex.deep())) {
-        const T* e = reinterpret_cast<const T*>(buf + (int64_t)i * kPieceBytes);
-#pragma unroll 1
-        for (int l = lane; l < min(vecs, kPieceVecs) * VEC; l += 32) one(Elt<T>::get(e + l));
-        continue;
-      }
-      uint64_t b0[2] = {0, 0}, b1[2] = {0, 0};
-      auto add = [&](const uint4& v) {
-        float f[VEC];
-        Elt<T>::unpack(v, f);
-#pragma unroll
-        for (int l = 0; l < VEC; l += 2) {
-          const uint64_t x = f2_pack(f[l], f[l + 1]), e = ex.first2(x);
-          b0[l / 2 & 1] = add2(b0[l / 2 & 1], e);
-          if (SECOND == kSquare) b1[l / 2 & 1] = fma2(e, e, b1[l / 2 & 1]);
-          else if (SECOND != kNone) b1[l / 2 & 1] = add2(b1[l / 2 & 1], ex.second2(x, e));
-        }
-      };
-      if (vecs > kPieceVecs - 32) {
-#pragma unroll
-        for (int j = 0; j < kLaneVecs; ++j) add(u[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kLaneVecs - 1; ++j)
-          if (vecs > j * 32) add(u[j]);
-      }
-      float p, q;
-      f2_unpack(add2(b0[0], b0[1]), p, q);
-      s += p + q;
-      if (SECOND != kNone) {
-        f2_unpack(add2(b1[0], b1[1]), p, q);
-        h += p + q;
-      }
-    }
-    if (single) one(xs);
+// A warp's sums of its pieces of a row and of its single element xs.
+template <int SECOND, typename T, int NW>
+__device__ __forceinline__ Sums2 distill_sums(Feed<T, NW>& feed, uint32_t& taken, const Span<T>& sp, float xs, bool single, float c,
+                                              int lane) {
+  constexpr int VEC = Elt<T>::VEC;
+  Sums2 t;
+  Exponent<SECOND> ex;
+  ex.at(-INFINITY, c);
+  float s = 0.f, h = 0.f;  // about ex
+  auto raise = [&](float most) {
     float f, f1;
     ex.settle(f, f1);
     t.m = ex.m; t.s = s * f; t.h = h * f1;
-    return t;
-  }
-  // d = wf e + wc e1 over this warp's pieces, each replaced by the next row's once it is read
-  template <int SECOND>
-  __device__ __forceinline__ void gradient(const Span<T>& sp, const T* x, T* d, bool zero, const Exponent<SECOND>& ex, float wf,
-                                           float wc, int64_t next, const Span<T>& nsp) {
-    const bool plain = d && !zero && !ex.deep() && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
-    const uint64_t wf2 = f2_pack(wf, wf), wc2 = f2_pack(wc, wc);
-    const int most = max(sp.hi - sp.lo, nsp.hi - nsp.lo);
-    T* o = d + sp.head + (int64_t)(sp.lo + warp * kPieceVecs + lane) * VEC;
-    for (int i = warp; i * kPieceVecs < most; i += NW, o += NW * kPieceVecs * VEC) {
-      const int vecs = sp.hi - sp.lo - i * kPieceVecs;
-      if (plain && vecs > 0) {
-        uint4 u[kLaneVecs];
-        read(i, vecs, u);
-        auto put = [&](int j) {
-          float f[VEC];
-          Elt<T>::unpack(u[j], f);
+    t.rebase(most, c);
+    s = t.s; h = t.h;
+    ex.at(most, c);
+  };
+  auto one = [&](float x) {
+    if (x > ex.m) raise(x);
+    float e, e1;
+    ex.one(x, e, e1);
+    s += e;
+    h += e1;
+  };
+  for (int v = sp.lo + feed.first * kPieceVecs; v < sp.hi; v += NW * kPieceVecs) {
+    uint4 u[kLaneVecs];
+    const int vecs = sp.hi - v;
+    take_piece(feed, taken++, vecs, lane, u);
+    const float most = max_vecs<T>(u);
+    if (most > ex.m) raise(most);
+    if (__any_sync(0xffffffffu, ex.deep())) {
+#pragma unroll 1
+      for (int i = 0; i < kLaneVecs * VEC; ++i) one(pick<T>(u, i));
+      continue;
+    }
+    uint64_t b0[2] = {0, 0}, b1[2] = {0, 0};
 #pragma unroll
-          for (int l = 0; l < VEC; l += 2) {
-            f2_unpack(ex.grad2(f2_pack(f[l], f[l + 1]), wf2, wc2), f[l], f[l + 1]);
-          }
-          *reinterpret_cast<uint4*>(o + j * 32 * VEC) = Elt<T>::pack(f);
-        };
-        if (vecs >= kPieceVecs) {
+    for (int j = 0; j < kLaneVecs; ++j) {
+      float f[VEC];
+      Elt<T>::unpack(u[j], f);
 #pragma unroll
-          for (int j = 0; j < kLaneVecs; ++j) put(j);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kLaneVecs; ++j)
-            if (j * 32 + lane < vecs) put(j);
-        }
-        __syncwarp();
-      } else if (d && vecs > 0) {
-        // one element at a time: rows without part in the loss, of masks only, or of another place within 16 bytes
-        const T* e = reinterpret_cast<const T*>(buf + (int64_t)i * kPieceBytes);
-        T* to = d + sp.head + (int64_t)(sp.lo + i * kPieceVecs) * VEC;
-#pragma unroll 4
-        for (int l = lane; l < min(vecs, kPieceVecs) * VEC; l += 32) {
-          Elt<T>::put(to + l, zero ? 0.f : ex.grad(Elt<T>::get(e + l), wf, wc));
-        }
-        __syncwarp();
+      for (int l = 0; l < VEC; l += 2) {
+        const uint64_t x = f2_pack(f[l], f[l + 1]), e = ex.first2(x);
+        b0[l / 2 & 1] = add2(b0[l / 2 & 1], e);
+        if (SECOND == kSquare) b1[l / 2 & 1] = fma2(e, e, b1[l / 2 & 1]);
+        else if (SECOND != kNone) b1[l / 2 & 1] = add2(b1[l / 2 & 1], ex.second2(x, e));
       }
-      if (next < a.rows) issue(next, nsp, i);
+      if (vecs <= (j + 1) * 32) break;
+    }
+    float p, q;
+    f2_unpack(add2(b0[0], b0[1]), p, q);
+    s += p + q;
+    if (SECOND != kNone) {
+      f2_unpack(add2(b1[0], b1[1]), p, q);
+      h += p + q;
     }
   }
-};
+  if (single) one(xs);
+  float f, f1;
+  ex.settle(f, f1);
+  t.m = ex.m; t.s = s * f; t.h = h * f1;
+  return t;
+}
+
+// d = wf e + wc e1 over a warp's pieces of a row.
+template <int SECOND, typename T, int NW>
+__device__ __forceinline__ void distill_gradient(Feed<T, NW>& feed, uint32_t& taken, const Span<T>& sp, const T* x, T* d, bool zero,
+                                                 const Exponent<SECOND>& ex, float wf, float wc, int lane) {
+  constexpr int VEC = Elt<T>::VEC;
+  const bool plain = !zero && !ex.deep() && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  const uint64_t wf2 = f2_pack(wf, wf), wc2 = f2_pack(wc, wc);
+  for (int v = sp.lo + feed.first * kPieceVecs; v < sp.hi; v += NW * kPieceVecs) {
+    const int vecs = sp.hi - v;
+    if (plain) {
+      uint4 u[kLaneVecs];
+      take_piece(feed, taken++, vecs, lane, u);
+      T* o = d + sp.head + (int64_t)(v + lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < kLaneVecs; ++j) {
+        float f[VEC];
+        Elt<T>::unpack(u[j], f);
+#pragma unroll
+        for (int l = 0; l < VEC; l += 2) f2_unpack(ex.grad2(f2_pack(f[l], f[l + 1]), wf2, wc2), f[l], f[l + 1]);
+        if (j * 32 + lane < vecs) *reinterpret_cast<uint4*>(o + j * 32 * VEC) = Elt<T>::pack(f);
+        if (vecs <= (j + 1) * 32) break;
+      }
+    } else {
+      // one element at a time: rows without part in the loss, of masks only, or of another place within 16 bytes
+      const T* e = reinterpret_cast<const T*>(feed.wait(taken++));
+      T* o = d + sp.head + (int64_t)v * VEC;
+#pragma unroll 4
+      for (int l = lane; l < min(vecs, kPieceVecs) * VEC; l += 32) Elt<T>::put(o + l, zero ? 0.f : ex.grad(Elt<T>::get(e + l), wf, wc));
+      __syncwarp();
+      feed.issue(lane);
+    }
+  }
+}
 
 // Loss and gradient, a row to NW warps (TEAMS rows to a block) or to a cluster of `parts` blocks: the sums of both
-// exponentials from one reading of the row into shared memory, the dense part of the gradient from there, then the at
-// most k + 1 elements with a teacher's or target's share.  The row is read before its gradient is written, so the
-// gradient may take its place.
+// exponentials from one reading of the row, the dense part of the gradient from a second one (out of L2, and already
+// under way while the sums are joined), then the at most k + 1 elements with a teacher's or target's share.  An element
+// is read for the last time before its gradient is written, so the gradient may take its place.
 template <typename T, int NW, int TEAMS>
-__global__ void __launch_bounds__(NW * TEAMS * 32, distill_blocks(NW * TEAMS)) distill_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(NW * TEAMS * 32, 24 / (NW * TEAMS)) distill_kernel(const DistillArgs a) {
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ DistillShared<NW> shared[TEAMS];
-  constexpr int ROUNDS = (kTopMax + NW * 32) / (NW * 32), LR = kTopMax / 32;
+  __shared__ uint64_t bars[NW * TEAMS * kDepth];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = NW == 1 ? warp : 0, tid = team_thread<NW>();
+  const bool lead = NW == 1 || warp == 0;  // the team's first warp
   const int parts = NW == 1 ? 1 : a.parts, part = parts > 1 ? (int)(blockIdx.x & (parts - 1)) : 0;
   const int V = a.vocab, k = a.k;
   DistillShared<NW>& sh = shared[team];
-  uint8_t* buf = dyn + (int64_t)team * a.pieces * kPieceBytes;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(dyn + (int64_t)TEAMS * a.pieces * kPieceBytes) + team * a.pieces;
-  DistillWarp<T, NW> w{a, buf, bar, 0u, NW == 1 ? 0 : warp, lane, part, parts};
-  if (lane == 0) {
-    for (int i = w.warp; i < a.pieces; i += NW) mbar_init(&bar[i], 1);
-    fence_mbar_init();
-    fence_proxy_async_smem();
-  }
-  __syncwarp();
   const int64_t row0 = parts > 1 ? blockIdx.x / parts : (int64_t)blockIdx.x * TEAMS + team;
-  const int64_t step = parts > 1 ? gridDim.x / parts : (int64_t)gridDim.x * TEAMS;
-  Span<T> sp = w.span(min(row0, (int64_t)a.rows - 1));
-  if (row0 < a.rows)
-    for (int i = w.warp; i < a.pieces; i += NW) w.issue(row0, sp, i);
+  const int step = parts > 1 ? (int)(gridDim.x / parts) : (int)gridDim.x * TEAMS;
+  Feed<T, NW> feed;
+  feed.init(static_cast<const T*>(a.logits), a.stride, a.rows, V, part, parts, NW == 1 ? 0 : warp, row0, step, a.d != nullptr,
+            dyn + warp * kDepth * kPieceBytes, bars + warp * kDepth, lane);
+  uint32_t taken = 0;
   if (parts > 1) cg::this_cluster().barrier_arrive();
   bool entered = parts == 1;
 
   const float s = a.opt.scale, c = s * kLog2e, kd = a.opt.distill_weight;
-  // What a row needs beside its logits is asked for one row ahead: the teacher's alternatives (LR to a lane of the
-  // first warp), weight and target.
-  int id[LR], t;
-  float val[LR], weight;
-  auto fetch = [&](int64_t r, int (&id)[LR], float (&val)[LR], int& t, float& weight) {
-    const bool row = r < a.rows;
-#pragma unroll
-    for (int i = 0; i < LR; ++i) {
-      const int j = i * 32 + lane;
-      const bool in = row && w.warp == 0 && j < k;
-      id[i] = in ? a.ids[r * k + j] : -1;
-      val[i] = in ? a.values[r * k + j] : 0.f;
-    }
-    t = row && a.targets && a.opt.target_weight != 0.f ? a.targets[r] : -1;
-    weight = row && a.row_weight ? a.row_weight[r] : 1.f;
+  // What a row needs beside its logits is asked for one row ahead: the teacher's alternatives, weight and target.
+  int t = -1;
+  float weight = 1.f;
+  auto fetch = [&](int64_t r, int& t, float& weight) {
+    if (r >= a.rows) return;
+    if (lead)
+      for (int j = lane; j < k; j += 32) {
+        copy4(&sh.next_id[j], a.ids + r * k + j);
+        copy4(&sh.next_val[j], a.values + r * k + j);
+      }
+    if (a.targets && a.opt.target_weight != 0.f) t = a.targets[r];
+    if (a.row_weight) weight = a.row_weight[r];
   };
-  fetch(row0, id, val, t, weight);
+  fetch(row0, t, weight);
   for (int64_t r = row0; r < a.rows; r += step) {
     const T* x = static_cast<const T*>(a.logits) + r * a.stride;
     T* d = a.d ? static_cast<T*>(a.d) + r * a.d_stride : nullptr;
-    const int64_t next = r + step;
-    const Span<T> nsp = w.span(min(next, (int64_t)a.rows - 1));
+    const Span<T> sp(x, V, part, parts);
     const int single = (NW == 1 || tid < 32) ? sp.single(V, part, parts, tid) : -1;
     const float xs = single >= 0 ? Elt<T>::get(x + single) : -INFINITY;
-    if (single >= 0) sh.single[tid & 15] = xs;
     if (t >= V) t = -1;
     const float ce = t >= 0 ? a.opt.target_weight : 0.f;
     const Second second = t < 0 || s == 1.f ? kNone : s == 0.5f ? kSquare : s == 0.25f ? kFourth : kOwn;
-    int id_n[LR], t_n;
-    float val_n[LR], weight_n;
-    fetch(next, id_n, val_n, t_n, weight_n);
-    // the teacher's distribution
-    if (w.warp == 0) {
+    int t_n = -1;
+    float weight_n = 1.f;
+    if (lead) {
+      // the alternatives, and the student's logits at them and at the target
+      copies_done();  // (each lane's own)
       float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < LR; ++i) {
-        if (i * 32 >= k) break;
-        if (id[i] < 0 || id[i] >= V) id[i] = -1;
-        val[i] = id[i] >= 0 ? val[i] * a.opt.teacher_scale : -INFINITY;
-        mx = fmaxf(mx, val[i]);
+      for (int j = lane; j < k; j += 32) {
+        int id = sh.next_id[j];
+        if (id >= V) id = -1;
+        if (id >= 0) sh.x[j] = Elt<T>::get(x + id);
+        const float v = id >= 0 ? sh.next_val[j] * a.opt.teacher_scale : -INFINITY;
+        sh.id[j] = id;
+        sh.q[j] = v;
+        mx = fmaxf(mx, v);
       }
       // normalised: q = e^(y - mx) / n and ln q = y - mx - ln n; as given: mx = ln n = 0, n = 1
       mx = a.opt.normalize ? max_warp(mx) : 0.f;
       if (mx == -INFINITY) mx = 0.f;
-      float e[LR], n = 0.f, dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < LR; ++i) {
-        e[i] = 0.f;
-        if (i * 32 >= k) continue;
-        e[i] = id[i] >= 0 ? expf(val[i] - mx) : 0.f;
-        n += e[i];
-        dot += e[i] == 0.f ? 0.f : e[i] * (val[i] - mx);
+      float n = 0.f, dot = 0.f;
+      for (int j = lane; j < k; j += 32) {
+        const float y = sh.q[j] - mx, e = sh.id[j] >= 0 ? expf(y) : 0.f;
+        n += e;
+        dot += e == 0.f ? 0.f : e * y;
+        sh.q[j] = e;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         n += __shfl_xor_sync(0xffffffffu, n, o);
         dot += __shfl_xor_sync(0xffffffffu, dot, o);
       }
-      const float inv = !a.opt.normalize ? 1.f : n == 0.f ? 0.f : 1.f / n;
-#pragma unroll
-      for (int i = 0; i < LR; ++i) {
-        if (i * 32 >= k) break;
-        sh.id[i * 32 + lane] = id[i];
-        sh.q[i * 32 + lane] = e[i] * inv;
+      if (a.opt.normalize) {
+        const float inv = n == 0.f ? 0.f : 1.f / n;
+        for (int j = lane; j < k; j += 32) sh.q[j] *= inv;
+        dot = n == 0.f ? 0.f : fmaf(dot, inv, -logf(n));
+        n *= inv;
       }
-      __syncwarp();
       if (lane < 4) {  // the entry after the last is the hard target; then none, up to a multiple of four
         sh.id[k + lane] = lane == 0 ? t : -1;
         sh.q[k + lane] = 0.f;
       }
       if (lane == 0) {
-        sh.sum = a.opt.normalize ? (n == 0.f ? 0.f : n * inv) : n;
-        sh.ent = a.opt.normalize ? (n == 0.f ? 0.f : fmaf(dot, inv, -logf(n))) : dot;
+        if (t >= 0) sh.x[k] = Elt<T>::get(x + t);
+        sh.sum = n;
+        sh.ent = dot;
       }
     }
+    fetch(r + step, t_n, weight_n);
 
-    Sums2 st = second == kNone ? w.template sums<kNone>(sp, xs, single >= 0, c)
-               : second == kSquare ? w.template sums<kSquare>(sp, xs, single >= 0, c)
-               : second == kFourth ? w.template sums<kFourth>(sp, xs, single >= 0, c)
-                                   : w.template sums<kOwn>(sp, xs, single >= 0, c);
+    Sums2 st = second == kNone ? distill_sums<kNone>(feed, taken, sp, xs, single >= 0, c, lane)
+               : second == kSquare ? distill_sums<kSquare>(feed, taken, sp, xs, single >= 0, c, lane)
+               : second == kFourth ? distill_sums<kFourth>(feed, taken, sp, xs, single >= 0, c, lane)
+                                   : distill_sums<kOwn>(feed, taken, sp, xs, single >= 0, c, lane);
     st.join_warp(c);
     if constexpr (NW > 1) {
       if (lane == 0) sh.red[warp] = st.pack();
@@ -1126,54 +1071,28 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, distill_blocks(NW * TEAMS)) d
       if (parts > 1) {
         if (!entered) { cg::this_cluster().barrier_wait(); entered = true; }  // the other blocks run: their memory may be written
         if (tid < parts) *cg::this_cluster().map_shared_rank(&sh.part[part], tid) = st.pack();
-        cg::this_cluster().sync();
+        cg::this_cluster().sync();  // (also: every block has read its logits at the alternatives)
         st = lane < parts ? Sums2(sh.part[lane]) : Sums2();
         st.join_warp(c);
       }
     } else {
       __syncwarp();
     }
-    // the alternatives and the target that lie in this block's part of the row, and their logits
-    int idx[ROUNDS];
-    float xj[ROUNDS];
-#pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const int j = i * NW * 32 + tid;
-      idx[i] = -1;
-      xj[i] = 0.f;
-      if (i * NW * 32 > k) continue;
-      if (j <= k) idx[i] = sh.id[j];
-      if (idx[i] >= 0 && !sp.has(idx[i], part, parts)) idx[i] = -1;
-      if (idx[i] >= 0) {
-        const int v = idx[i] - sp.head;
-        xj[i] = v < 0 ? sh.single[idx[i]] : idx[i] >= sp.tail ? sh.single[8 + idx[i] - sp.tail]
-                : Elt<T>::get(reinterpret_cast<const T*>(buf) + (v - sp.lo * Elt<T>::VEC));
-      }
-    }
     // a row without weight, or with nothing left, has no part in the loss, whatever else it holds
     const bool none = weight == 0.f || st.s == 0.f;
     if (second == kNone) st.h = st.s;
-    const float ln_s = logf(st.s), ln_h = second == kNone ? ln_s : logf(st.h);
-    auto log_p = [&](float v, float scale, float ln) { return fmaf(v - st.m, scale, -ln); };
-    float loss = 0.f;
+    if (part == 0 && lead) {
+      const float ln_s = logf(st.s), ln_h = second == kNone ? ln_s : logf(st.h);
+      float loss = 0.f;
+      for (int j = lane; j <= k; j += 32) {
+        const bool hard = j == k;
+        if (sh.id[j] < 0 || (hard ? false : sh.q[j] == 0.f || kd == 0.f)) continue;
+        const float w = hard ? ce : kd * sh.q[j];
+        loss -= w * fmaf(sh.x[j] - st.m, hard && second != kNone ? 1.f : s, -(hard ? ln_h : ln_s));
+      }
 #pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const int j = i * NW * 32 + tid;
-      if (idx[i] < 0) continue;
-      if (j == k) loss -= ce * log_p(xj[i], second == kNone ? s : 1.f, ln_h);
-      else if (sh.q[j] != 0.f && kd != 0.f) loss -= kd * sh.q[j] * log_p(xj[i], s, ln_s);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-    if constexpr (NW > 1) {
-      if (lane == 0) sh.slots[warp] = loss;
-      __syncthreads();  // (also: every thread has read its logits)
-      loss = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) loss += sh.slots[i];
-      if (parts > 1 && tid == 0) *cg::this_cluster().map_shared_rank(&sh.loss[part], 0) = loss;
-    } else {
-      __syncwarp();
+      for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+      if (lane == 0) a.loss_rows[r] = none ? 0.f : weight * fmaf(kd, sh.ent, loss);
     }
     const float gs = a.opt.grad_scale * weight, wq = gs * kd * s, wc = gs * ce;
     auto write = [&](auto tag) {
@@ -1183,42 +1102,31 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, distill_blocks(NW * TEAMS)) d
       float f, f1;
       ex.settle(f, f1);
       const float ff = (SECOND == kNone ? fmaf(wq, sh.sum, wc) : wq * sh.sum) * f / st.s, fc = SECOND == kNone ? 0.f : wc * f1 / st.h;
-      w.template gradient<SECOND>(sp, x, d, none, ex, ff, fc, next, nsp);
-      if (!d) return;
+      distill_gradient<SECOND>(feed, taken, sp, x, d, none, ex, ff, fc, lane);
       if (single >= 0) Elt<T>::put(d + single, none ? 0.f : ex.grad(xs, ff, fc));
       team_sync<NW>();  // the elements below are written a second time, by other threads
-#pragma unroll
-      for (int i = 0; i < ROUNDS; ++i) {
-        if (i * NW * 32 > k) break;
-        if (idx[i] < 0 || none) continue;
+      for (int j = tid; j <= k && !none; j += NW * 32) {
+        const int i = sh.id[j];
+        if (i < 0 || !sp.has(i, part, parts)) continue;
         float q = 0.f;
-        for (int j = 0; j < k; j += 4) {  // (the target's q is 0)
-          const int4 ids = *reinterpret_cast<const int4*>(&sh.id[j]);
-          const float4 qs = *reinterpret_cast<const float4*>(&sh.q[j]);
-          q += (ids.x == idx[i] ? qs.x : 0.f) + (ids.y == idx[i] ? qs.y : 0.f) + (ids.z == idx[i] ? qs.z : 0.f) +
-               (ids.w == idx[i] ? qs.w : 0.f);
+        for (int l = 0; l < k; l += 4) {  // (the target's q is 0)
+          const int4 ids = *reinterpret_cast<const int4*>(&sh.id[l]);
+          const float4 qs = *reinterpret_cast<const float4*>(&sh.q[l]);
+          q += (ids.x == i ? qs.x : 0.f) + (ids.y == i ? qs.y : 0.f) + (ids.z == i ? qs.z : 0.f) + (ids.w == i ? qs.w : 0.f);
         }
-        Elt<T>::put(d + idx[i], ex.grad(xj[i], ff, fc) - wq * q - (idx[i] == t ? wc : 0.f));
+        Elt<T>::put(d + i, ex.grad(sh.x[j], ff, fc) - wq * q - (i == t ? wc : 0.f));
       }
     };
-    if (second == kNone) write(std::integral_constant<int, kNone>());
-    else if (second == kSquare) write(std::integral_constant<int, kSquare>());
-    else if (second == kFourth) write(std::integral_constant<int, kFourth>());
-    else write(std::integral_constant<int, kOwn>());
-    if (parts > 1) {
-      cg::this_cluster().sync();
-      if (part == 0 && tid == 0) {
-        loss = 0.f;
-        for (int q = 0; q < parts; ++q) loss += sh.loss[q];
-      }
+    if (d) {
+      if (second == kNone) write(std::integral_constant<int, kNone>());
+      else if (second == kSquare) write(std::integral_constant<int, kSquare>());
+      else if (second == kFourth) write(std::integral_constant<int, kFourth>());
+      else write(std::integral_constant<int, kOwn>());
     }
-    if (part == 0 && tid == 0) a.loss_rows[r] = none ? 0.f : weight * fmaf(kd, sh.ent, loss);
-    sp = nsp;
     t = t_n;
     weight = weight_n;
-#pragma unroll
-    for (int i = 0; i < LR; ++i) { id[i] = id_n[i]; val[i] = val_n[i]; }
     team_sync<NW>();
+    if (parts > 1) cg::this_cluster().sync();  // this row's sums are read: the next row's may come
   }
   if (!entered) cg::this_cluster().barrier_wait();
 }
@@ -1242,10 +1150,25 @@ __global__ void __launch_bounds__(1024) scaled_sum_kernel(const float* __restric
 }
 
 // ------------------------------------------------------------------ host side
-// Blocks that share a row: more while the rows alone leave SMs idle and each block keeps at least 2048 logits.
-int row_parts(int rows, int vocab) {
+// Warps to a row: as many as let all rows run at once (24 warps on an SM), if each has a piece of its own; with
+// more rows than that one warp where a row is short, four where it is 16 pieces or longer, whose rows would leave
+// SMs idle at the end.  Measured, log probabilities: 2400 x 6400 17 us with one, 22 / 25 / 41 us with 2 / 4 / 8;
+// 1021 x 50001 35 us with two, 39 / 41 us with 4 / 8; 600 x 50001 25 us with four, 29 us with 2 or 8; 2048 x 32000
+// 45 us with four, 56 us with one.  Distillation: 32768 x 6400 201 us with one, 280 / 303 us with 2 / 4; 2048 x
+// 32000 66 us with four, 84 / 74 us with 1 / 8; 500 x 50001 39 us with four, 54 / 42 us with 2 / 8.
+int team_warps(int rows, int pieces) {
+  const int64_t room = 24 * (int64_t)sm_count_current();
+  if (rows > room / 2) return pieces >= 16 ? 4 : 1;
+  int nw = 1;
+  while (nw < 8 && (int64_t)rows * 2 * nw <= room && pieces >= 2 * nw) nw *= 2;
+  return nw;
+}
+// Blocks of eight warps to a row: more while all still run at once and each warp has a piece.  Log probabilities:
+// 64 x 131072 21 / 15 / 13 / 22 us with 1 / 2 / 4 / 8; 1 x 131072 19 / 15 / 13 / 11 us.  Distillation: 64 x 262139
+// fp32 82 / 54 / 42 / 50 us; 100 x 100003 31 / 27 / 24 / 35 us.
+int team_parts(int rows, int pieces) {
   int p = 1;
-  while (p < kMaxParts && (int64_t)rows * p < 2 * sm_count_current() && vocab / (2 * p) >= 2048) p *= 2;
+  while (p < kMaxParts && (int64_t)rows * 2 * p * 8 <= 24 * (int64_t)sm_count_current() && pieces >= 14 * p) p *= 2;
   return p;
 }
 
@@ -1300,11 +1223,11 @@ zl_status launch_rows(const char* what, K kern, int rows, int parts, zl_stream s
 template <typename T, int NW, int TEAMS, typename K>
 zl_status launch_distill(const char* what, K kern, zl_stream s, const DistillArgs& a) {
   static std::atomic<uint64_t> done{0};
-  const size_t smem = (size_t)TEAMS * a.pieces * (kPieceBytes + 8);
+  const size_t smem = (size_t)TEAMS * NW * kDepth * kPieceBytes;
   const cudaError_t e = allow_dynamic(kern, done);
   if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(distill_blocks(NW * TEAMS), (227 * 1024) / (smem + sizeof(DistillShared<NW>) * TEAMS + 2048)));
-  const int64_t rows = ((int64_t)a.rows + TEAMS - 1) / TEAMS, room = std::max<int64_t>(1, per_sm * sm_count_current() / a.parts);
+  const int64_t rows = ((int64_t)a.rows + TEAMS - 1) / TEAMS;
+  const int64_t room = std::max<int64_t>(1, 24 / (NW * TEAMS) * sm_count_current() / a.parts);
   return launch(what, kern, std::min(rows, room) * a.parts, NW * TEAMS * 32, a.parts, smem, s, a);
 }
 
@@ -1332,27 +1255,15 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   if (top_k > 0 && !top_ids) return set_error(ZL_EINVAL, "token_logprobs: null top_ids");
   if (rows == 0) return ZL_OK;
   LogprobArgs a{logits, stride, targets, rows, vocab, top_k, 1, 0, scale, logp, entropy, lse, top_logp, top_ids};
-  const int vecs = vocab / Elt<T>::VEC + 1, sms = sm_count_current();
+  const int vecs = vocab / Elt<T>::VEC + 1;
   a.pieces = (vecs + kPieceVecs - 1) / kPieceVecs;
-  // Warps to a row: as many as let all rows run at once (24 warps on an SM), if each has a piece of its own; with
-  // more rows than that one warp where a row is short, four where it is 16 pieces or longer, whose rows would
-  // leave SMs idle at the end (measured: 2400 x 6400 17 us with one, 22 / 25 / 41 us with 2 / 4 / 8; 1021 x 50001
-  // 35 us with two, 39 / 41 us with 4 / 8; 600 x 50001 25 us with four, 29 us with 2 or 8; 2048 x 32000 45 us with
-  // four, 56 us with one).
-  const int64_t room = 24 * (int64_t)sms;
-  int nw = 1;
-  if (rows > room / 2) nw = a.pieces >= 16 ? 4 : 1;
-  else
-    while (nw < 8 && rows * 2 * nw <= room && a.pieces >= 2 * nw) nw *= 2;
+  int nw = team_warps(rows, a.pieces);
   // the vectors' maxima of a row fit beside the rings, and a single warp has 128 groups
   while (nw < 8 && (vecs > 4096 * nw || (nw == 1 && top_k > 96))) nw *= 2;
   if (nw == 1) return launch_rows<T, 1, 4>("token_logprobs", logprobs_kernel<T, 1, 4>, rows, 1, s, a);
   if (nw == 2) return launch_rows<T, 2, 1>("token_logprobs", logprobs_kernel<T, 2, 1>, rows, 1, s, a);
   if (nw == 4) return launch_rows<T, 4, 1>("token_logprobs", logprobs_kernel<T, 4, 1>, rows, 1, s, a);
-  // blocks to a row: while all still run at once and each warp has a piece (64 x 131072: 21 / 15 / 13 / 22 us with
-  // 1 / 2 / 4 / 8; 1 x 131072: 19 / 15 / 13 / 11 us)
-  const int pieces = a.pieces;
-  while (a.parts < kMaxParts && rows * 2 * (int64_t)a.parts * 8 <= room && pieces >= 14 * a.parts) a.parts *= 2;
+  a.parts = team_parts(rows, a.pieces);
   for (;; a.parts *= 2) {
     a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
     if (logprobs_smem<T, 8, 1>(a) <= kMaxDynamic) break;
@@ -1404,22 +1315,14 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
     return set_error(ZL_EINVAL, "%s: a gradient in the logits' place has their row stride", what);
   if (rows > 0 && !loss_rows) return set_error(ZL_EINVAL, "%s: null loss_rows", what);
   if (rows > 0) {
-    DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, 1, 0, *opt, d, d_stride, loss_rows};
-    const int vecs = vocab / Elt<T>::VEC + 1;
-    int nw = getenv("ZL_DI_NW") ? atoi(getenv("ZL_DI_NW")) : 8;
-    a.parts = getenv("ZL_DI_PARTS") ? atoi(getenv("ZL_DI_PARTS")) : 1;
-    for (;; a.parts *= 2) {
-      a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
-      if ((size_t)a.pieces * (kPieceBytes + 8) <= kMaxDynamic) break;
-      if (a.parts == kMaxParts) return set_error(ZL_EUNSUPPORTED, "%s: vocab too large", what);
-    }
-    if (a.parts > 1 && nw < 8) nw = 8;
-    while (nw < 4 && a.pieces > 24 * nw) nw *= 2;
+    DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, 1, *opt, d, d_stride, loss_rows};
+    const int pieces = (vocab / Elt<T>::VEC + kPieceVecs) / kPieceVecs;
+    const int nw = team_warps(rows, pieces);
+    if (nw == 8) a.parts = team_parts(rows, pieces);
     if (nw == 1) st = launch_distill<T, 1, 4>(what, distill_kernel<T, 1, 4>, s, a);
     else if (nw == 2) st = launch_distill<T, 2, 1>(what, distill_kernel<T, 2, 1>, s, a);
     else if (nw == 4) st = launch_distill<T, 4, 1>(what, distill_kernel<T, 4, 1>, s, a);
-    else if (nw == 8) st = launch_distill<T, 8, 1>(what, distill_kernel<T, 8, 1>, s, a);
-    else st = launch_distill<T, 16, 1>(what, distill_kernel<T, 16, 1>, s, a);
+    else st = launch_distill<T, 8, 1>(what, distill_kernel<T, 8, 1>, s, a);
     if (st != ZL_OK) return st;
   }
   if (!loss_out) return ZL_OK;
