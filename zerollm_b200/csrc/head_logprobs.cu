@@ -23,60 +23,116 @@ bool make_tma_map(CUtensorMap* map, const void* ptr, bool is_f32, uint64_t inner
 namespace {
 constexpr int BM = 128, BN = 256, BK = 64;   // rows of a CTA, vocabulary entries of a tile, reduction block
 constexpr int kEpiWarps = 8, kThreads = 64 + kEpiWarps * 32;
-constexpr int kStages = 6;
-constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of the weight, in one stage
-constexpr int kStageBytes = 2 * kTileBytes;
-constexpr int kBarOff = kStages * kStageBytes;
-constexpr int kSmem = kBarOff + 256 + 1024;  // barriers, alignment slack
+constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of the weight, in one reduction block
+// A short reduction (up to kHeld blocks) keeps the row tile of hidden in shared memory from one vocabulary tile to the
+// next; its ring holds weight blocks.  A longer one streams both through a ring of pairs.
+constexpr int kHeld = 8;
+template <bool HELD> struct Smem {
+  static constexpr int STAGES = HELD ? 5 : 6;
+  static constexpr int STAGE_BYTES = HELD ? kTileBytes : 2 * kTileBytes;
+  static constexpr int RING = HELD ? kHeld * kTileBytes : 0;  // offset of the ring
+  static constexpr int BARS = RING + STAGES * STAGE_BYTES;
+  static constexpr int TOTAL = BARS + 512 + 1024;  // barriers, alignment slack
+};
 
-// Work: (row tile, vocabulary tile) steps, row tile by row tile; pair p takes the steps [p per, (p + 1) per).
-// A row tile's steps fall to the pairs first .. last, each of which writes one partial (slot p - first).
 int pair_slots();  // CTA pairs that the current device runs at once
 
+// Work: (row tile, vocabulary tile) steps in segments of one row tile and some consecutive vocabulary tiles; each
+// segment leaves one partial per row.
+//  * group = 0 (the weight fits into L2): steps are numbered row tile by row tile and pair p takes the steps
+//    [p per, (p + 1) per), the same number each; a row tile's steps fall to the pairs first .. last, slot p - first.
+//  * group > 0 (it does not): segments of `group` vocabulary tiles, row tiles running fastest, pair p takes every
+//    pairs-th.  All pairs work on the same few vocabulary tiles at a time, so the weight comes from memory once, not
+//    once per row tile (16384 x 2048 x 32000: see below).  Slot: the group.
 struct Plan {
-  int row_tiles, n_tiles, pairs, slots;
+  int row_tiles, n_tiles, pairs, slots, group;
   int64_t steps, per;
 };
-Plan make_plan(int rows, int vocab) {
+Plan make_plan(int rows, int dim, int vocab) {
   Plan p;
   p.row_tiles = (rows + 2 * BM - 1) / (2 * BM);
   p.n_tiles = (vocab + BN - 1) / BN;
   p.steps = (int64_t)p.row_tiles * p.n_tiles;
   p.pairs = (int)std::min<int64_t>(p.steps, pair_slots());
-  p.per = p.pairs ? (p.steps + p.pairs - 1) / p.pairs : 0;
-  p.slots = p.per ? (int)std::min<int64_t>(p.pairs, (p.n_tiles - 1) / p.per + 2) : 0;
+  p.per = (p.steps + p.pairs - 1) / p.pairs;
+  p.group = 0;
+  if ((int64_t)vocab * dim * 2 > (int64_t)40 << 20 && p.row_tiles > 1) {
+    // rounds of segments, a segment's steps and a tenth for its partials
+    double best = 1e30;
+    for (int g = 1; g <= std::min(p.n_tiles, 16); ++g) {
+      const int64_t units = (int64_t)p.row_tiles * ((p.n_tiles + g - 1) / g);
+      const double t = (double)((units + p.pairs - 1) / p.pairs) * (g + 0.1);
+      if (t < best) { best = t; p.group = g; }
+    }
+  }
+  p.slots = p.group ? (p.n_tiles + p.group - 1) / p.group : (int)std::min<int64_t>(p.pairs, (p.n_tiles - 1) / p.per + 2);
   return p;
 }
 
 struct HeadArgs {
   const int32_t* targets;
-  int rows, vocab, k_blocks, n_tiles, slots;
+  int rows, vocab, k_blocks, row_tiles, n_tiles, slots, group;
   int64_t steps, per;
   float c;  // scale * log2(e)
   float4* partials;  // [row][slot][half] (m, S0, S1, target logit)
 };
 
+// The segments of a pair, one after the other.
+struct Segments {
+  int64_t at, end;
+  int pair, pairs;
+  int rt, nt0, nt1, slot;
+  __device__ __forceinline__ Segments(const HeadArgs& a, int p, int n) : pair(p), pairs(n) {
+    at = a.group ? p : p * a.per;
+    end = a.group ? (int64_t)a.row_tiles * a.slots : min(a.steps, (p + 1) * a.per);
+  }
+  __device__ __forceinline__ bool next(const HeadArgs& a) {
+    if (at >= end) return false;
+    if (a.group) {
+      rt = (int)(at % a.row_tiles);
+      slot = (int)(at / a.row_tiles);
+      nt0 = slot * a.group;
+      nt1 = min(a.n_tiles, nt0 + a.group);
+      at += pairs;
+    } else {
+      rt = (int)(at / a.n_tiles);
+      slot = pair - (int)((int64_t)rt * a.n_tiles / a.per);
+      nt0 = (int)(at % a.n_tiles);
+      nt1 = (int)min((int64_t)a.n_tiles, nt0 + (end - at));
+      at += nt1 - nt0;
+    }
+    return true;
+  }
+};
+
+template <bool HELD>
 __global__ void __launch_bounds__(kThreads, 1)
     head_logprobs_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
                          const HeadArgs a) {
+  using L = Smem<HELD>;
+  constexpr int STAGES = L::STAGES;
   constexpr uint32_t IDESC = make_idesc(1, 2 * BM, BN, 0, 0);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* h_full = acc_empty + 2;  // [kHeld] the held blocks of hidden
+  uint64_t* h_empty = h_full + kHeld;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(h_empty + kHeld);
+  static_assert((2 * STAGES + 4 + 2 * kHeld + 1) * 8 <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int64_t s0 = (int64_t)(blockIdx.x >> 1) * a.per, s1 = min(a.steps, s0 + a.per);
+  Segments seg(a, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1));
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kEpiWarps * 32); }
+    for (int i = 0; i < kHeld; ++i) { mbar_init(&h_full[i], 1); mbar_init(&h_empty[i], 1); }
     fence_mbar_init();
     tma_prefetch_desc(&tmH);
     tma_prefetch_desc(&tmW);
@@ -95,47 +151,62 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
       int stage = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, h_phase = 0;
       bool ok = true;
-      for (int64_t s = s0; s < s1 && ok; ++s) {
-        const int m0 = (int)(s / a.n_tiles) * (2 * BM) + (int)rank * BM;
-        const int n0 = (int)(s % a.n_tiles) * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < a.k_blocks; ++kb) {
-          if (!bounded_wait(&empty[stage], phase ^ 1u, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
-          uint8_t* sA = smem + stage * kStageBytes;
-          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);  // the even CTA's barrier
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kStageBytes);
-          tma_load_2d_pair(sA, &tmH, bar, kb * BK, m0);
-          tma_load_2d_pair(sA + kTileBytes, &tmW, bar, kb * BK, n0);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      while (ok && seg.next(a)) {
+        const int m0 = seg.rt * (2 * BM) + (int)rank * BM;
+        for (int nt = seg.nt0; nt < seg.nt1 && ok; ++nt) {
+          const int n0 = nt * BN + (int)rank * (BN / 2);
+          for (int kb = 0; kb < a.k_blocks; ++kb) {
+            if (HELD && nt == seg.nt0) {
+              // block kb of the new row tile, as soon as the last product with the old one is done
+              if (!bounded_wait(&h_empty[kb], h_phase ^ 1u, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
+              if (leader) mbar_arrive_expect_tx(&h_full[kb], 2 * kTileBytes);
+              tma_load_2d_pair(smem + kb * kTileBytes, &tmH, mapa_shared(smem_u32(&h_full[kb]), 0), kb * BK, m0);
+            }
+            if (!bounded_wait(&empty[stage], phase ^ 1u, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
+            uint8_t* st = smem + L::RING + stage * L::STAGE_BYTES;
+            const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);  // the even CTA's barrier
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * L::STAGE_BYTES);
+            if (!HELD) tma_load_2d_pair(st + kTileBytes, &tmH, bar, kb * BK, m0);
+            tma_load_2d_pair(st, &tmW, bar, kb * BK, n0);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          }
         }
+        h_phase ^= 1u;
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (even CTA only)
     if (leader) {
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      uint32_t phase = 0, acc_phase = 0, h_phase = 0;
       bool ok = true;
-      for (int64_t s = s0; s < s1 && ok; ++s) {
-        // both CTAs' epilogues have drained accumulator `acc`
-        if (!__all_sync(0xffffffffu, bounded_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, DEV_TIMEOUT_ACC))) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-        for (int kb = 0; kb < a.k_blocks; ++kb) {
-          if (!bounded_wait_warp(&full[stage], phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+      while (ok && seg.next(a)) {
+        for (int nt = seg.nt0; nt < seg.nt1 && ok; ++nt) {
+          // both CTAs' epilogues have drained accumulator `acc`
+          if (!__all_sync(0xffffffffu, bounded_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, DEV_TIMEOUT_ACC))) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_base = smem_u32(smem + stage * kStageBytes), b_base = a_base + kTileBytes;
+          const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+          for (int kb = 0; kb < a.k_blocks; ++kb) {
+            if (HELD && nt == seg.nt0 && !bounded_wait_warp(&h_full[kb], h_phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+            if (!bounded_wait_warp(&full[stage], phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t w_base = smem_u32(smem + L::RING + stage * L::STAGE_BYTES);
+            const uint32_t h_base = HELD ? smem_u32(smem + kb * kTileBytes) : w_base + kTileBytes;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            umma_f16_pair_w(d_tmem, smem_desc_sw128(a_base + k * 32, 16, 1024), smem_desc_sw128(b_base + k * 32, 16, 1024),
-                            IDESC, (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit_pair_w(&empty[stage], 0x3);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+            for (int k = 0; k < BK / 16; ++k)
+              umma_f16_pair_w(d_tmem, smem_desc_sw128(h_base + k * 32, 16, 1024), smem_desc_sw128(w_base + k * 32, 16, 1024),
+                              IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+            umma_commit_pair_w(&empty[stage], 0x3);
+            if (HELD && nt + 1 == seg.nt1) umma_commit_pair_w(&h_empty[kb], 0x3);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          }
+          if (!ok) break;
+          umma_commit_pair_w(&acc_full[acc], 0x3);
+          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
-        if (!ok) break;
-        umma_commit_pair_w(&acc_full[acc], 0x3);
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        h_phase ^= 1u;
       }
     }
   } else {
@@ -144,47 +215,43 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t acc_empty_leader[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
     int acc = 0;
     uint32_t acc_phase = 0;
-    Running run;
-    float xt = 0.f;
-    int row = 0, t = -1;
-    for (int64_t s = s0; s < s1; ++s) {
-      const int rt = (int)(s / a.n_tiles), nt = (int)(s % a.n_tiles);
-      if (s == s0 || nt == 0) {  // a segment begins
-        row = rt * (2 * BM) + (int)rank * BM + quarter * 32 + lane;
-        t = (a.targets && row < a.rows) ? a.targets[row] : -1;
-        run = Running();
-        xt = 0.f;
-      }
-      if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) break;
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
+    bool ok = true;
+    while (ok && seg.next(a)) {
+      const int row = seg.rt * (2 * BM) + (int)rank * BM + quarter * 32 + lane;
+      const int t = (a.targets && row < a.rows) ? a.targets[row] : -1;
+      Running run;
+      float xt = 0.f;
+      for (int nt = seg.nt0; nt < seg.nt1; ++nt) {
+        if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
 #pragma unroll 1
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        uint32_t u[32];
-        tmem_ld32(t_row + (uint32_t)c, u);
-        tmem_ld_wait();
-        float v[32];
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+          const int n = nt * BN + c;
+          if (n >= a.vocab) break;
+          uint32_t u[32];
+          tmem_ld32(t_row + (uint32_t)c, u);
+          tmem_ld_wait();
+          float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
-        const int n = nt * BN + c;
-        if (n >= a.vocab) break;
-        if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
+          if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
+          }
+          if (t >= n && t < n + 32 && t < a.vocab) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
+          }
+          run.add_any(v, a.c);
         }
-        if (t >= n && t < n + 32 && t < a.vocab) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
-        }
-        run.add_any(v, a.c);
+        tc_fence_before();
+        mbar_arrive_cluster(acc_empty_leader[acc]);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      tc_fence_before();
-      mbar_arrive_cluster(acc_empty_leader[acc]);
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-      if ((s + 1 == s1 || nt + 1 == a.n_tiles) && row < a.rows) {  // it ends: this pair's partial of the row
-        const int slot = (int)((int64_t)(blockIdx.x >> 1) - (int64_t)rt * a.n_tiles / a.per);
+      if (ok && row < a.rows) {  // this pair's partial of the row
         const Stats st = run.sums(a.c);
-        a.partials[((int64_t)row * a.slots + slot) * 2 + half] = make_float4(st.m, st.s0, st.s1, xt);
+        a.partials[((int64_t)row * a.slots + seg.slot) * 2 + half] = make_float4(st.m, st.s0, st.s1, xt);
       }
     }
   }
@@ -199,11 +266,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-cudaLaunchConfig_t pair_config(int pairs, cudaStream_t st, cudaLaunchAttribute* attr) {
+cudaLaunchConfig_t pair_config(int pairs, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr->id = cudaLaunchAttributeClusterDimension;
   attr->val.clusterDim.x = 2;
@@ -225,9 +292,10 @@ int pair_slots() {
   int n = found[dev].load();
   if (n == 0) {
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = pair_config(sms, nullptr, &attr);
-    if (cudaFuncSetAttribute(head_logprobs_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, head_logprobs_kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaLaunchConfig_t cfg = pair_config(sms, Smem<true>::TOTAL, nullptr, &attr);
+    if (cudaFuncSetAttribute(head_logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<true>::TOTAL) != cudaSuccess ||
+        cudaFuncSetAttribute(head_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<false>::TOTAL) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, head_logprobs_kernel<true>, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       return sms;
     }
@@ -243,7 +311,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadArgs a, float 
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= a.rows) return;
   const int64_t rt = row / (2 * BM);
-  const int n = 2 * (int)(((rt + 1) * a.n_tiles - 1) / a.per - rt * a.n_tiles / a.per + 1);
+  const int n = 2 * (a.group ? a.slots : (int)(((rt + 1) * a.n_tiles - 1) / a.per - rt * a.n_tiles / a.per + 1));
   Stats s;
   float xt = 0.f;
   for (int i = lane; i < n; i += 32) {
@@ -281,7 +349,7 @@ using namespace zl;
 
 extern "C" int64_t zl_linear_logprobs_workspace_floats(int rows, int dim, int vocab) {
   if (rows <= 0 || dim <= 0 || vocab <= 0) return 0;
-  return (int64_t)rows * make_plan(rows, vocab).slots * 8;
+  return (int64_t)rows * make_plan(rows, dim, vocab).slots * 8;
 }
 
 extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf16* weight, const int32_t* targets, int rows,
@@ -296,16 +364,19 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
   if (!hidden || !weight || !workspace) return set_error(ZL_EINVAL, "%s: null hidden, weight or workspace", what);
   if ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return set_error(ZL_EINVAL, "%s: hidden, weight and workspace must be 16-byte aligned", what);
-  const Plan p = make_plan(rows, vocab);
+  const Plan p = make_plan(rows, dim, vocab);
   CUtensorMap mh, mw;
   if (!make_tma_map(&mh, hidden, false, dim, rows, BK, BM, 128, 0) ||
       !make_tma_map(&mw, weight, false, dim, vocab, BK, BN / 2, 128, 0))
     return set_error(ZL_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
-  HeadArgs a{targets, rows, vocab, (dim + BK - 1) / BK, p.n_tiles, p.slots, p.steps, p.per, scale * kLog2e,
-             reinterpret_cast<float4*>(workspace)};
+  HeadArgs a{targets, rows, vocab, (dim + BK - 1) / BK, p.row_tiles, p.n_tiles, p.slots, p.group, p.steps, p.per,
+             scale * kLog2e, reinterpret_cast<float4*>(workspace)};
+  const bool held = a.k_blocks <= kHeld;
   cudaLaunchAttribute attr;
-  const cudaLaunchConfig_t cfg = pair_config(p.pairs, (cudaStream_t)stream, &attr);  // (make_plan has set the kernel's attribute)
-  cudaError_t e = cudaLaunchKernelEx(&cfg, head_logprobs_kernel, mh, mw, a);
+  const cudaLaunchConfig_t cfg = pair_config(p.pairs, held ? Smem<true>::TOTAL : Smem<false>::TOTAL, (cudaStream_t)stream, &attr);
+  // (make_plan has set the kernels' shared-memory attributes)
+  cudaError_t e = held ? cudaLaunchKernelEx(&cfg, head_logprobs_kernel<true>, mh, mw, a)
+                       : cudaLaunchKernelEx(&cfg, head_logprobs_kernel<false>, mh, mw, a);
   if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
   head_join_kernel<<<(rows + 7) / 8, 256, 0, (cudaStream_t)stream>>>(a, scale, logp, entropy, lse);
   return check_launch(what);
