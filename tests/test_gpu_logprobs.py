@@ -611,7 +611,8 @@ def check_head(L, h, w, scale=1.0, t=None):
 @pytest.mark.parametrize("rows,dim,vocab", [(1, 8, 1), (1, 64, 2), (2, 512, 6400), (7, 72, 300), (8, 2048, 32000), (9, 520, 1000),
                                             (33, 200, 257), (128, 128, 640), (129, 512, 255), (256, 64, 256), (257, 576, 513),
                                             (300, 1032, 1025), (1000, 512, 6400), (5000, 64, 130), (40, 264, 20011), (1, 1000, 100003),
-                                            (300, 512, 45001), (600, 2048, 12000), (2000, 504, 3001)])
+                                            (300, 512, 45001), (600, 2048, 12000), (2000, 504, 3001),
+                                            (8, 8, 15), (5, 24, 17), (3, 8192, 333), (8, 8200, 100), (6, 1048, 50007)])
 def test_linear_logprobs_sizes(L, rows, dim, vocab):
     g = torch.Generator(device="cuda").manual_seed(rows + dim)
     h = torch.randn(rows, dim, device="cuda", generator=g).bfloat16()

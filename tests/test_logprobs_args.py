@@ -116,10 +116,14 @@ def test_linear_logprobs_refusals(L):
 
 
 def test_linear_logprobs_workspace(L):
-    """A partial (four floats, two column halves) of every row for each pair that can meet its row tile: at least
-    one, no more than the vocabulary has tiles of 256 (one more where segments do not begin with the row tile)."""
+    """A partial (four floats, two halves of a tile's columns) of every row for each pair of SMs that can meet its row
+    tile: at least one, no more than the vocabulary has tiles of 256 (one more where segments do not begin with the row
+    tile).  Up to eight rows: one for each block of 128 vocabulary entries, at most two blocks an SM."""
     f = L.load().zl_linear_logprobs_workspace_floats
-    for rows, vocab in [(1, 1), (1, 32000), (300, 6400), (32768, 6400), (16384, 32000)]:
+    for rows, vocab in [(300, 6400), (32768, 6400), (16384, 32000)]:
         n = f(rows, 512, vocab)
         assert n % (rows * 8) == 0 and 1 <= n // (rows * 8) <= (vocab + 255) // 256 + 1
+    for rows, vocab in [(1, 1), (1, 32000), (8, 6400)]:
+        n = f(rows, 512, vocab)
+        assert n % (rows * 4) == 0 and 1 <= n // (rows * 4) <= (vocab + 127) // 128
     assert f(0, 512, 100) == 0

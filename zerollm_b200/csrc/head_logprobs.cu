@@ -22,7 +22,8 @@ bool make_tma_map(CUtensorMap* map, const void* ptr, bool is_f32, uint64_t inner
 
 namespace {
 constexpr int BM = 128, BN = 256, BK = 64;   // rows of a CTA, vocabulary entries of a tile, reduction block
-constexpr int kEpiWarps = 8, kThreads = 64 + kEpiWarps * 32;
+constexpr int kEpiWarps = 8, kShares = kEpiWarps / 4;  // epilogue warps; those that share a row, each its columns of a tile
+constexpr int kThreads = 64 + kEpiWarps * 32;
 constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of the weight, in one reduction block
 // A short reduction (up to kHeld blocks) keeps the row tile of hidden in shared memory from one vocabulary tile to the
 // next; its ring holds weight blocks.  A longer one streams both through a ring of pairs.
@@ -74,7 +75,8 @@ struct HeadArgs {
   int rows, vocab, k_blocks, row_tiles, n_tiles, slots, group;
   int64_t steps, per;
   float c;  // scale * log2(e)
-  float4* partials;  // [row][slot][half] (m, S0, S1, target logit)
+  int few;           // few rows: partials of a row, one of each block
+  float4* partials;  // [row][slot][share] (m, S0, S1, target logit)
 };
 
 // The segments of a pair, one after the other.
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------ epilogue (both CTAs, own half of the rows)
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, share = (warp - 2) >> 2;
     const uint32_t acc_empty_leader[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
 #pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+        for (int c = share * (BN / kShares); c < (share + 1) * (BN / kShares); c += 32) {
           const int n = nt * BN + c;
           if (n >= a.vocab) break;
           uint32_t u[32];
@@ -237,13 +239,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
           if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : kClamp;
           }
           if (t >= n && t < n + 32 && t < a.vocab) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
           }
-          run.add_any(v, a.c);
+          run.add_near(v, a.c);
         }
         tc_fence_before();
         mbar_arrive_cluster(acc_empty_leader[acc]);
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok && row < a.rows) {  // this pair's partial of the row
         const Stats st = run.sums(a.c);
-        a.partials[((int64_t)row * a.slots + seg.slot) * 2 + half] = make_float4(st.m, st.s0, st.s1, xt);
+        a.partials[((int64_t)row * a.slots + seg.slot) * kShares + share] = make_float4(st.m, st.s0, st.s1, xt);
       }
     }
   }
@@ -305,20 +307,124 @@ int pair_slots() {
   return n;
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 8 rows: the weight is read once, at the rate of device memory, and tensor-core tiles of 256 rows would be
+// empty.  Every warp takes tiles of 16 vocabulary entries: mma.m16n8k16 with the weight's rows as A, straight from
+// device memory to registers, and the rows of hidden as B, from shared memory.  The order of the reduction index is
+// free as long as both operands use the same one, so a lane's 16-byte load of 8 consecutive elements of one weight row
+// serves as its A registers of two products.  A lane has the logits of 2 entries x 2 rows and folds them into the
+// statistics of these rows; a block leaves one partial per row.
+constexpr int kFewRows = 8, kFewWarps = 8, kFewBlocks = 2, kFewDim = 8192;  // (hidden: up to 128 KB of shared memory)
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
+    head_few_kernel(const __nv_bfloat16* __restrict__ hidden, const __nv_bfloat16* __restrict__ weight, int dim, const HeadArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint4* h = reinterpret_cast<uint4*>(smem_raw);  // [block of 32][row of 8][quad of 4]: 8 elements each, 0 past the ends
+  __shared__ float4 part[kFewWarps][kFewRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int blocks = (dim + 31) / 32, vecs = dim / 8;
+  for (int i = threadIdx.x; i < blocks * 32; i += kFewWarps * 32) {
+    const int r = (i >> 2) & 7, v = (i >> 5) * 4 + (i & 3);
+    h[i] = r < a.rows && v < vecs ? __ldg(reinterpret_cast<const uint4*>(hidden + (int64_t)r * dim) + v) : make_uint4(0, 0, 0, 0);
+  }
+  int t[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) t[i] = a.targets && 2 * q + i < a.rows ? a.targets[2 * q + i] : -1;
+  __syncthreads();
+  Running run[2];
+  float xt[2] = {0.f, 0.f};
+  let_follow();
+  const int tiles = (a.vocab + 15) / 16, step = gridDim.x * kFewWarps;
+  for (int tile = warp * gridDim.x + blockIdx.x; tile < tiles; tile += step) {  // (spread over all SMs)
+    const int n0 = tile * 16 + g, n1 = n0 + 8;  // this lane's weight rows (the last one again past the end)
+    const uint4* w0 = reinterpret_cast<const uint4*>(weight + (int64_t)min(n0, a.vocab - 1) * dim) + q;
+    const uint4* w1 = reinterpret_cast<const uint4*>(weight + (int64_t)min(n1, a.vocab - 1) * dim) + q;
+    float d[2][4] = {};
+    auto product = [&](const uint4& u0, const uint4& u1, int b) {
+      const uint4 x = h[(b * 8 + g) * 4 + q];
+      mma_16816(d[0], u0.x, u1.x, u0.y, u1.y, x.x, x.y);
+      mma_16816(d[1], u0.z, u1.z, u0.w, u1.w, x.z, x.w);
+    };
+    constexpr int U = 8;
+    const int whole = vecs / 4;  // blocks of 32 elements without an end inside
+    int b = 0;
+    for (; b + U <= whole; b += U) {
+      uint4 u0[U], u1[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        u0[i] = __ldg(w0 + (b + i) * 4);
+        u1[i] = __ldg(w1 + (b + i) * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) product(u0[i], u1[i], b + i);
+    }
+    for (; b < blocks; ++b) {
+      const bool in = b * 4 + q < vecs;
+      product(in ? __ldg(w0 + b * 4) : make_uint4(0, 0, 0, 0), in ? __ldg(w1 + b * 4) : make_uint4(0, 0, 0, 0), b);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x0 = d[0][i] + d[1][i], x1 = d[0][2 + i] + d[1][2 + i];
+      if (n0 < a.vocab) {
+        run[i].add_one(x0, a.c);
+        if (t[i] == n0) xt[i] = x0;
+      }
+      if (n1 < a.vocab) {
+        run[i].add_one(x1, a.c);
+        if (t[i] == n1) xt[i] = x1;
+      }
+    }
+  }
+  // a row's statistics are in the eight lanes of one q
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    Stats s = run[i].sums(a.c);
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      Stats p;
+      p.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+      p.s0 = __shfl_xor_sync(0xffffffffu, s.s0, o);
+      p.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
+      s.join(p, a.c);
+      xt[i] += __shfl_xor_sync(0xffffffffu, xt[i], o);
+    }
+    if (g == 0) part[warp][2 * q + i] = make_float4(s.m, s.s0, s.s1, xt[i]);
+  }
+  __syncthreads();
+  if (threadIdx.x < kFewRows && threadIdx.x < a.rows) {
+    Stats s;
+    float x = 0.f;
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float4 p = part[w][threadIdx.x];
+      s.join(Stats(make_float3(p.x, p.y, p.z)), a.c);
+      x += p.w;
+    }
+    a.partials[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float4(s.m, s.s0, s.s1, x);
+  }
+}
+int few_blocks(int vocab) {
+  return std::min((vocab + 16 * kFewWarps - 1) / (16 * kFewWarps), kFewBlocks * sm_count_current());
+}
+
 // One warp per row: its partials joined in a fixed order.
 __global__ void __launch_bounds__(256) head_join_kernel(const HeadArgs a, float scale, float* __restrict__ logp,
                                                         float* __restrict__ entropy, float* __restrict__ lse) {
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  follows();
   if (row >= a.rows) return;
   const int64_t rt = row / (2 * BM);
-  const int n = 2 * (a.group ? a.slots : (int)(((rt + 1) * a.n_tiles - 1) / a.per - rt * a.n_tiles / a.per + 1));
+  const int n = a.few ? a.few : kShares * (a.group ? a.slots : (int)(((rt + 1) * a.n_tiles - 1) / a.per - rt * a.n_tiles / a.per + 1));
   Stats s;
   float xt = 0.f;
   for (int i = lane; i < n; i += 32) {
-    const float4 p = a.partials[(int64_t)row * a.slots * 2 + i];
-    Stats o;
-    o.m = p.x; o.s0 = p.y; o.s1 = p.z;
-    s.join(o, a.c);
+    const float4 p = a.partials[(int64_t)row * (a.few ? a.few : a.slots * kShares) + i];
+    s.join(Stats(make_float3(p.x, p.y, p.z)), a.c);
     xt += p.w;
   }
   s.join_warp(a.c);
@@ -349,7 +455,8 @@ using namespace zl;
 
 extern "C" int64_t zl_linear_logprobs_workspace_floats(int rows, int dim, int vocab) {
   if (rows <= 0 || dim <= 0 || vocab <= 0) return 0;
-  return (int64_t)rows * make_plan(rows, dim, vocab).slots * 8;
+  if (rows <= kFewRows && dim <= kFewDim) return (int64_t)rows * few_blocks(vocab) * 4;
+  return (int64_t)rows * make_plan(rows, dim, vocab).slots * kShares * 4;
 }
 
 extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf16* weight, const int32_t* targets, int rows,
@@ -364,13 +471,23 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
   if (!hidden || !weight || !workspace) return set_error(ZL_EINVAL, "%s: null hidden, weight or workspace", what);
   if ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return set_error(ZL_EINVAL, "%s: hidden, weight and workspace must be 16-byte aligned", what);
+  if (rows <= kFewRows && dim <= kFewDim) {
+    HeadArgs a{targets, rows, vocab, 0, 0, 0, 0, 0, 0, 0, scale * kLog2e, few_blocks(vocab), reinterpret_cast<float4*>(workspace)};
+    const size_t smem = (size_t)(dim + 31) / 32 * 512;
+    cudaError_t e = cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewDim / 32 * 512);
+    if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+    head_few_kernel<<<a.few, kFewWarps * 32, smem, (cudaStream_t)stream>>>(reinterpret_cast<const __nv_bfloat16*>(hidden),
+                                                                           reinterpret_cast<const __nv_bfloat16*>(weight), dim, a);
+    const zl_status st = check_launch(what);
+    return st != ZL_OK ? st : launch_after(what, head_join_kernel, 1, 256, (cudaStream_t)stream, a, scale, logp, entropy, lse);
+  }
   const Plan p = make_plan(rows, dim, vocab);
   CUtensorMap mh, mw;
   if (!make_tma_map(&mh, hidden, false, dim, rows, BK, BM, 128, 0) ||
       !make_tma_map(&mw, weight, false, dim, vocab, BK, BN / 2, 128, 0))
     return set_error(ZL_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
   HeadArgs a{targets, rows, vocab, (dim + BK - 1) / BK, p.row_tiles, p.n_tiles, p.slots, p.group, p.steps, p.per,
-             scale * kLog2e, reinterpret_cast<float4*>(workspace)};
+             scale * kLog2e, 0, reinterpret_cast<float4*>(workspace)};
   const bool held = a.k_blocks <= kHeld;
   cudaLaunchAttribute attr;
   const cudaLaunchConfig_t cfg = pair_config(p.pairs, held ? Smem<true>::TOTAL : Smem<false>::TOTAL, (cudaStream_t)stream, &attr);
@@ -378,6 +495,5 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
   cudaError_t e = held ? cudaLaunchKernelEx(&cfg, head_logprobs_kernel<true>, mh, mw, a)
                        : cudaLaunchKernelEx(&cfg, head_logprobs_kernel<false>, mh, mw, a);
   if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  head_join_kernel<<<(rows + 7) / 8, 256, 0, (cudaStream_t)stream>>>(a, scale, logp, entropy, lse);
-  return check_launch(what);
+  return launch_after(what, head_join_kernel, (rows + 7) / 8, 256, (cudaStream_t)stream, a, scale, logp, entropy, lse);
 }

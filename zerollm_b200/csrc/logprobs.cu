@@ -1136,6 +1136,7 @@ __global__ void __launch_bounds__(1024) scaled_sum_kernel(const float* __restric
                                                           float* __restrict__ out) {
   __shared__ double red[32];
   double s = 0.0;
+  follows();
   for (int i = threadIdx.x; i < n; i += 1024) s += v[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -1326,8 +1327,7 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
     if (st != ZL_OK) return st;
   }
   if (!loss_out) return ZL_OK;
-  scaled_sum_kernel<<<1, 1024, 0, (cudaStream_t)s>>>(loss_rows, rows, opt->grad_scale, loss_out);
-  return check_launch("distill_topk loss");
+  return launch_after(what, scaled_sum_kernel, 1, 1024, (cudaStream_t)s, (const float*)loss_rows, rows, opt->grad_scale, loss_out);
 }
 }  // namespace
 

@@ -12,6 +12,25 @@ constexpr float kFloor = -1000.f;  // a log2 probability this low has p = 0; sta
 
 inline bool bad_scale(float s) { return !(s >= 1e-4f && s <= 1e4f); }
 
+// A kernel launched by launch_after() may start while the one before it in the stream still runs; follows() waits
+// until that one is done and its results are seen.  let_follow(): this kernel's successor may start from here on.
+__device__ __forceinline__ void follows() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename K, typename... A>
+zl_status launch_after(const char* what, K kern, int blocks, int threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? ZL_OK : set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 __device__ __forceinline__ float ex2(float t) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
@@ -98,8 +117,8 @@ template <bool ENTROPY> struct RunningT {
     m = most; mc = m * c;
     s0 = s.s0; s1 = s.s1;
   }
-  // N elements, none above m and none below kClamp: pairs of partial sums (paired fp32 instructions)
-  template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
+  // sums of N elements about m, none below kClamp: pairs of partial sums (paired fp32 instructions)
+  template <int N> __device__ __forceinline__ void fold(const float (&v)[N], float c, float& x0, float& x1) const {
     const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(-mc, -mc);
     uint64_t a0[2] = {0, 0}, a1[2] = {0, 0};
 #pragma unroll
@@ -113,10 +132,30 @@ template <bool ENTROPY> struct RunningT {
     }
     float x, y;
     f2_unpack(add2(a0[0], a0[1]), x, y);
-    s0 += x + y;
+    x0 = x + y;
     if (ENTROPY) {
       f2_unpack(add2(a1[0], a1[1]), x, y);
-      s1 += x + y;
+      x1 = x + y;
+    }
+  }
+  // N elements, none above m and none below kClamp
+  template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
+    float x0, x1 = 0.f;
+    fold(v, c, x0, x1);
+    s0 += x0;
+    s1 += x1;
+  }
+  // N elements, none below kClamp, whose maximum is only looked for where their sum says that it lies well above m (by
+  // 3 at least, in powers of two): m need not be the maximum for the sums to be exact, only near enough to it that
+  // neither they nor ln S0 - S1 / S0 lose digits.
+  template <int N> __device__ __forceinline__ void add_near(float (&v)[N], float c) {
+    float x0 = INFINITY, x1 = 0.f;
+    if (m >= kDeep) fold(v, c, x0, x1);
+    if (x0 <= 8.f * N) {
+      s0 += x0;
+      s1 += x1;
+    } else {
+      add_any(v, c);
     }
   }
   // one element of any value
