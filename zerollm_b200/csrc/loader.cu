@@ -212,11 +212,13 @@ extern "C" zl_status zl_loader_next_device(zl_loader* L, int32_t* d_ids, int32_t
   }
   {
     std::lock_guard<std::mutex> g(L->mu);
-    s->state = s->count > 0 ? 2 : 0;
+    s->state = *count > 0 ? 2 : 0;
     ++L->next_use;
   }
   L->cv.notify_all();
   if (e != cudaSuccess) return zl::set_error(ZL_ECUDA, "loader: %s", cudaGetErrorString(e));
-  if (s->count == 0) L->running = false;  // epoch over: the worker has returned
+  // epoch over: the worker has returned.  (*count, not the slot's: from the unlock above on the worker may be refilling
+  // the slot, with the empty batch that ends the epoch among others)
+  if (*count == 0) L->running = false;
   return ZL_OK;
 }
