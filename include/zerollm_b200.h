@@ -443,6 +443,20 @@ zl_status zl_model_set_optimizer(zl_model *m, const zl_adamw_config *opt);
  * rank's batch.  update=0 skips AdamW (gradients stay in the grad arena). */
 zl_status zl_model_train_step(zl_model *m, const int32_t *ids, const int32_t *targets, int batch, int seq_len,
                               float lr, int update, float *loss_out, zl_stream stream);
+/* A distillation step: zl_model_train_step with zl_distill_topk_bf16 in place of the cross-entropy, on a teacher's
+ * record of batch * seq rows (as zl_model_score of the teacher writes it, with normalize = 1, or as given
+ * log probabilities).  opt->grad_scale is usually 1 / (batch * seq); row_weight and loss_out may be NULL.  Runs
+ * without a graph. */
+zl_status zl_model_distill_step(zl_model *m, const int32_t *ids, const int32_t *teacher_ids, const float *teacher_logits,
+                                int top_k, const int32_t *targets, const float *row_weight,
+                                const zl_distill_options *opt, int batch, int seq_len, float lr, int update,
+                                float *loss_out, zl_stream stream);
+/* Forward and, for each of the batch * seq rows, the outputs of zl_token_logprobs_bf16.  With top_k = 0 no logits are
+ * formed (zl_linear_logprobs_bf16 on the head's input); with top_k > 0 they are those the training step rounds to
+ * bf16.  Leaves the activations of its forward, as zl_model_forward does. */
+zl_status zl_model_score(zl_model *m, const int32_t *ids, const int32_t *targets, int batch, int seq_len, float scale,
+                         int top_k, float *logp, float *entropy, float *lse, float *top_logp, int32_t *top_ids,
+                         zl_stream stream);
 /* Step as a CUDA graph (default on, single process): the second call with the same ids/targets/loss
  * pointers and shape captures zero_grad -> forward -> CE -> backward into a graph that later calls replay
  * (AdamW stays a separate launch so lr may change).  0 disables. */

@@ -427,7 +427,8 @@ def test_distill_sizes(L, rows, vocab, k, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("o", [dict(normalize=0), dict(kd=0.0), dict(ce=0.0), dict(ce=0.0, scale=0.3), dict(kd=0.0, scale=2.0),
-                               dict(scale=2.0, teacher_scale=3.0, normalize=0, gs=-3.0), dict(gs=0.0)])
+                               dict(scale=2.0, teacher_scale=3.0, normalize=0, gs=-3.0), dict(gs=0.0),
+                               dict(scale=0.25), dict(scale=0.5, kd=0.0)])
 @pytest.mark.parametrize("targets,weights", [(True, True), (True, False)])
 def test_distill_options(L, o, targets, weights, dtype):
     check_distill(L, make("normal", 5, 3001, dtype), dtype, 17, opts(L, **o), targets, weights, dup=True)

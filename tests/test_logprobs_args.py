@@ -127,3 +127,9 @@ def test_linear_logprobs_workspace(L):
         n = f(rows, 512, vocab)
         assert n % (rows * 4) == 0 and 1 <= n // (rows * 4) <= (vocab + 127) // 128
     assert f(0, 512, 100) == 0
+
+
+def test_model_entries_refuse_null_arguments(L):
+    o = L.DistillOptions(1.0, 1.0, 1, 0.5, 0.5, 1.0)
+    refused(L, "zl_model_distill_step", L.ZL_EINVAL, "null", None, A, A, A, 4, A, None, C.byref(o), 1, 128, 0.0, 1, None, None)
+    refused(L, "zl_model_score", L.ZL_EINVAL, "null", None, A, A, 1, 128, 1.0, 0, A, A, A, None, None, None)

@@ -243,6 +243,9 @@ int64_t step_workspace(const zl_model_config& c, int64_t T, int B_max) {
   w = std::max(w, zl_attention_workspace_floats(B_max, (int)(T / B_max), c.num_heads, d / c.num_heads));
   w = std::max(w, (int64_t)3 * d * zl_norm_bwd_blocks(T));  // dgamma | dbeta | bias column sums
   w = std::max(w, zl_colsum_workspace_floats(T, std::max(3 * d, F)));
+  for (int64_t r = 0; r < T; r += 256)  // scoring any number of tokens up to T (partials of row tiles of 256)
+    w = std::max(w, zl_linear_logprobs_workspace_floats((int)std::min(T, r + 256), d, V));
+  w = std::max(w, zl_linear_logprobs_workspace_floats((int)std::min<int64_t>(T, 8), d, V));
   return w;
 }
 
@@ -297,9 +300,8 @@ int64_t end_of_any(zl_model* M, std::initializer_list<int64_t> offs) {
 }
 
 // ----------------------------------------------------------------------------- forward
-// Runs the forward to the bf16 logits (kept in M->logits).  If logits_f32 is non-null the head GEMM
-// writes fp32 logits there instead.
-zl_status forward(zl_model* M, const int32_t* ids, int B, int S, float* logits_f32, cudaStream_t st) {
+// Runs the forward to the hidden states before the head (M->hf).
+zl_status forward_hidden(zl_model* M, const int32_t* ids, int B, int S, cudaStream_t st) {
   const zl_model_config& c = M->cfg;
   const int64_t T = (int64_t)B * S;
   const int d = c.embed_dim, F = c.ff_hidden_dim, V = c.vocab_size, H = c.num_heads;
@@ -354,14 +356,24 @@ zl_status forward(zl_model* M, const int32_t* ids, int B, int S, float* logits_f
   TRY(zl_norm_forward_bf16(c.norm, reinterpret_cast<zl_bf16*>(M->x[c.num_layers]), P(M, M->L.nog), P(M, M->L.nob),
                            reinterpret_cast<zl_bf16*>(M->hf), M->meanf, M->rstdf, T, d, c.eps, st));
   M->launches++;
-  const int64_t head_off = c.tied ? M->L.emb : M->L.head;
+  M->last_B = B;
+  M->last_S = S;
+  return ZL_OK;
+}
+
+// Runs the forward to the bf16 logits (kept in M->logits).  If logits_f32 is non-null the head GEMM
+// writes fp32 logits there instead.
+zl_status forward(zl_model* M, const int32_t* ids, int B, int S, float* logits_f32, cudaStream_t st) {
+  TRY(forward_hidden(M, ids, B, S, st));
+  const int64_t T = (int64_t)B * S;
+  const int d = M->cfg.embed_dim, V = M->cfg.vocab_size;
+  const int KK = ZL_A_KMAJOR | ZL_B_KMAJOR;
+  const int64_t head_off = M->cfg.tied ? M->L.emb : M->L.head;
   if (logits_f32) {
     TRY(gemm(M, M->hf, W(M, head_off), logits_f32, (int)T, V, d, KK, ZL_EPI_OUT_F32, nullptr, st));
   } else {
     TRY(gemm(M, M->hf, W(M, head_off), M->logits, (int)T, V, d, KK, 0, nullptr, st));
   }
-  M->last_B = B;
-  M->last_S = S;
   return ZL_OK;
 }
 
@@ -625,10 +637,19 @@ extern "C" zl_status zl_model_zero_grad(zl_model* M, zl_stream s) {
 }
 
 namespace {
-// zero_grad -> forward -> fused CE -> backward on `st` (gradient buckets are all-reduced on the
-// side stream as they become final when a communicator is attached).
+// A teacher's record for a distillation step.
+struct Teacher {
+  const int32_t* ids;
+  const float* logits;
+  int top_k;
+  const float* row_weight;
+  const zl_distill_options* opt;
+};
+
+// zero_grad -> forward -> fused CE (or distillation loss) -> backward on `st` (gradient buckets are
+// all-reduced on the side stream as they become final when a communicator is attached).
 zl_status step_body(zl_model* M, const int32_t* ids, const int32_t* targets, int B, int S, float* loss_out,
-                    cudaStream_t st) {
+                    cudaStream_t st, const Teacher* teacher = nullptr) {
   M->launches = 0;
   M->dist.next_bucket = 0;
   const size_t kt_step = 4 * (size_t)M->cfg.num_layers;  // step-phase events follow the per-layer ones
@@ -637,12 +658,38 @@ zl_status step_body(zl_model* M, const int32_t* ids, const int32_t* targets, int
   M->launches++;
   TRY(forward(M, ids, B, S, nullptr, st));
   const int64_t T = (int64_t)B * S;
-  TRY(zl_cross_entropy_fused_bf16(reinterpret_cast<zl_bf16*>(M->logits), targets, (int)T, M->cfg.vocab_size, 1e-8f,
-                                  1.0f / (float)T, M->loss_rows, loss_out, st));
+  zl_bf16* logits = reinterpret_cast<zl_bf16*>(M->logits);
+  if (teacher)
+    TRY(zl_distill_topk_bf16(logits, M->cfg.vocab_size, teacher->ids, teacher->logits, teacher->top_k, targets,
+                             teacher->row_weight, teacher->opt, (int)T, M->cfg.vocab_size, logits, M->cfg.vocab_size,
+                             M->loss_rows, loss_out, st));
+  else
+    TRY(zl_cross_entropy_fused_bf16(logits, targets, (int)T, M->cfg.vocab_size, 1e-8f, 1.0f / (float)T, M->loss_rows,
+                                    loss_out, st));
   M->launches += loss_out ? 2 : 1;
   TRY(backward(M, ids, B, S, st));
   if (!M->kt_ev.empty()) zl::record_timing_event(M->kt_ev[kt_step + 1], st);
   return ZL_OK;
+}
+
+// The end of a step whose gradients are under way: the exchange rejoins, AdamW where wanted.
+zl_status finish_step(zl_model* M, float lr, int update, cudaStream_t st) {
+  if (!M->kt_ev.empty()) {
+    // step end: once the gradient exchange on the side stream has rejoined this stream
+    if (M->dist.comm && !M->dist.joined) {
+      cudaEventRecord(M->dist.done_ev, M->dist.comm_stream);
+      cudaStreamWaitEvent(st, M->dist.done_ev, 0);
+      M->dist.joined = true;
+    }
+    zl::record_timing_event(M->kt_ev[4 * (size_t)M->cfg.num_layers + 2], st);
+    M->kt_valid = true;
+  }
+  if (update) TRY(adamw(M, lr, st));
+  else if (M->dist.comm && !M->dist.joined) {
+    cudaEventRecord(M->dist.done_ev, M->dist.comm_stream);
+    cudaStreamWaitEvent(st, M->dist.done_ev, 0);
+  }
+  return zl::check_launch("train_step");
 }
 
 // Replays (or captures, the second time a binding is seen) the step body as one CUDA graph.
@@ -775,22 +822,49 @@ extern "C" zl_status zl_model_train_step(zl_model* M, const int32_t* ids, const 
   M->dist.joined = false;
   if (M->use_graph) TRY(step_graph(M, ids, targets, B, S, loss_out, st));
   else TRY(step_body(M, ids, targets, B, S, loss_out, st));
-  if (!M->kt_ev.empty()) {
-    // step end: once the gradient exchange on the side stream has rejoined this stream
-    if (M->dist.comm && !M->dist.joined) {
-      cudaEventRecord(M->dist.done_ev, M->dist.comm_stream);
-      cudaStreamWaitEvent(st, M->dist.done_ev, 0);
-      M->dist.joined = true;
-    }
-    zl::record_timing_event(M->kt_ev[4 * (size_t)M->cfg.num_layers + 2], st);
-    M->kt_valid = true;
+  return finish_step(M, lr, update, st);
+}
+
+extern "C" zl_status zl_model_distill_step(zl_model* M, const int32_t* ids, const int32_t* teacher_ids,
+                                           const float* teacher_logits, int top_k, const int32_t* targets,
+                                           const float* row_weight, const zl_distill_options* opt, int B, int S, float lr,
+                                           int update, float* loss_out, zl_stream stream) {
+  if (!M || !ids || (top_k > 0 && (!teacher_ids || !teacher_logits))) return zl::set_error(ZL_EINVAL, "null argument");
+  TRY(check_shape(M, B, S));
+  const int V = M->cfg.vocab_size;
+  // (no rows: the checks of the options before anything runs)
+  TRY(zl_distill_topk_bf16(nullptr, V, teacher_ids, teacher_logits, top_k, targets, row_weight, opt, 0, V, nullptr, V,
+                           nullptr, nullptr, stream));
+  cudaStream_t st = (cudaStream_t)stream;
+  M->dist.joined = false;
+  const Teacher teacher{teacher_ids, teacher_logits, top_k, row_weight, opt};
+  TRY(step_body(M, ids, targets, B, S, loss_out, st, &teacher));
+  return finish_step(M, lr, update, st);
+}
+
+extern "C" zl_status zl_model_score(zl_model* M, const int32_t* ids, const int32_t* targets, int B, int S, float scale,
+                                    int top_k, float* logp, float* entropy, float* lse, float* top_logp, int32_t* top_ids,
+                                    zl_stream stream) {
+  if (!M || !ids) return zl::set_error(ZL_EINVAL, "null argument");
+  TRY(check_shape(M, B, S));
+  const int V = M->cfg.vocab_size, d = M->cfg.embed_dim, T = (int)((int64_t)B * S);
+  cudaStream_t st = (cudaStream_t)stream;
+  // (no rows: the checks of the arguments before anything runs)
+  TRY(zl_token_logprobs_bf16(nullptr, V, targets, 0, V, scale, top_k, logp, entropy, lse, top_logp, top_ids, st));
+  M->launches = 0;
+  if (top_k > 0) {
+    TRY(forward(M, ids, B, S, nullptr, st));
+    M->launches += 1;
+    return zl_token_logprobs_bf16(reinterpret_cast<zl_bf16*>(M->logits), V, targets, T, V, scale, top_k, logp, entropy, lse,
+                                  top_logp, top_ids, st);
   }
-  if (update) TRY(adamw(M, lr, st));
-  else if (M->dist.comm && !M->dist.joined) {
-    cudaEventRecord(M->dist.done_ev, M->dist.comm_stream);
-    cudaStreamWaitEvent(st, M->dist.done_ev, 0);
-  }
-  return zl::check_launch("train_step");
+  TRY(forward_hidden(M, ids, B, S, st));
+  if (zl_linear_logprobs_workspace_floats(T, d, V) > M->ws_floats)
+    return zl::set_error(ZL_ESTATE, "score: the model was made for another device");
+  M->launches += 2;
+  return zl_linear_logprobs_bf16(reinterpret_cast<zl_bf16*>(M->hf),
+                                 reinterpret_cast<const zl_bf16*>(W(M, M->cfg.tied ? M->L.emb : M->L.head)), targets, T, d, V,
+                                 scale, logp, entropy, lse, M->ws, st);
 }
 
 extern "C" zl_status zl_model_forward(zl_model* M, const int32_t* ids, int B, int S, float* logits, zl_stream stream) {

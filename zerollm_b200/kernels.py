@@ -8,6 +8,8 @@ oracle module so the same test drivers run both.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import torch
 
@@ -193,3 +195,37 @@ def sgd(p, g, vel, lr, momentum, wd):
     L.call("zl_sgd_step_f32", _p(pd), _p(gd), _p(vd), int(np.size(p)), lr, momentum, wd, None)
     torch.cuda.synchronize()
     return pd.cpu().numpy(), (vd.cpu().numpy() if vd is not None else None)
+
+
+def token_logprobs(x, targets, M, N, scale=1.0, top_k=0):
+    """(logp, entropy, lse) of M rows of N logits, and with top_k (top_logp, top_ids) [M, top_k] after them."""
+    xd, t = _dev(x), _dev(targets, torch.int32)
+    out = [_out(M) for _ in range(3)]
+    top = [_out(M * top_k), _out(M * top_k, torch.int32)] if top_k else [None, None]
+    L.call("zl_token_logprobs_f32", _p(xd), N, _p(t), M, N, scale, top_k, *map(_p, out), *map(_p, top), None)
+    if not top_k:
+        return _fin(*out)
+    r = _fin(*out, *top)
+    return r[:3] + (r[3].reshape(M, top_k), r[4].reshape(M, top_k))
+
+
+def token_logprobs_backward(x, targets, lse, entropy, g_logp, g_entropy, M, N, scale=1.0):
+    """dx of sum(g_logp logp + g_entropy entropy); g_entropy (and then entropy) may be None."""
+    xd, t, ls, gl, d = _dev(x), _dev(targets, torch.int32), _dev(lse), _dev(g_logp), _out(M * N)
+    en, ge = (None, None) if g_entropy is None else (_dev(entropy), _dev(g_entropy))
+    L.call("zl_token_logprobs_backward_f32", _p(xd), N, _p(t), _p(ls), _p(en), _p(gl), _p(ge), M, N, scale, _p(d), N, None)
+    return _fin(d)
+
+
+def distill_topk(x, teacher_ids, teacher_logits, top_k, targets, M, N, scale=1.0, teacher_scale=1.0, normalize=True,
+                 distill_weight=1.0, target_weight=0.0, grad_scale=1.0, row_weight=None):
+    """(loss rows, loss, dx) of the distillation loss of M rows of N logits."""
+    xd, i, v = _dev(x), _dev(teacher_ids, torch.int32), _dev(teacher_logits)
+    t = _dev(targets, torch.int32) if targets is not None else None
+    w = _dev(row_weight) if row_weight is not None else None
+    lr, lo, d = _out(M), _out(1), _out(M * N)
+    opt = L.DistillOptions(scale, teacher_scale, int(normalize), distill_weight, target_weight, grad_scale)
+    L.call("zl_distill_topk_f32", _p(xd), N, _p(i), _p(v), top_k, _p(t), _p(w), C.byref(opt), M, N, _p(d), N, _p(lr), _p(lo),
+           None)
+    rows, loss, dx = _fin(lr, lo, d)
+    return rows, float(loss[0]), dx

@@ -124,6 +124,8 @@ SIGNATURES = {
     "zl_model_params_updated": (i32, [vp, vp]),
     "zl_model_set_optimizer": (i32, [vp, C.POINTER(AdamWConfig)]),
     "zl_model_train_step": (i32, [vp, vp, vp, i32, i32, f32, i32, vp, vp]),
+    "zl_model_distill_step": (i32, [vp, vp, vp, vp, i32, vp, vp, C.POINTER(DistillOptions), i32, i32, f32, i32, vp, vp]),
+    "zl_model_score": (i32, [vp, vp, vp, i32, i32, f32, i32, vp, vp, vp, vp, vp, vp]),
     "zl_model_forward": (i32, [vp, vp, i32, i32, vp, vp]),
     "zl_model_backward": (i32, [vp, vp, vp, i32, i32, vp]),
     "zl_model_zero_grad": (i32, [vp, vp]),

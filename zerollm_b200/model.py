@@ -138,6 +138,36 @@ class ZeroLLM:
                self.loss_dev.data_ptr(), _stream(stream))
         return self.loss_dev
 
+    def distill_step(self, ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                     targets: torch.Tensor | None, B: int, S: int, lr: float, scale: float = 1.0,
+                     distill_weight: float = 1.0, target_weight: float = 0.0, normalize: bool = True,
+                     row_weight: torch.Tensor | None = None, update: bool = True, stream=None) -> torch.Tensor:
+        """train_step with the distillation loss on a teacher's record ([B * S, k] ids and logits, as `score` of the
+        teacher returns them), averaged over the rows.  Returns the device loss."""
+        k = teacher_ids.shape[-1]
+        assert teacher_ids.numel() == teacher_logits.numel() == B * S * k
+        opt = L.DistillOptions(scale, 1.0, int(normalize), distill_weight, target_weight, 1.0 / (B * S))
+        L.call("zl_model_distill_step", self.h, ids.data_ptr(), teacher_ids.data_ptr(), teacher_logits.data_ptr(), k,
+               None if targets is None else targets.data_ptr(), None if row_weight is None else row_weight.data_ptr(),
+               C.byref(opt), B, S, lr, int(update), self.loss_dev.data_ptr(), _stream(stream))
+        return self.loss_dev
+
+    def score(self, ids: torch.Tensor, targets: torch.Tensor | None, B: int, S: int, scale: float = 1.0, top_k: int = 0,
+              stream=None) -> dict:
+        """Log probabilities of `targets` (where given), entropy and log-sum-exp of each of the B * S rows, and with
+        top_k > 0 the top alternatives' ids and log probabilities [B * S, top_k]."""
+        n = B * S
+        out = {"entropy": torch.empty(n, device="cuda"), "lse": torch.empty(n, device="cuda")}
+        if targets is not None:
+            out["logp"] = torch.empty(n, device="cuda")
+        if top_k:
+            out["top_logp"] = torch.empty(n, top_k, device="cuda")
+            out["top_ids"] = torch.empty(n, top_k, dtype=torch.int32, device="cuda")
+        p = {k: v.data_ptr() for k, v in out.items()}
+        L.call("zl_model_score", self.h, ids.data_ptr(), None if targets is None else targets.data_ptr(), B, S, scale, top_k,
+               p.get("logp"), p["entropy"], p["lse"], p.get("top_logp"), p.get("top_ids"), _stream(stream))
+        return out
+
     def forward(self, ids: torch.Tensor, B: int, S: int, logits: torch.Tensor, stream=None):
         L.call("zl_model_forward", self.h, ids.data_ptr(), B, S, logits.data_ptr(), _stream(stream))
 

@@ -44,7 +44,12 @@ def _subset(tokens, offsets, begin, end):
 class Trainer:
     def __init__(self, cfg: Config, tokens: np.ndarray, offsets: np.ndarray, batch: int, seq: int, lr: float,
                  eos_id: int = 1, pad_id: int = 0, seed: int = 0, rank: int = 0, world: int = 1,
-                 local_rank: int = 0, bucket_bytes: int = 25 * 1024 * 1024, feed_depth: int = 3):
+                 local_rank: int = 0, bucket_bytes: int = 25 * 1024 * 1024, feed_depth: int = 3,
+                 teacher: str | None = None, teacher_top_k: int = 16, teacher_weight: float = 0.5,
+                 temperature: float = 1.0):
+        """teacher: a checkpoint directory (of the same configuration) to distill from; epochs then train on
+        teacher_weight * T^2 * KL(teacher's top k || student), both at temperature T, plus (1 - teacher_weight) *
+        cross-entropy."""
         self.rank, self.world = rank, world
         self.batch, self.seq, self.lr = batch, seq, lr
         torch.cuda.set_device(local_rank)
@@ -63,6 +68,11 @@ class Trainer:
             dist.broadcast_object_list(uid, src=0)
             # the library broadcasts rank 0's weights (train_zerollm_dp.cpp:335-341)
             self.model.attach_nccl(uid[0], rank, world, bucket_bytes)
+        self.teacher = None
+        if teacher is not None:
+            self.teacher = ZeroLLM(cfg, batch * seq, seed=seed)
+            self.teacher.load(teacher)
+            self.teacher_args = (int(teacher_top_k), float(teacher_weight), float(temperature))
         self.d_ids = torch.empty(batch * seq, dtype=torch.int32, device="cuda")
         self.d_tg = torch.empty_like(self.d_ids)
         self.step_no = 0
@@ -92,7 +102,7 @@ class Trainer:
             n = self.train_data.next_device(self.d_ids, self.d_tg)
             if n < self.batch:  # short last batch (or end of data): skipped
                 break
-            loss = self.model.train_step(self.d_ids, self.d_tg, self.batch, self.seq, self.lr)
+            loss = self.train_step()
             self.step_no += 1
             done += 1
             if done % log_every == 0 or done == steps:
@@ -104,6 +114,16 @@ class Trainer:
                                     "tokens_per_s": round(done * self.batch * self.seq * self.world / dt, 1)}))
         self.train_data.reset()  # stops the feed
         return float(np.mean(losses)) if losses else float("nan")
+
+    def train_step(self) -> torch.Tensor:
+        """One step on the batch in d_ids / d_tg; returns the device loss."""
+        if self.teacher is None:
+            return self.model.train_step(self.d_ids, self.d_tg, self.batch, self.seq, self.lr)
+        k, weight, temperature = self.teacher_args
+        rec = self.teacher.score(self.d_ids, None, self.batch, self.seq, 1.0 / temperature, k)
+        return self.model.distill_step(self.d_ids, rec["top_ids"], rec["top_logp"], self.d_tg, self.batch, self.seq, self.lr,
+                                       scale=1.0 / temperature, distill_weight=weight * temperature ** 2,
+                                       target_weight=1.0 - weight)
 
     def validate(self, max_batches: int = 8) -> float:
         """Mean loss over the rank's validation stories (a step without the weight update).  Every rank
@@ -129,6 +149,8 @@ class Trainer:
         self.train_data.close()
         self.valid_data.close()
         self.model.close()
+        if self.teacher is not None:
+            self.teacher.close()
 
 
 def main(argv=None):
@@ -147,6 +169,10 @@ def main(argv=None):
     ap.add_argument("--log-every", type=int, default=10)
     ap.add_argument("--save", default=None, help="checkpoint directory written by rank 0 at the end")
     ap.add_argument("--resume", default=None, help="checkpoint directory (with optimizer state) to start from")
+    ap.add_argument("--teacher", default=None, help="checkpoint directory of a teacher of the same configuration")
+    ap.add_argument("--teacher-top-k", type=int, default=16, help="alternatives of a token that the teacher passes on")
+    ap.add_argument("--teacher-weight", type=float, default=0.5, help="weight of the teacher's loss beside the targets'")
+    ap.add_argument("--temperature", type=float, default=1.0)
     args = ap.parse_args(argv)
     rank, world = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1))
     local_rank = int(os.environ.get("LOCAL_RANK", 0))
@@ -161,7 +187,8 @@ def main(argv=None):
     else:
         tokens, offsets = synthetic_stories(args.synthetic, args.seq, cfg.vocab_size, args.seed)
     tr = Trainer(cfg, tokens, offsets, args.batch, args.seq, args.lr, args.eos, args.pad, args.seed, rank, world,
-                 local_rank)
+                 local_rank, teacher=args.teacher, teacher_top_k=args.teacher_top_k, teacher_weight=args.teacher_weight,
+                 temperature=args.temperature)
     if args.resume:
         tr.model.load(args.resume, with_optimizer=True)
     for ep in range(args.epochs):
