@@ -307,6 +307,13 @@ int pair_slots() {
   return n;
 }
 
+// The tensor core cuts each step of 16 products to fp32 toward zero, so a logit comes out too small in magnitude by a
+// part that grows with the number of steps: measured against 64-bit sums 1.1e-7 to 3.6e-7 of it at dim 256, 1.3e-6 to
+// 5.4e-6 at 2048, 3.1e-6 to 1.4e-5 at 4096 (signs at random, shifted, or all alike), which is 0.12 to 0.9 of 2^-24 a
+// step.  Like a temperature, that moves every row's entropy the same way.  The scale makes up for 0.2 of 2^-24 a step;
+// logits of random signs then keep their random part alone (entropy of 16384 x 2048 x 32000: 1.7e-6 off without it).
+float scale_of(float scale, int dim) { return (float)(scale * (1.0 + 0.2 * ((dim + 15) / 16) * 0x1p-24)); }
+
 // ------------------------------------------------------------------ few rows
 // Up to 8 rows: the weight is read once, at the rate of device memory, and tensor-core tiles of 256 rows would be
 // empty.  Every warp takes tiles of 16 vocabulary entries: mma.m16n8k16 with the weight's rows as A, straight from
@@ -345,11 +352,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
     const int n0 = tile * 16 + g, n1 = n0 + 8;  // this lane's weight rows (the last one again past the end)
     const uint4* w0 = reinterpret_cast<const uint4*>(weight + (int64_t)min(n0, a.vocab - 1) * dim) + q;
     const uint4* w1 = reinterpret_cast<const uint4*>(weight + (int64_t)min(n1, a.vocab - 1) * dim) + q;
-    float d[2][4] = {};
-    auto product = [&](const uint4& u0, const uint4& u1, int b) {
+    float d[4][4] = {};  // (four sums of a quarter of the products each: a quarter of the steps that cut one)
+    auto product = [&](const uint4& u0, const uint4& u1, int b, int half) {
       const uint4 x = h[(b * 8 + g) * 4 + q];
-      mma_16816(d[0], u0.x, u1.x, u0.y, u1.y, x.x, x.y);
-      mma_16816(d[1], u0.z, u1.z, u0.w, u1.w, x.z, x.w);
+      mma_16816(d[half], u0.x, u1.x, u0.y, u1.y, x.x, x.y);
+      mma_16816(d[half + 1], u0.z, u1.z, u0.w, u1.w, x.z, x.w);
     };
     constexpr int U = 8;
     const int whole = vecs / 4;  // blocks of 32 elements without an end inside
@@ -362,15 +369,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
         u1[i] = __ldg(w1 + (b + i) * 4);
       }
 #pragma unroll
-      for (int i = 0; i < U; ++i) product(u0[i], u1[i], b + i);
+      for (int i = 0; i < U; ++i) product(u0[i], u1[i], b + i, i % 2 * 2);
     }
     for (; b < blocks; ++b) {
       const bool in = b * 4 + q < vecs;
-      product(in ? __ldg(w0 + b * 4) : make_uint4(0, 0, 0, 0), in ? __ldg(w1 + b * 4) : make_uint4(0, 0, 0, 0), b);
+      product(in ? __ldg(w0 + b * 4) : make_uint4(0, 0, 0, 0), in ? __ldg(w1 + b * 4) : make_uint4(0, 0, 0, 0), b, 0);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float x0 = d[0][i] + d[1][i], x1 = d[0][2 + i] + d[1][2 + i];
+      const float x0 = (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]), x1 = (d[0][2 + i] + d[1][2 + i]) + (d[2][2 + i] + d[3][2 + i]);
       if (n0 < a.vocab) {
         run[i].add_one(x0, a.c);
         if (t[i] == n0) xt[i] = x0;
@@ -385,13 +392,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     Stats s = run[i].sums(a.c);
+    float M = s.m;  // (one common maximum, then one rescaling: each costs an exponential's rounding)
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    s.rebase(M, a.c);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
-      Stats p;
-      p.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-      p.s0 = __shfl_xor_sync(0xffffffffu, s.s0, o);
-      p.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
-      s.join(p, a.c);
+      s.s0 += __shfl_xor_sync(0xffffffffu, s.s0, o);
+      s.s1 += __shfl_xor_sync(0xffffffffu, s.s1, o);
       xt[i] += __shfl_xor_sync(0xffffffffu, xt[i], o);
     }
     if (g == 0) part[warp][2 * q + i] = make_float4(s.m, s.s0, s.s1, xt[i]);
@@ -400,9 +408,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
   if (threadIdx.x < kFewRows && threadIdx.x < a.rows) {
     Stats s;
     float x = 0.f;
+    for (int w = 0; w < kFewWarps; ++w) s.m = fmaxf(s.m, part[w][threadIdx.x].x);
     for (int w = 0; w < kFewWarps; ++w) {
       const float4 p = part[w][threadIdx.x];
-      s.join(Stats(make_float3(p.x, p.y, p.z)), a.c);
+      Stats o(make_float3(p.x, p.y, p.z));
+      o.rebase(s.m, a.c);
+      s.s0 += o.s0;
+      s.s1 += o.s1;
       x += p.w;
     }
     a.partials[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = make_float4(s.m, s.s0, s.s1, x);
@@ -420,16 +432,25 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadArgs a, float 
   if (row >= a.rows) return;
   const int64_t rt = row / (2 * BM);
   const int n = a.few ? a.few : kShares * (a.group ? a.slots : (int)(((rt + 1) * a.n_tiles - 1) / a.per - rt * a.n_tiles / a.per + 1));
+  const float4* parts = a.partials + (int64_t)row * (a.few ? a.few : a.slots * kShares);
   Stats s;
   float xt = 0.f;
+  for (int i = lane; i < n; i += 32) s.m = fmaxf(s.m, parts[i].x);
+  s.m = max_warp(s.m);
   for (int i = lane; i < n; i += 32) {
-    const float4 p = a.partials[(int64_t)row * (a.few ? a.few : a.slots * kShares) + i];
-    s.join(Stats(make_float3(p.x, p.y, p.z)), a.c);
+    const float4 p = parts[i];
+    Stats o(make_float3(p.x, p.y, p.z));
+    o.rebase(s.m, a.c);
+    s.s0 += o.s0;
+    s.s1 += o.s1;
     xt += p.w;
   }
-  s.join_warp(a.c);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) xt += __shfl_xor_sync(0xffffffffu, xt, o);
+  for (int o = 16; o > 0; o >>= 1) {
+    s.s0 += __shfl_xor_sync(0xffffffffu, s.s0, o);
+    s.s1 += __shfl_xor_sync(0xffffffffu, s.s1, o);
+    xt += __shfl_xor_sync(0xffffffffu, xt, o);
+  }
   if (lane) return;
   const float ln_s0 = logf(s.s0), h = fmaf(-kLn2, s.s1 / s.s0, ln_s0);
   const int t = a.targets ? a.targets[row] : -1;
@@ -482,6 +503,7 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
     return st != ZL_OK ? st : launch_after(what, head_join_kernel, 1, 256, (cudaStream_t)stream, a, scale, logp, entropy, lse);
   }
   const Plan p = make_plan(rows, dim, vocab);
+  scale = scale_of(scale, dim);
   CUtensorMap mh, mw;
   if (!make_tma_map(&mh, hidden, false, dim, rows, BK, BM, 128, 0) ||
       !make_tma_map(&mw, weight, false, dim, vocab, BK, BN / 2, 128, 0))

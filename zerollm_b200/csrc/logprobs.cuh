@@ -77,14 +77,6 @@ struct Stats {
     s0 *= f;
     m = M;
   }
-  __device__ __forceinline__ void join(const Stats& o, float c) {
-    Stats a = o;
-    const float M = fmaxf(m, o.m);
-    rebase(M, c);
-    a.rebase(M, c);
-    s0 += a.s0;
-    s1 += a.s1;
-  }
   __device__ __forceinline__ void join_warp(float c) {
     rebase(max_warp(m), c);
 #pragma unroll
