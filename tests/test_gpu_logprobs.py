@@ -74,6 +74,8 @@ def make(kind, rows, vocab, dtype, pad=0, offset=0, seed=0):
         v.masked_fill_(torch.rand(vocab, device="cuda", generator=g) < 0.4, low)
         v[rows // 2] = low
         v[:, 0] = torch.where(v[:, 0] == low, v[:, 0], v[:, 0])
+    elif kind == "highest":                                   # one token forced with the type's highest value
+        v[:, vocab // 3] = torch.finfo(DT[dtype]).max
     elif kind == "constant":
         v.fill_(-2.5)
     elif kind == "ties":                                      # few distinct values, both zeros among them
@@ -178,7 +180,7 @@ def test_token_logprobs_sizes(L, rows, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("kind", ["masked", "few", "lowest", "constant", "ties", "sorted", "sharp", "column"])
+@pytest.mark.parametrize("kind", ["masked", "few", "lowest", "highest", "constant", "ties", "sorted", "sharp", "column"])
 @pytest.mark.parametrize("rows,vocab,k", [(3, 900, 20), (3, 6400, 16), (7, 6400, 128), (1, 33333, 50), (2, 140000, 64),
                                           (1200, 900, 20), (1201, 6400, 64), (2500, 5003, 1)])
 def test_token_logprobs_values(L, rows, vocab, k, kind, dtype):
@@ -230,7 +232,7 @@ def call_backward(L, x, dtype, t, lse, ent, gl, ge, scale, d):
 
 def backward64(x, t, lse, ent, gl, ge, scale):
     rows, vocab = x.shape
-    none = (lse < -1e30)[:, None]   # rows masked wholly, with -inf or with the type's lowest value
+    none = (lse.abs() > 1e30)[:, None]   # rows masked wholly, or with a token forced by the type's highest value
     logp = torch.where(none, torch.full((), NINF, device="cuda", dtype=torch.float64), x.double() * scale - lse.double()[:, None])
     p = logp.exp()
     g = torch.zeros(rows, device="cuda", dtype=torch.float64) if gl is None else gl.double()
@@ -254,7 +256,7 @@ def backward64(x, t, lse, ent, gl, ge, scale):
 @pytest.mark.parametrize("rows,vocab,pad,offset,dpad,kind", [
     (1, 1, 0, 0, 0, "normal"), (3, 7, 0, 1, 0, "normal"), (5, 257, 3, 0, 3, "normal"), (3, 6400, 0, 0, 0, "masked"),
     (4, 6401, 0, 0, 0, "normal"), (3, 6400, 13, 0, 0, "normal"), (3, 5003, 13, 2, 5, "masked"), (2, 40001, 0, 0, 0, "sharp"),
-    (3, 2000, 0, 0, 0, "few"), (3, 2000, 0, 0, 0, "lowest")])
+    (3, 2000, 0, 0, 0, "few"), (3, 2000, 0, 0, 0, "lowest"), (3, 2000, 0, 0, 0, "highest")])
 @pytest.mark.parametrize("which", ["logp", "entropy", "both"])
 def test_token_logprobs_backward(L, rows, vocab, pad, offset, dpad, kind, dtype, which):
     scale = C.c_float(0.7).value
@@ -389,6 +391,7 @@ def check_distill(L, x, dtype, k, o, targets=True, weights=True, dup=False, dpad
         clean[3, :5] = 0
     loss, want, size, flush, (weight, away) = distill64(clean, ids, v, t, w, o)
     E, lnv = err(vocab, dtype), math.log(vocab) + 1
+    loss = torch.where(loss > torch.finfo(torch.float32).max, torch.full_like(loss, math.inf), loss)  # (beyond an fp32 output)
     # each ln p is off by E + 4u (ln vocab + |ln p|), each q by 8u |ln q| + 132 u (its sum); products of both
     close(lr, loss, 2 * weight * E + 4 * U * lnv * weight + 160 * U * away * 4 + 1e-30, "loss_rows")
     if torch.isfinite(loss).all():
@@ -435,7 +438,7 @@ def test_distill_options(L, o, targets, weights, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("kind", ["masked", "few", "lowest", "constant", "sharp"])
+@pytest.mark.parametrize("kind", ["masked", "few", "lowest", "highest", "constant", "sharp"])
 @pytest.mark.parametrize("vocab", [900, 6400, 40001])
 def test_distill_values(L, kind, vocab, dtype):
     x = make(kind, 5, vocab, dtype)

@@ -41,6 +41,9 @@ def test_token_logprobs_refusals(L, t):
     refused(L, n, bad, "top_k", *args(k=101))
     refused(L, n, L.ZL_EUNSUPPORTED, "top_k", *args(k=129, vocab=200, stride=200))
     refused(L, n, bad, "top_ids", *args(ids=None))
+    refused(L, n, bad, "4-byte", *args(tg=A + 2))
+    refused(L, n, bad, "4-byte", *args(ids=A + 1))
+    refused(L, n, L.ZL_EUNSUPPORTED, "2^30", *args(vocab=(1 << 30) + 1, stride=1 << 31))
     assert getattr(L.load(), n)(*args(rows=0, x=None)) == L.ZL_OK
 
 
@@ -61,6 +64,7 @@ def test_token_logprobs_backward_refusals(L, t):
     refused(L, n, bad, "element boundary", *args(d=A + 1))
     refused(L, n, bad, "targets", *args(tg=None))
     refused(L, n, bad, "entropies", *args(ent=None))
+    refused(L, n, bad, "4-byte", *args(gl=A + 2))
     refused(L, n, bad, "row stride", *args(d=A, ds=101))
     assert getattr(L.load(), n)(*args(rows=0, x=None, d=None, lse=None)) == L.ZL_OK
 
@@ -93,6 +97,8 @@ def test_distill_refusals(L, t):
     refused(L, n, bad, "element boundary", *args(d=A + 1))
     refused(L, n, bad, "row stride", *args(d=A, ds=104))
     refused(L, n, bad, "loss_rows", *args(lr=None))
+    refused(L, n, bad, "4-byte", *args(ids=A + 2))
+    refused(L, n, bad, "4-byte", *args(lo=A + 3))
 
 
 def test_linear_logprobs_refusals(L):
@@ -112,6 +118,8 @@ def test_linear_logprobs_refusals(L):
     refused(L, n, bad, "null", *args(h=None))
     refused(L, n, bad, "aligned", *args(w=A + 8))
     refused(L, n, bad, "aligned", *args(ws=A + 4))
+    refused(L, n, bad, "4-byte", *args(tg=A + 1))
+    refused(L, n, L.ZL_EUNSUPPORTED, "2^30", *args(vocab=(1 << 30) + 1))
     assert getattr(L.load(), n)(*args(rows=0, h=None, w=None, ws=None)) == L.ZL_OK
 
 

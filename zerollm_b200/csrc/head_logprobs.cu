@@ -485,6 +485,7 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
                                              float* workspace, zl_stream stream) {
   const char* what = "linear_logprobs";
   if (rows < 0 || dim <= 0 || vocab <= 0) return set_error(ZL_EINVAL, "%s: sizes must be positive", what);
+  if (vocab > (1 << 30)) return set_error(ZL_EUNSUPPORTED, "%s: at most 2^30 vocabulary entries", what);
   if (dim % 8) return set_error(ZL_EUNSUPPORTED, "%s: dim %% 8 != 0", what);
   if (bad_scale(scale)) return set_error(ZL_EINVAL, "%s: scale must be in [1e-4, 1e4]", what);
   if (logp && !targets) return set_error(ZL_EINVAL, "%s: log probabilities need targets", what);
@@ -492,6 +493,9 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
   if (!hidden || !weight || !workspace) return set_error(ZL_EINVAL, "%s: null hidden, weight or workspace", what);
   if ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return set_error(ZL_EINVAL, "%s: hidden, weight and workspace must be 16-byte aligned", what);
+  if ((reinterpret_cast<uintptr_t>(targets) | reinterpret_cast<uintptr_t>(logp) | reinterpret_cast<uintptr_t>(entropy) |
+       reinterpret_cast<uintptr_t>(lse)) & 3)
+    return set_error(ZL_EINVAL, "%s: a target or output array off a 4-byte boundary", what);
   if (rows <= kFewRows && dim <= kFewDim) {
     HeadArgs a{targets, rows, vocab, 0, 0, 0, 0, 0, 0, 0, scale * kLog2e, few_blocks(vocab), reinterpret_cast<float4*>(workspace)};
     const size_t smem = (size_t)(dim + 31) / 32 * 512;

@@ -13,6 +13,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "logprobs.cuh"
 
@@ -309,7 +310,7 @@ template <typename T, bool E>
 __device__ __forceinline__ void add_piece(RunningT<E>& s, const uint4 (&u)[kLaneVecs], int vecs, float most, float c) {
   constexpr int VEC = Elt<T>::VEC;
   if (most > s.m) s.raise(most, c);
-  if (__any_sync(0xffffffffu, s.deep())) {
+  if (__any_sync(0xffffffffu, s.far())) {
 #pragma unroll 1
     for (int i = 0; i < kLaneVecs * VEC; ++i) s.add_one(pick<T>(u, i), c);
   } else if (vecs >= kPieceVecs) {
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
     }
     const float ln_s0 = logf(s.s0);
     if (part == 0 && tid == 0) {
-      const float h = fmaf(-kLn2, s.s1 / s.s0, ln_s0);
+      const float h = fmaf(-kLn2, __fdividef(s.s1, s.s0), ln_s0);
       if (a.lse) a.lse[r] = s.s0 == 0.f ? -INFINITY : fmaf(s.m, a.scale, ln_s0);
       if (a.entropy) a.entropy[r] = (s.s0 == 0.f || h < 0.f) ? 0.f : h;
       if (a.logp) a.logp[r] = t >= 0 ? log_prob(xt, s, ln_s0, a.scale) : 0.f;
@@ -708,7 +709,7 @@ struct LogprobBwdArgs {
 // block per (row, slice of the vocabulary); a thread has four vectors on the way at once, or, where logits and gradient
 // rows do not share their place within 16 bytes, that many bytes' worth of single elements.
 // With l = scale x - lse: d = p (-scale h l - scale (g + h H)), one exponential and paired fp32 instructions.  Masked
-// logits are kept at -2^40 (l finite, p = 0) while lse is not itself that low.
+// logits are kept at -2^40 (l finite, p = 0) while lse is not itself a mask's size.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a, int slices) {
   constexpr int VEC = Elt<T>::VEC, U = 4;
@@ -729,9 +730,9 @@ __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a
       if (v0 + i * NT < sp.hi) u[i] = load16(x + sp.head + (int64_t)(v0 + i * NT) * VEC);
   }
   const float lse = a.lse[r], scale = a.scale;
-  // a row masked wholly has no gradient: with -inf, or with the type's lowest value, beside which its saved
-  // lse cannot hold the ln V that its p would need
-  const bool none = lse < -1e30f;
+  // a row masked wholly (with -inf, or with the type's lowest value) or with a token forced by the highest value has
+  // no gradient: beside a mask's value the saved lse cannot hold what its p would need
+  const bool none = fabsf(lse) > 1e30f;
   int t = (a.g_logp && a.targets) ? a.targets[r] : -1;
   if (t >= V) t = -1;
   const float g = t >= 0 ? a.g_logp[r] * scale : 0.f;
@@ -743,7 +744,7 @@ __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a
     return p * fmaf(-h, fmaxf(l, kFloor), -gh) + (i == t ? g : 0.f);  // (ln p kept off -inf where p = 0)
   };
   if (same) {
-    const bool fast = lse >= -1e6f;
+    const bool fast = fabsf(lse) <= 1e6f;
     const uint64_t s2 = f2_pack(scale, scale), n2 = f2_pack(-lse, -lse), e2 = f2_pack(kLog2e, kLog2e), h2 = f2_pack(-h, -h),
                    g2 = f2_pack(-gh, -gh);
 #pragma unroll
@@ -837,7 +838,7 @@ struct Sums2 {
 };
 
 // A thread's exponentials about a maximum m: x c - fl(m c), the rounding of m c taken out by settle() (as in RunningT);
-// below kDeep (masks only) (x - m) c.
+// beyond kFar (masks only) (x - m) c.
 template <int SECOND> struct Exponent {
   float m, c, mc, mc1;
   __device__ __forceinline__ void at(float M, float scale_c) {
@@ -845,11 +846,11 @@ template <int SECOND> struct Exponent {
     mc = m == -INFINITY ? 0.f : m * c;
     mc1 = m == -INFINITY ? 0.f : m * kLog2e;
   }
-  __device__ __forceinline__ bool deep() const { return m < kDeep && m != -INFINITY; }
+  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar && m != -INFINITY; }
   // factors that make sums of e and e1 exact about m
   __device__ __forceinline__ void settle(float& f, float& f1) const {
     f = f1 = 1.f;
-    if (m >= kDeep) {
+    if (fabsf(m) <= kFar) {
       const float off = fmaf(m, c, -mc) * kLn2;
       f = 1.f - off;
       f1 = SECOND == kSquare ? fmaf(-2.f, off, 1.f) : SECOND == kFourth ? fmaf(-4.f, off, 1.f)
@@ -870,14 +871,14 @@ template <int SECOND> struct Exponent {
   }
   // one element of any value
   __device__ __forceinline__ void one(float x, float& e, float& e1) const {
-    const bool dp = deep();
+    const bool dp = far();
     e = ex2(dp ? (x - m) * c : fmaf(x, c, -mc));
     if (SECOND == kSquare) e1 = e * e;
     else if (SECOND == kFourth) e1 = (e * e) * (e * e);
     else if (SECOND == kOwn) e1 = ex2(dp ? (x - m) * kLog2e : fmaf(x, kLog2e, -mc1));
     else e1 = 0.f;
   }
-  // wf e + wc e1, of a pair (m not below kDeep) and of one element, rounded alike
+  // wf e + wc e1, of a pair (m not beyond kFar) and of one element, rounded alike
   __device__ __forceinline__ uint64_t grad2(uint64_t x, uint64_t wf, uint64_t wc) const {
     const uint64_t e = first2(x);
     if (SECOND == kNone) return mul2(e, wf);
@@ -938,7 +939,7 @@ __device__ __forceinline__ Sums2 distill_sums(Feed<T, NW>& feed, uint32_t& taken
     take_piece(feed, taken++, vecs, lane, u);
     const float most = max_vecs<T>(u);
     if (most > ex.m) raise(most);
-    if (__any_sync(0xffffffffu, ex.deep())) {
+    if (__any_sync(0xffffffffu, ex.far())) {
 #pragma unroll 1
       for (int i = 0; i < kLaneVecs * VEC; ++i) one(pick<T>(u, i));
       continue;
@@ -977,7 +978,7 @@ template <int SECOND, typename T, int NW>
 __device__ __forceinline__ void distill_gradient(Feed<T, NW>& feed, uint32_t& taken, const Span<T>& sp, const T* x, T* d, bool zero,
                                                  const Exponent<SECOND>& ex, float wf, float wc, int lane) {
   constexpr int VEC = Elt<T>::VEC;
-  const bool plain = !zero && !ex.deep() && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  const bool plain = !zero && !ex.far() && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
   const uint64_t wf2 = f2_pack(wf, wf), wc2 = f2_pack(wc, wc);
   for (int v = sp.lo + feed.first * kPieceVecs; v < sp.hi; v += NW * kPieceVecs) {
     const int vecs = sp.hi - v;
@@ -1083,7 +1084,7 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, 24 / (NW * TEAMS)) distill_ke
         dot += __shfl_xor_sync(0xffffffffu, dot, o);
       }
       if (a.opt.normalize) {
-        const float inv = n == 0.f ? 0.f : 1.f / n;
+        const float inv = n == 0.f ? 0.f : __fdividef(1.f, n);
         for (int j = lane; j < k; j += 32) sh.q[j] *= inv;
         dot = n == 0.f ? 0.f : fmaf(dot, inv, -logf(n));
         n *= inv;
@@ -1139,7 +1140,7 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, 24 / (NW * TEAMS)) distill_ke
       ex.at(st.m, c);
       float f, f1;
       ex.settle(f, f1);
-      const float ff = (SECOND == kNone ? fmaf(wq, sh.sum, wc) : wq * sh.sum) * f / st.s, fc = SECOND == kNone ? 0.f : wc * f1 / st.h;
+      const float ff = (SECOND == kNone ? fmaf(wq, sh.sum, wc) : wq * sh.sum) * __fdividef(f, st.s), fc = SECOND == kNone ? 0.f : wc * __fdividef(f1, st.h);
       distill_gradient<SECOND>(feed, taken, sp, x, d, none, ex, ff, fc, lane);
       if (single >= 0) Elt<T>::put(d + single, none ? 0.f : ex.grad(xs, ff, fc));
       team_sync<NW>();  // the elements below are written a second time, by other threads
@@ -1268,11 +1269,18 @@ template <typename T, int SECOND> zl_status launch_distill(const char* what, int
          : nw == 4 ? launch_distill<T, 4, 1, SECOND>(what, s, a) : launch_distill<T, 8, 1, SECOND>(what, s, a);
 }
 
+constexpr int kVocabMax = 1 << 30;  // (column arithmetic is 32-bit)
+bool off_words(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) & 3) return true;
+  return false;
+}
 template <typename T> bool off_element(const void* p) { return (reinterpret_cast<uintptr_t>(p) % sizeof(T)) != 0; }
 
 template <typename T>
 zl_status check_rows(const char* what, const void* logits, int64_t stride, int rows, int vocab, float scale) {
   if (rows < 0 || vocab <= 0) return set_error(ZL_EINVAL, "%s: sizes must be positive", what);
+  if (vocab > kVocabMax) return set_error(ZL_EUNSUPPORTED, "%s: at most 2^30 logits to a row", what);
   if (stride < vocab) return set_error(ZL_EINVAL, "%s: the row stride is below the vocabulary size", what);
   if (bad_scale(scale)) return set_error(ZL_EINVAL, "%s: scale must be in [1e-4, 1e4]", what);
   if (rows > 0 && !logits) return set_error(ZL_EINVAL, "%s: null logits", what);
@@ -1290,6 +1298,8 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   if (top_k < 0 || top_k > vocab) return set_error(ZL_EINVAL, "token_logprobs: top_k must be in [0, vocab]");
   if (top_k > kTopMax) return set_error(ZL_EUNSUPPORTED, "token_logprobs: top_k is at most %d", kTopMax);
   if (top_k > 0 && !top_ids) return set_error(ZL_EINVAL, "token_logprobs: null top_ids");
+  if (off_words({targets, logp, entropy, lse, top_logp, top_ids}))
+    return set_error(ZL_EINVAL, "token_logprobs: a target or output array off a 4-byte boundary");
   if (rows == 0) return ZL_OK;
   LogprobArgs a{logits, stride, targets, rows, vocab, top_k, 1, 0, scale, logp, entropy, lse, top_logp, top_ids};
   const int vecs = vocab / Elt<T>::VEC + 1;
@@ -1320,6 +1330,7 @@ zl_status token_logprobs_backward(const T* logits, int64_t stride, const int32_t
   if (rows == 0) return ZL_OK;
   if (!d || !lse) return set_error(ZL_EINVAL, "%s: null gradient or lse", what);
   if (off_element<T>(d)) return set_error(ZL_EINVAL, "%s: gradient off an element boundary", what);
+  if (off_words({targets, lse, entropy, g_logp, g_entropy})) return set_error(ZL_EINVAL, "%s: an input array off a 4-byte boundary", what);
   if (g_logp && !targets) return set_error(ZL_EINVAL, "%s: a gradient of log probabilities needs targets", what);
   if (g_entropy && !entropy) return set_error(ZL_EINVAL, "%s: a gradient of entropies needs the entropies", what);
   if ((const void*)d == (const void*)logits && d_stride != stride)
@@ -1352,6 +1363,8 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
   if (d && (const void*)d == (const void*)logits && d_stride != stride)
     return set_error(ZL_EINVAL, "%s: a gradient in the logits' place has their row stride", what);
   if (rows > 0 && !loss_rows) return set_error(ZL_EINVAL, "%s: null loss_rows", what);
+  if (off_words({ids, values, targets, row_weight, loss_rows, loss_out}))
+    return set_error(ZL_EINVAL, "%s: an array of 4-byte values off a 4-byte boundary", what);
   if (rows > 0) {
     DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, 1, *opt, d, d_stride, loss_rows};
     const int pieces = (vocab / Elt<T>::VEC + kPieceVecs) / kPieceVecs;

@@ -40,10 +40,10 @@ __device__ __forceinline__ float ex2(float t) {
 // ------------------------------------------------------------------ running softmax statistics
 // c = scale * log2(e).  Sums of e = 2^((x - m) c) and e (x - m) c about the running maximum m.  A masked logit
 // (-inf) has e = 0; it is kept off -inf before anything is multiplied with e.  A NaN or +inf logit makes s0 and
-// s1 NaN.  While m >= kDeep the exponent is one fused product x c - fl(m c); the rounding of m c is taken out of
+// s1 NaN.  While |m| <= kFar the exponent is one fused product x c - fl(m c); the rounding of m c is taken out of
 // the sums again when they leave the thread or m rises.
-constexpr float kDeep = -0x1p90f;    // logits below it only occur as masks
-constexpr float kClamp = -0x1p96f;   // masked logits in products: e = 0 beside any m >= kDeep
+constexpr float kFar = 0x1p90f;      // beyond it, logits only occur as masks (the type's lowest or highest value)
+constexpr float kClamp = -0x1p96f;   // masked logits in products: e = 0 beside any m >= -kFar
 constexpr uint32_t kClampBf16 = 0xef80ef80u;
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -90,12 +90,12 @@ struct Stats {
 // A thread's running statistics.
 template <bool ENTROPY> struct RunningT {
   float m = -INFINITY, mc = 0.f, s0 = 0.f, s1 = 0.f;
-  // whether m is a finite mask: add() does not hold for its elements then, add_one() does
-  __device__ __forceinline__ bool deep() const { return m < kDeep && m != -INFINITY; }
+  // whether m is a mask's value (or +inf): add() does not hold for its elements then, add_one() does
+  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar && m != -INFINITY; }
   __device__ __forceinline__ Stats sums(float c) const {
     Stats s;
     s.m = m; s.s0 = s0; s.s1 = s1;
-    if (m >= kDeep) {  // m c - fl(m c), exact
+    if (fabsf(m) <= kFar) {  // m c - fl(m c), exact
       const float off = fmaf(m, c, -mc), f = fmaf(-off, kLn2, 1.f);
       s.s1 = f * fmaf(-off, s.s0, s.s1);
       s.s0 *= f;
@@ -142,7 +142,7 @@ template <bool ENTROPY> struct RunningT {
   // neither they nor ln S0 - S1 / S0 lose digits.
   template <int N> __device__ __forceinline__ void add_near(float (&v)[N], float c) {
     float x0 = INFINITY, x1 = 0.f;
-    if (m >= kDeep) fold(v, c, x0, x1);
+    if (fabsf(m) <= kFar) fold(v, c, x0, x1);
     if (x0 <= 8.f * N) {
       s0 += x0;
       s1 += x1;
@@ -153,7 +153,7 @@ template <bool ENTROPY> struct RunningT {
   // one element of any value
   __device__ __forceinline__ void add_one(float v, float c) {
     if (v > m) raise(v, c);
-    const float t = m >= kDeep ? fmaf(v, c, -mc) : (v - (m == -INFINITY ? 0.f : m)) * c, e = ex2(t);
+    const float t = fabsf(m) <= kFar ? fmaf(v, c, -mc) : (v - (m == -INFINITY ? 0.f : m)) * c, e = ex2(t);
     s0 += e;
     if (ENTROPY) s1 = fmaf(e, fmaxf(t, kFloor), s1);
   }
@@ -163,7 +163,7 @@ template <bool ENTROPY> struct RunningT {
 #pragma unroll
     for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
     if (b > m) raise(b, c);
-    if (deep()) {
+    if (far()) {
 #pragma unroll
       for (int j = 0; j < N; ++j) add_one(v[j], c);
     } else {
