@@ -676,3 +676,45 @@ def test_linear_logprobs_graph_replay(L):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out[n], a[n]) for n in out)
+
+
+def test_first_calls_inside_a_capture():
+    """In a fresh process the first call of every operator may be one that is captured: nothing that an entry sets up
+    on its first call is forbidden then."""
+    code = """
+import ctypes as C, torch
+from zerollm_b200 import lib as L
+torch.cuda.set_device(0)
+V, k, dim, n = 6400, 8, 512, 300
+x = torch.randn(n, V, device='cuda').bfloat16()
+h = torch.randn(n, dim, device='cuda').bfloat16()
+w = (torch.randn(V, dim, device='cuda') * 0.1).bfloat16()
+t = torch.randint(0, V, (n,), device='cuda', dtype=torch.int32)
+f = [torch.zeros(n, device='cuda') for _ in range(6)]
+top, ids = torch.zeros(n, k, device='cuda'), torch.zeros(n, k, device='cuda', dtype=torch.int32)
+d, lo = torch.zeros_like(x), torch.zeros(1, device='cuda')
+o = L.DistillOptions(0.5, 1.0, 1, 1.0, 0.5, 1.0 / n)
+ws = [torch.empty(L.load().zl_linear_logprobs_workspace_floats(r, dim, V), device='cuda') for r in (n, 4)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    p = lambda a: a.data_ptr()
+    L.call('zl_token_logprobs_bf16', p(x), V, p(t), n, V, 1.0, k, p(f[0]), p(f[1]), p(f[2]), p(top), p(ids), s)
+    L.call('zl_token_logprobs_backward_bf16', p(x), V, p(t), p(f[2]), p(f[1]), p(f[0]), None, n, V, 1.0, p(d), V, s)
+    L.call('zl_distill_topk_bf16', p(x), V, p(ids), p(top), k, p(t), None, C.byref(o), n, V, p(d), V, p(f[3]), p(lo), s)
+    L.call('zl_linear_logprobs_bf16', p(h), p(w), p(t), n, dim, V, 1.0, p(f[3]), p(f[4]), p(f[5]), p(ws[0]), s)
+    L.call('zl_linear_logprobs_bf16', p(h), p(w), p(t), 4, dim, V, 1.0, p(f[3]), p(f[4]), p(f[5]), p(ws[1]), s)
+g.replay()
+torch.cuda.synchronize()
+y = x.float()
+assert float((f[2] - torch.logsumexp(y, 1)).abs().max()) < 1e-4
+assert float((f[5] - torch.logsumexp(h.float() @ w.float().t(), 1)).abs().max()) < 1e-3
+print('captured')
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
