@@ -718,3 +718,69 @@ print('captured')
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(L):
+    """Rows more than 2^31 elements apart, and a weight of more than 2^31 elements."""
+    stride = (1 << 31) // 2 + 1000007
+    rows, vocab, k = 4, 3000, 6
+    buf = torch.empty(3 * stride + vocab, device="cuda", dtype=torch.bfloat16)
+    x = torch.as_strided(buf, (rows, vocab), (stride, 1))
+    small = make("normal", rows, vocab, "bf16")
+    x.copy_(small)
+    t = targets_for(rows, vocab)
+    a, at, ai = call_logprobs(L, x, "bf16", t, 1.0, k)
+    logp, lse = softmax64(small, 1.0)
+    order = torch.sort(small.float(), dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(ai.long(), order)
+    close(a["lse"], lse, err(vocab, "bf16") + 4 * U * (math.log(vocab) + lse.abs()), "lse")
+    ids, v = teacher(rows, vocab, k)
+    o = opts(L)
+    lr, lo = torch.empty(rows, device="cuda"), torch.empty(1, device="cuda")
+    want, got = torch.empty_like(small), torch.empty_like(small)
+    L.call("zl_distill_topk_bf16", small.data_ptr(), vocab, ids.data_ptr(), v.data_ptr(), k, t.data_ptr(), None, C.byref(o), rows,
+           vocab, want.data_ptr(), vocab, lr.data_ptr(), lo.data_ptr(), stream())
+    L.call("zl_distill_topk_bf16", x.data_ptr(), stride, ids.data_ptr(), v.data_ptr(), k, t.data_ptr(), None, C.byref(o), rows,
+           vocab, x.data_ptr(), stride, lr.data_ptr(), lo.data_ptr(), stream())
+    got.copy_(x)
+    # (the rows lie at other places within 16 bytes: sums in another order, an entry off by a rounding of bf16 at most)
+    assert float((got.double() - want.double()).abs().max()) <= 2.0 ** -7 * float(want.double().abs().max())
+    x.copy_(small)
+    g = torch.ones(rows, device="cuda")
+    call_backward(L, x, "bf16", t, a["lse"], None, g, None, 1.0, x)
+    call_backward(L, small, "bf16", t, a["lse"], None, g, None, 1.0, want)
+    got.copy_(x)
+    assert torch.equal(got, want)
+    del buf, x
+    dim, big = 8192, 270000
+    w = torch.empty(big, dim, device="cuda", dtype=torch.bfloat16).normal_(0, 2.0 / math.sqrt(dim))
+    for n in (2, 20):
+        h = torch.randn(n, dim, device="cuda").bfloat16()
+        tt = torch.full((n,), big - 1, device="cuda", dtype=torch.int32)
+        out = call_head(L, h, w, tt, 1.0)
+        y = torch.cat([h.double() @ c.double().T for c in w.split(30000)], 1)
+        lp, ls = softmax64(y, 1.0)
+        off = 2 * (dim / 16 + 4) * U * float(h.double().abs().sum(1).max()) * float(w.abs().max())
+        assert float((out["lse"] - ls).abs().max()) < off + 1e-3 and float((out["logp"] - lp[:, -1]).abs().max()) < 2 * off + 1e-3
+
+
+def test_linear_logprobs_on_two_streams(L):
+    """Two calls in flight, each with its own workspace, share nothing."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    w = (torch.randn(9000, 256, device="cuda", generator=g) * 0.1).bfloat16()
+    for rows in (4, 700):
+        hs = [torch.randn(rows, 256, device="cuda", generator=g).bfloat16() for _ in range(2)]
+        t = targets_for(rows, 9000)
+        want = [call_head(L, h, w, t, 1.0) for h in hs]
+        n = L.load().zl_linear_logprobs_workspace_floats(rows, 256, 9000)
+        ss = [torch.cuda.Stream(), torch.cuda.Stream()]
+        ws = [torch.empty(n, device="cuda") for _ in ss]
+        outs = [{k: torch.zeros(rows, device="cuda") for k in ("logp", "entropy", "lse")} for _ in ss]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for h, s, q, o in zip(hs, ss, ws, outs):
+                L.call("zl_linear_logprobs_bf16", h.data_ptr(), w.data_ptr(), t.data_ptr(), rows, 256, 9000, 1.0, o["logp"].data_ptr(),
+                       o["entropy"].data_ptr(), o["lse"].data_ptr(), q.data_ptr(), s.cuda_stream)
+            torch.cuda.synchronize()
+            for o, a in zip(outs, want):
+                assert all(torch.equal(o[k], a[k]) for k in o)

@@ -508,7 +508,7 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
     HeadArgs a{targets, rows, vocab, 0, 0, 0, 0, 0, 0, 0, scale * kLog2e, few_blocks(vocab), reinterpret_cast<float4*>(workspace)};
     const size_t smem = (size_t)(dim + 31) / 32 * 512;
     cudaError_t e = cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewDim / 32 * 512);
-    if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+    if (e != cudaSuccess) return launched(what, e);
     head_few_kernel<<<a.few, kFewWarps * 32, smem, (cudaStream_t)stream>>>(reinterpret_cast<const __nv_bfloat16*>(hidden),
                                                                            reinterpret_cast<const __nv_bfloat16*>(weight), dim, a);
     const zl_status st = check_launch(what);
@@ -528,6 +528,6 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
   // (make_plan has set the kernels' shared-memory attributes)
   cudaError_t e = held ? cudaLaunchKernelEx(&cfg, head_logprobs_kernel<true>, mh, mw, a)
                        : cudaLaunchKernelEx(&cfg, head_logprobs_kernel<false>, mh, mw, a);
-  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (e != cudaSuccess) return launched(what, e);
   return launch_after(what, head_join_kernel, (rows + 7) / 8, 256, (cudaStream_t)stream, a, scale, logp, entropy, lse);
 }

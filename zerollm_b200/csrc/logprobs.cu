@@ -1240,9 +1240,7 @@ zl_status launch(const char* what, K kern, int64_t blocks, int threads, int part
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  return ZL_OK;
+  return launched(what, cudaLaunchKernelEx(&cfg, kern, args...));
 }
 // Teams of NW warps to a row, or clusters of `parts` blocks; single warps go on to further rows, no more blocks of
 // them than run at once.
@@ -1251,7 +1249,7 @@ zl_status launch_rows(const char* what, K kern, int rows, int parts, zl_stream s
   static std::atomic<uint64_t> done{0};
   const size_t smem = logprobs_smem<T, NW, TEAMS>(a);
   const cudaError_t e = allow_dynamic(kern, done);
-  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (e != cudaSuccess) return launched(what, e);
   int64_t blocks = ((int64_t)rows + TEAMS - 1) / TEAMS * parts;
   if (NW == 1) {
     const int64_t per_sm = std::min<int64_t>(kRowBlocks, (227 * 1024) / (smem + sizeof(TopShared<NW>) * TEAMS + 2048));
@@ -1266,7 +1264,7 @@ template <typename T, int NW, int TEAMS, int SECOND> zl_status launch_distill(co
   const auto kern = distill_kernel<T, NW, TEAMS, SECOND>;
   const size_t smem = (size_t)TEAMS * NW * kDepth * kPieceBytes;
   const cudaError_t e = allow_dynamic(kern, done);
-  if (e != cudaSuccess) return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (e != cudaSuccess) return launched(what, e);
   const int64_t rows = ((int64_t)a.rows + TEAMS - 1) / TEAMS;
   const int64_t room = std::max<int64_t>(1, 24 / (NW * TEAMS) * sm_count_current() / a.parts);
   return launch(what, kern, std::min(rows, room) * a.parts, NW * TEAMS * 32, a.parts, smem, s, a);

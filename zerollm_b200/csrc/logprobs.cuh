@@ -16,6 +16,12 @@ inline bool bad_scale(float s) { return !(s >= 1e-4f && s <= 1e4f); }
 // until that one is done and its results are seen.  let_follow(): this kernel's successor may start from here on.
 __device__ __forceinline__ void follows() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The status of a launch or of a call before it; its error is not left behind for a later call to report.
+inline zl_status launched(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) return ZL_OK;
+  cudaGetLastError();
+  return set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+}
 template <typename K, typename... A>
 zl_status launch_after(const char* what, K kern, int blocks, int threads, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
@@ -27,8 +33,7 @@ zl_status launch_after(const char* what, K kern, int blocks, int threads, cudaSt
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  return e == cudaSuccess ? ZL_OK : set_error(ZL_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  return launched(what, cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
 __device__ __forceinline__ float ex2(float t) {
