@@ -288,7 +288,7 @@ zl_status zl_cross_entropy_fused_bf16(zl_bf16 *logits, const int32_t *targets, i
  * temperature.  rows = 0 does nothing.  -inf masks a logit: its p is 0 and adds nothing to any sum; a row
  * whose logits are all -inf has lse and every log probability -inf, entropy 0, no gradient.  A NaN or +inf
  * logit makes its row's statistics NaN.  No entry allocates or waits; all can be captured into a graph.
- * Results do not depend on the launch: every sum has a fixed order.
+ * The same call gives the same results each time: every sum has a fixed order.
  *
  * Log probabilities of given tokens, entropy, log-sum-exp and top alternatives of each row:
  *   lse[r] = ln sum_j e^{y_j},  logp[r] = y_t - lse with t = targets[r] (0 where t is not in [0, vocab)),

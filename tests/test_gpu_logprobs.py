@@ -182,7 +182,8 @@ def test_token_logprobs_sizes(L, rows, vocab, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("kind", ["masked", "few", "lowest", "highest", "constant", "ties", "sorted", "sharp", "column"])
 @pytest.mark.parametrize("rows,vocab,k", [(3, 900, 20), (3, 6400, 16), (7, 6400, 128), (1, 33333, 50), (2, 140000, 64),
-                                          (1200, 900, 20), (1201, 6400, 64), (2500, 5003, 1)])
+                                          (1200, 900, 20), (1201, 6400, 64), (2500, 5003, 1),
+                                          (1500, 130, 100), (1300, 300, 64), (1200, 1024, 128), (5, 1023, 97), (600, 1100, 20)])
 def test_token_logprobs_values(L, rows, vocab, k, kind, dtype):
     check_logprobs(L, make(kind, rows, vocab, dtype), dtype, 1.0, k, targets_for(rows, vocab))
 
@@ -209,6 +210,21 @@ def test_token_logprobs_nan_and_inf_rows(L):
     x[1] = math.nan  # nothing but NaN: the lowest indices
     _, _, ids = call_logprobs(L, x, "f32", targets_for(4, 700), 1.0, 8)
     assert ids[1].tolist() == list(range(8))
+
+
+@pytest.mark.parametrize("rows,vocab,k", [(1500, 150, 100), (1500, 300, 64), (1500, 1001, 128)])
+def test_token_logprobs_nan_in_short_rows(L, rows, vocab, k):
+    """NaN logits come last among the alternatives, by their index."""
+    x = make("normal", rows, vocab, "bf16")
+    x[1] = math.nan
+    x[2, k // 2:] = math.nan
+    x[3] = -math.inf
+    x[3, 5] = math.nan
+    out, _, ids = call_logprobs(L, x, "bf16", targets_for(rows, vocab), 1.0, k)
+    assert ids[1].tolist() == list(range(k))
+    assert sorted(ids[2, :k // 2].tolist()) == list(range(k // 2)) and ids[2, k // 2:].tolist() == list(range(k // 2, k))
+    assert ids[3].tolist() == [i for i in range(k + 1) if i != 5]
+    assert torch.isfinite(out["lse"][torch.arange(rows, device="cuda") > 3]).all() and torch.isnan(out["lse"][1:3]).all()
 
 
 def test_token_logprobs_optional_outputs(L):

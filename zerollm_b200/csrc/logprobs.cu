@@ -485,6 +485,36 @@ template <typename T, int NW> __device__ int select_slow(const T* x, int V, int 
   return append_equal<T, NW>(x, V, K, n, k, sh);
 }
 
+// The candidates of a short row (one warp): its keys in registers, the k-th largest found bit by bit, every element
+// above it and the lowest-indexed ones equal to it.
+constexpr int kShortRow = 1024;
+template <typename T> __device__ int select_short(const T* x, int V, int k, TopShared<1>& sh) {
+  constexpr int R = kShortRow / 32;
+  const int lane = threadIdx.x & 31;
+  uint32_t q[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) q[i] = i * 32 + lane < V ? order_key(Elt<T>::get(x + i * 32 + lane)) : 0u;
+  uint32_t K = 0;
+#pragma unroll 1
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = K | (1u << b);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (i * 32 < V) n += q[i] >= t;
+    if (__reduce_add_sync(0xffffffffu, n) >= k) K = t;
+  }
+  int n = 0;  // (fewer than k are above K)
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i * 32 < V) push(q[i] > K, candidate(q[i], i * 32 + lane), sh.cand, n, k);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i * 32 < V && n < k) push(q[i] == K && i * 32 + lane < V, candidate(K, i * 32 + lane), sh.cand, n, k);
+  __syncwarp();
+  return min(n, k);
+}
+
 struct LogprobArgs {
   const void* logits;
   int64_t stride;
@@ -508,7 +538,12 @@ template <typename T, int NW, int TEAMS> size_t logprobs_smem(const LogprobArgs&
 // alone, without arithmetic, takes 64 us).  Bound by instructions: about 270 for a lane's 32 logits of a piece
 // (unpacking, maxima, clamp, exponential, two sums) and 700 for a row's alternatives fill 2/3 of the issue slots and
 // half of the exponential units.  1021 x 50001 39 us, 1 x 32000 with 20 about 9 us (8 of them the host's call).
-template <typename T, int NW, int TEAMS>
+//
+// LOOSE (one warp to a row): a short row with too few vectors for its groups to bound anything, or a large k with
+// fewer than 256 groups.  All of its elements are ranked, or where those are too many none is found by a bound and
+// select_short is asked: 32768 rows of 300 with 64 alternatives 243 us (364 by the bound), of 900 with 128 366 us
+// (1011 by a whole block to a row), of 64 with 30 76 us (86).  A kernel of its own, since the code costs the other 3%.
+template <typename T, int NW, int TEAMS, bool LOOSE = false>
 __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / NW) logprobs_kernel(const LogprobArgs a) {
   constexpr int VEC = Elt<T>::VEC, CAP = TopShared<NW>::CAP;
   using Store = typename Maxima<T>::Store;
@@ -618,8 +653,9 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
                  : groups == 128 ? kth_key<4>(sh.group, k, t0, hi, lo) : kth_key<8>(sh.group, k, t0, hi, lo);
         }
       };
-      const uint32_t tau = groups == 32 ? max_key(kth_of_32(NW == 1 ? max_of(g4) : sh.group[lane % 256], k)) : bound(0u, 31, 16);
-      const float least = tau == 0 ? -Elt<T>::MAX : key_value(tau);
+      const uint32_t tau = LOOSE ? 0u
+                           : groups == 32 ? max_key(kth_of_32(NW == 1 ? max_of(g4) : sh.group[lane % 256], k)) : bound(0u, 31, 16);
+      const float least = LOOSE && V > CAP ? NAN : tau == 0 ? -Elt<T>::MAX : key_value(tau);
       TopShared<NW>& first = parts > 1 ? *cg::this_cluster().map_shared_rank(&sh, 0) : sh;
       int own_n = 0, own_vec = 0;  // the counters of a single warp
       auto push_cand = [&](bool yes, float v, int i) {
@@ -672,7 +708,9 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
       if (part == 0) {
         int n = NW == 1 ? own_n : sh.n;
         team_sync<NW>();
-        if (n > CAP) {
+        if (LOOSE && V > CAP) {
+          if constexpr (LOOSE) n = select_short<T>(x, V, k, sh);
+        } else if (n > CAP) {
           n = select_slow<T, NW>(x, V, k, groups == 32 || tau == 0 ? tau : bound(tau, 15, 0), sh);
         } else if (n < k) {  // (tau = 0) masked logits, then NaN ones, by their index
           n = append_equal<T, NW>(x, V, kKeyMasked, n, k, sh);
@@ -1201,7 +1239,7 @@ int team_warps(int rows, int pieces) {
   const int64_t room = 24 * (int64_t)sm_count_current();
   if (rows > room / 2) return pieces >= 16 ? 4 : 1;
   int nw = 1;
-  while (nw < 8 && (int64_t)rows * 2 * nw <= room && pieces >= 2 * nw) nw *= 2;
+  while (nw < 8 && (int64_t)rows * 2 * nw <= room && pieces > 2 * nw) nw *= 2;  // (a whole piece for each)
   return nw;
 }
 // Blocks of eight warps to a row: more while all still run at once and each warp has a piece.  Log probabilities:
@@ -1310,8 +1348,10 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   const int vecs = vocab / Elt<T>::VEC + 1;
   a.pieces = (vecs + kPieceVecs - 1) / kPieceVecs;
   int nw = team_warps(rows, a.pieces);
-  // the vectors' maxima of a row fit beside the rings, and a single warp has 128 groups
-  while (nw < 8 && (vecs > 4096 * nw || (nw == 1 && top_k > 96))) nw *= 2;
+  // the vectors' maxima of a row fit beside the rings, and a single warp has 128 groups (or the row is short)
+  while (nw < 8 && (vecs > 4096 * nw || (nw == 1 && top_k > 96 && vocab > kShortRow))) nw *= 2;
+  const bool loose = vocab <= kShortRow && (3 * (vocab / Elt<T>::VEC) < 4 * top_k || top_k > 96);
+  if (nw == 1 && loose) return launch_rows<T, 1, 4>("token_logprobs", logprobs_kernel<T, 1, 4, true>, rows, 1, s, a);
   if (nw == 1) return launch_rows<T, 1, 4>("token_logprobs", logprobs_kernel<T, 1, 4>, rows, 1, s, a);
   if (nw == 2) return launch_rows<T, 2, 1>("token_logprobs", logprobs_kernel<T, 2, 1>, rows, 1, s, a);
   if (nw == 4) return launch_rows<T, 4, 1>("token_logprobs", logprobs_kernel<T, 4, 1>, rows, 1, s, a);
