@@ -736,6 +736,28 @@ print('captured')
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
+def test_short_rows_first_in_a_process():
+    """What a kernel is allowed on its first call is not taken as given to another of the same arguments."""
+    code = """
+import torch
+from zerollm_b200 import lib as L
+for rows, V, k in ((1500, 300, 64), (4000, 7600, 16)):
+    x = torch.randn(rows, V, device='cuda')
+    lse, ids = torch.zeros(rows, device='cuda'), torch.zeros(rows, k, device='cuda', dtype=torch.int32)
+    L.call('zl_token_logprobs_f32', x.data_ptr(), V, None, rows, V, 1.0, k, None, None, lse.data_ptr(), None, ids.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert float((lse - torch.logsumexp(x, 1)).abs().max()) < 1e-4
+    assert torch.equal(ids.long(), torch.sort(x, dim=1, descending=True, stable=True).indices[:, :k])
+print('both')
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "both" in r.stdout, r.stderr[-2000:]
+
+
 def test_offsets_past_32_bits(L):
     """Rows more than 2^31 elements apart, and a weight of more than 2^31 elements."""
     stride = (1 << 31) // 2 + 1000007

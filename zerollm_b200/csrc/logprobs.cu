@@ -1232,6 +1232,7 @@ __global__ void __launch_bounds__(1024) scaled_sum_kernel(const float* __restric
 // Warps to a row: as many as let all rows run at once (24 warps on an SM), if each has a piece of its own; with
 // more rows than that one warp where a row is short, four where it is 16 pieces or longer, whose rows would leave
 // SMs idle at the end.  Measured, log probabilities: 2400 x 6400 17 us with one, 22 / 25 / 41 us with 2 / 4 / 8;
+// 600 x 1100 9 us with one, 27 us with two, of which the second has nine vectors;
 // 1021 x 50001 35 us with two, 39 / 41 us with 4 / 8; 600 x 50001 25 us with four, 29 us with 2 or 8; 2048 x 32000
 // 45 us with four, 56 us with one.  Distillation: 32768 x 6400 201 us with one, 280 / 303 us with 2 / 4; 2048 x
 // 32000 66 us with four, 84 / 74 us with 1 / 8; 500 x 50001 39 us with four, 54 / 42 us with 2 / 8.
@@ -1282,9 +1283,10 @@ zl_status launch(const char* what, K kern, int64_t blocks, int threads, int part
 }
 // Teams of NW warps to a row, or clusters of `parts` blocks; single warps go on to further rows, no more blocks of
 // them than run at once.
-template <typename T, int NW, int TEAMS, typename K>
-zl_status launch_rows(const char* what, K kern, int rows, int parts, zl_stream s, const LogprobArgs& a) {
+template <typename T, int NW, int TEAMS, bool LOOSE = false>
+zl_status launch_rows(const char* what, int rows, int parts, zl_stream s, const LogprobArgs& a) {
   static std::atomic<uint64_t> done{0};
+  const auto kern = logprobs_kernel<T, NW, TEAMS, LOOSE>;
   const size_t smem = logprobs_smem<T, NW, TEAMS>(a);
   const cudaError_t e = allow_dynamic(kern, done);
   if (e != cudaSuccess) return launched(what, e);
@@ -1351,17 +1353,17 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   // the vectors' maxima of a row fit beside the rings, and a single warp has 128 groups (or the row is short)
   while (nw < 8 && (vecs > 4096 * nw || (nw == 1 && top_k > 96 && vocab > kShortRow))) nw *= 2;
   const bool loose = vocab <= kShortRow && (3 * (vocab / Elt<T>::VEC) < 4 * top_k || top_k > 96);
-  if (nw == 1 && loose) return launch_rows<T, 1, 4>("token_logprobs", logprobs_kernel<T, 1, 4, true>, rows, 1, s, a);
-  if (nw == 1) return launch_rows<T, 1, 4>("token_logprobs", logprobs_kernel<T, 1, 4>, rows, 1, s, a);
-  if (nw == 2) return launch_rows<T, 2, 1>("token_logprobs", logprobs_kernel<T, 2, 1>, rows, 1, s, a);
-  if (nw == 4) return launch_rows<T, 4, 1>("token_logprobs", logprobs_kernel<T, 4, 1>, rows, 1, s, a);
+  if (nw == 1 && loose) return launch_rows<T, 1, 4, true>("token_logprobs", rows, 1, s, a);
+  if (nw == 1) return launch_rows<T, 1, 4>("token_logprobs", rows, 1, s, a);
+  if (nw == 2) return launch_rows<T, 2, 1>("token_logprobs", rows, 1, s, a);
+  if (nw == 4) return launch_rows<T, 4, 1>("token_logprobs", rows, 1, s, a);
   a.parts = team_parts(rows, a.pieces);
   for (;; a.parts *= 2) {
     a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
     if (logprobs_smem<T, 8, 1>(a) <= kMaxDynamic) break;
     if (a.parts == kMaxParts) return set_error(ZL_EUNSUPPORTED, "token_logprobs: vocab too large for top alternatives");
   }
-  return launch_rows<T, 8, 1>("token_logprobs", logprobs_kernel<T, 8, 1>, rows, a.parts, s, a);
+  return launch_rows<T, 8, 1>("token_logprobs", rows, a.parts, s, a);
 }
 
 template <typename T>
