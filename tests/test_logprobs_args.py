@@ -120,6 +120,7 @@ def test_linear_logprobs_refusals(L):
     refused(L, n, bad, "aligned", *args(ws=A + 4))
     refused(L, n, bad, "4-byte", *args(tg=A + 1))
     refused(L, n, L.ZL_EUNSUPPORTED, "2^30", *args(vocab=(1 << 30) + 1))
+    refused(L, n, L.ZL_EUNSUPPORTED, "2^30", *args(rows=(1 << 31) - 1))
     assert getattr(L.load(), n)(*args(rows=0, h=None, w=None, ws=None)) == L.ZL_OK
 
 
@@ -134,7 +135,7 @@ def test_linear_logprobs_workspace(L):
     for rows, vocab in [(1, 1), (1, 32000), (8, 6400)]:
         n = f(rows, 512, vocab)
         assert n % (rows * 4) == 0 and 1 <= n // (rows * 4) <= (vocab + 127) // 128
-    assert f(0, 512, 100) == 0
+    assert f(0, 512, 100) == 0 and f((1 << 31) - 1, 512, 100) == 0
 
 
 def test_model_entries_refuse_null_arguments(L):

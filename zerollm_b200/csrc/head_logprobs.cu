@@ -483,7 +483,7 @@ int head_dev_error_read_and_clear() {
 using namespace zl;
 
 extern "C" int64_t zl_linear_logprobs_workspace_floats(int rows, int dim, int vocab) {
-  if (rows <= 0 || dim <= 0 || vocab <= 0) return 0;
+  if (rows <= 0 || dim <= 0 || vocab <= 0 || rows > (1 << 30) || vocab > (1 << 30)) return 0;
   if (rows <= kFewRows && dim <= kFewDim) return (int64_t)rows * few_blocks(vocab) * 4;
   return (int64_t)rows * make_plan(rows, dim, vocab).slots * kShares * 4;
 }
@@ -493,7 +493,7 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
                                              float* workspace, zl_stream stream) {
   const char* what = "linear_logprobs";
   if (rows < 0 || dim <= 0 || vocab <= 0) return set_error(ZL_EINVAL, "%s: sizes must be positive", what);
-  if (vocab > (1 << 30)) return set_error(ZL_EUNSUPPORTED, "%s: at most 2^30 vocabulary entries", what);
+  if (rows > (1 << 30) || vocab > (1 << 30)) return set_error(ZL_EUNSUPPORTED, "%s: at most 2^30 rows and vocabulary entries", what);
   if (dim % 8) return set_error(ZL_EUNSUPPORTED, "%s: dim %% 8 != 0", what);
   if (bad_scale(scale)) return set_error(ZL_EINVAL, "%s: scale must be in [1e-4, 1e4]", what);
   if (logp && !targets) return set_error(ZL_EINVAL, "%s: log probabilities need targets", what);
