@@ -655,7 +655,10 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
       };
       const uint32_t tau = LOOSE ? 0u
                            : groups == 32 ? max_key(kth_of_32(NW == 1 ? max_of(g4) : sh.group[lane % 256], k)) : bound(0u, 31, 16);
-      const float least = LOOSE && V > CAP ? NAN : tau == 0 ? -Elt<T>::MAX : key_value(tau);
+      // as a logit: of a cut bf16 key the value itself (below zero a bf16 value's key ends in ones), so that vectors and
+      // their elements are compared with the same number and -inf, which also stands for no element, never reaches it
+      const uint32_t exact = sizeof(T) == 2 && tau < 0x80000000u ? tau | 0xffffu : tau;
+      const float least = LOOSE && V > CAP ? NAN : tau == 0 ? -Elt<T>::MAX : key_value(exact);
       TopShared<NW>& first = parts > 1 ? *cg::this_cluster().map_shared_rank(&sh, 0) : sh;
       int own_n = 0, own_vec = 0;  // the counters of a single warp
       auto push_cand = [&](bool yes, float v, int i) {
@@ -673,8 +676,9 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
         while (__any_sync(0xffffffffu, bits != 0)) {
           const int b = __ffs(bits) - 1;
           const int v = v0 + b / kLaneVecs * NW * kPieceVecs + b % kLaneVecs * 32 + lane;
-          if constexpr (NW == 1) push(bits != 0, v, sh.vec, own_vec, CAP);
-          else push(bits != 0, v, sh.vec, &sh.nvec, CAP);
+          const bool in = bits != 0 && v < sp.hi;
+          if constexpr (NW == 1) push(in, v, sh.vec, own_vec, CAP);
+          else push(in, v, sh.vec, &sh.nvec, CAP);
           bits &= bits - 1;
         }
       }
@@ -700,8 +704,8 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
         }
       }
       if (nvec > CAP) {  // vectors were dropped: the slow way
-        own_n += CAP;
-        if (NW > 1 && tid == 0) atomicAdd(&first.n, CAP);
+        own_n += CAP + 1;
+        if (NW > 1 && tid == 0) atomicAdd(&first.n, CAP + 1);
       }
       if (parts > 1) cg::this_cluster().sync();
       else team_sync<NW>();
