@@ -1,9 +1,13 @@
 """Rows masked with finite values, alone and beside -inf, in the operators on next-token distributions: against the
 fp64 formulas and with the tolerances of tests/test_gpu_logprobs.py."""
+import ctypes as C
+import math
+
 import pytest
 import torch
 
-from tests.test_gpu_logprobs import DT, L, NINF, check_logprobs, strided, targets_for  # noqa: F401
+from tests.test_gpu_logprobs import (DT, L, NINF, U, call_head, check_logprobs, close, entropy64, softmax64,  # noqa: F401
+                                     strided, targets_for)
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +42,99 @@ def test_alternatives_behind_a_long_masked_run(L, rows, dtype):
     """Masks of the lowest value in more vectors than are listed at once, behind a run of -inf."""
     for vocab, low, lead in [(3700, 2000, 1700), (8000, 6000, 1600), (30000, 20000, 9000)]:
         check_logprobs(L, mixed_masks(rows, vocab, dtype, 7, low, lead), dtype, 1.0, 40, targets_for(rows, vocab))
+
+
+# ------------------------------------------------------------------ statistics
+MASKS = [-1e4, -1e6, -1e9, -1e10, -1e12, -1e20, -1e30]
+
+
+def finite_masks(rows, vocab, dtype, value, layout, seed=0):
+    """Ordinary logits masked with `value`; the middle row wholly."""
+    g = torch.Generator(device="cuda").manual_seed(seed + rows * 31 + vocab)
+    x, _ = strided(rows, vocab, dtype)
+    v = torch.randn(rows, vocab, device="cuda", generator=g) * 3
+    left = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+    if layout == "some":
+        left |= torch.rand(vocab, device="cuda", generator=g) < 0.6
+    elif layout == "few":
+        left[torch.randperm(vocab, device="cuda", generator=g)[:5]] = True
+    else:                                                     # "behind": whole pieces of masks before the first logit
+        left[vocab * 7 // 8:] = True
+    left[vocab - 1] = True
+    v.masked_fill_(~left, value)
+    v[rows // 2] = value
+    x.copy_(v)
+    return x, left.nonzero()[:, 0]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("layout", ["some", "few", "behind"])
+@pytest.mark.parametrize("value", MASKS)
+def test_token_logprobs_finite_masks(L, value, layout, dtype):
+    for rows, vocab, k in [(3, 900, 9), (3, 6400, 16), (1300, 1001, 40), (1201, 6400, 0), (600, 9000, 7), (1, 33333, 50),
+                           (3, 140000, 64)]:
+        x, _ = finite_masks(rows, vocab, dtype, value, layout)
+        for scale in (1.0, 0.7):
+            check_logprobs(L, x, dtype, scale, k, targets_for(rows, vocab))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("offset", [-1e9, -1e7, -1e5, 1e4, 1e5, 1e6, 1e7, 1e8, 1e9])
+def test_token_logprobs_far_from_zero(L, offset, dtype):
+    """Rows of ordinary spread about a far value (as far as the type still tells its neighbours apart)."""
+    for rows, vocab in [(3, 900), (1300, 640), (2, 50001)]:
+        g = torch.Generator(device="cuda").manual_seed(vocab)
+        x, _ = strided(rows, vocab, dtype)
+        x.copy_(torch.randn(rows, vocab, device="cuda", generator=g, dtype=torch.float64) * 3 + offset)
+        for scale in (1.0, 1.3):
+            check_logprobs(L, x, dtype, scale, 5, targets_for(rows, vocab))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale,size", [(1e4, 30.0), (1e4, 3000.0), (1e4, 1e-3), (1e3, 10.0), (300.0, 60.0), (1e-4, 3e4), (1e-4, 1e9)])
+def test_token_logprobs_extreme_scales(L, scale, size, dtype):
+    for rows, vocab in [(3, 900), (1300, 640), (2, 50001)]:
+        g = torch.Generator(device="cuda").manual_seed(vocab + 1)
+        x, _ = strided(rows, vocab, dtype)
+        x.copy_(torch.randn(rows, vocab, device="cuda", generator=g) * size)
+        check_logprobs(L, x, dtype, scale, 5, targets_for(rows, vocab))
+
+
+@pytest.mark.parametrize("value", [1e4, 1e6, 1e9, 1e20])
+def test_linear_logprobs_of_large_exact_logits(L, value):
+    """One entry of hidden is not 0, so a logit is a single product, exact in fp32: tolerances without a product's."""
+    check_exact_head(L, 5, 264, 5003, value)
+
+
+def exact_head(rows, dim, vocab, value, seed=0):
+    """hidden of one entry 1 a row, and a weight of ordinary entries, a third of them -value; column 0 of it is -value
+    but for eight entries, so rows with that entry are nearly wholly masked."""
+    g = torch.Generator(device="cuda").manual_seed(seed + rows + dim)
+    at = torch.randint(0, dim, (rows,), device="cuda", generator=g)
+    at[0] = 0
+    h = torch.zeros(rows, dim, device="cuda").scatter_(1, at[:, None], 1.0).bfloat16()
+    w = torch.randn(vocab, dim, device="cuda", generator=g) * 3
+    w = torch.where(torch.rand(vocab, dim, device="cuda", generator=g) < 0.33, torch.full((), -value, device="cuda"), w)
+    w[8:, 0] = -value
+    w[:, 1] = -value
+    if rows > 1:
+        h[1] = 0
+        h[1, 1] = 1                                           # (wholly masked)
+    return h, w.bfloat16()
+
+
+def check_exact_head(L, rows, dim, vocab, value):
+    h, w = exact_head(rows, dim, vocab, value)
+    t = targets_for(rows, vocab)
+    for scale in (1.0, C.c_float(0.7).value):
+        out = call_head(L, h, w, t, scale)
+        x = h.double() @ w.double().T
+        logp, lse = softmax64(x, scale)
+        # a thread's sums: chunks of 32 (8 additions to a chain), at most vocab / 64 chunks; 148 partials joined; terms
+        # below the maximum as in the other operators
+        E, lnv = (8 + math.ceil(vocab / 64) + 5 * 20) * U, math.log(vocab)
+        close(out["lse"], lse, E + 4 * U * (lnv + (x * scale).amax(1).abs()), "lse")
+        close(out["entropy"], entropy64(logp), E * (2 + lnv) + 4 * U * (lnv + 1), "entropy")
+        ok = (t >= 0) & (t < vocab)
+        at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
+        close(out["logp"], torch.where(ok, at, torch.zeros_like(at)), E + 4 * U * (lnv + at.abs()), "logp")

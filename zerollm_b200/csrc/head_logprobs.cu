@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
           if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : kClamp;
+            for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
           }
           if (t >= n && t < n + 32 && t < a.vocab) {
 #pragma unroll

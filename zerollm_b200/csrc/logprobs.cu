@@ -303,16 +303,23 @@ template <typename T, int N, bool E> __device__ __forceinline__ void add_vecs(Ru
 #pragma unroll
     for (int i = 0; i < VEC; ++i) f[j * VEC + i] = e[i];
   }
-  s.add(f, c);
+  s.template add<true>(f, c);
 }
 // A lane's vectors of a piece, the maximum of which is known.
 template <typename T, bool E>
 __device__ __forceinline__ void add_piece(RunningT<E>& s, const uint4 (&u)[kLaneVecs], int vecs, float most, float c) {
   constexpr int VEC = Elt<T>::VEC;
   if (most > s.m) s.raise(most, c);
-  if (__any_sync(0xffffffffu, s.far())) {
+  if (__any_sync(0xffffffffu, !s.near())) {
 #pragma unroll 1
-    for (int i = 0; i < kLaneVecs * VEC; ++i) s.add_one(pick<T>(u, i), c);
+    for (int j = 0; j < kLaneVecs; ++j) {  // (a short loop: unrolled it cost the rows that never come here 3%)
+      uint4 w = u[0];
+#pragma unroll
+      for (int i = 1; i < kLaneVecs; ++i) w = i == j ? u[i] : w;
+      float f[VEC];
+      Elt<T>::unpack(w, f);
+      s.template add<false>(f, c);
+    }
   } else if (vecs >= kPieceVecs) {
     add_vecs<T, kLaneVecs>(s, u, c);
   } else {
@@ -882,6 +889,7 @@ struct Sums2 {
   }
 };
 
+constexpr float kFar = 0x1p90f;  // beyond it, logits only occur as masks (the type's lowest or highest value)
 // A thread's exponentials about a maximum m: x c - fl(m c), the rounding of m c taken out by settle() (as in RunningT);
 // beyond kFar (masks only) (x - m) c.
 template <int SECOND> struct Exponent {

@@ -45,10 +45,12 @@ __device__ __forceinline__ float ex2(float t) {
 // ------------------------------------------------------------------ running softmax statistics
 // c = scale * log2(e).  Sums of e = 2^((x - m) c) and e (x - m) c about the running maximum m.  A masked logit
 // (-inf) has e = 0; it is kept off -inf before anything is multiplied with e.  A NaN or +inf logit makes s0 and
-// s1 NaN.  While |m| <= kFar the exponent is one fused product x c - fl(m c); the rounding of m c is taken out of
-// the sums again when they leave the thread or m rises.
-constexpr float kFar = 0x1p90f;      // beyond it, logits only occur as masks (the type's lowest or highest value)
-constexpr float kClamp = -0x1p96f;   // masked logits in products: e = 0 beside any m >= -kFar
+// s1 NaN.  While |m c| <= kNear the exponent is one fused product x c - fl(m c); the rounding of m c, at most 2^-12
+// there, is taken out of the sums again, to first order (the rest is below 2^-25), when they leave the thread or m
+// rises.  Beyond it (large logits, masks of finite values) the exponent is (x - m) c, of a difference that is exact
+// where x is near m.
+constexpr float kNear = 0x1p13f;
+constexpr float kClamp = -0x1p96f;   // masked logits in fused products: e = 0 beside any |m c| <= kNear
 constexpr uint32_t kClampBf16 = 0xef80ef80u;
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -95,12 +97,12 @@ struct Stats {
 // A thread's running statistics.
 template <bool ENTROPY> struct RunningT {
   float m = -INFINITY, mc = 0.f, s0 = 0.f, s1 = 0.f;
-  // whether m is a mask's value (or +inf): add() does not hold for its elements then, add_one() does
-  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar && m != -INFINITY; }
+  // whether the fused product holds about m (also before any logit, mc = 0: nothing but masks adds to the sums then)
+  __device__ __forceinline__ bool near() const { return fabsf(mc) <= kNear; }
   __device__ __forceinline__ Stats sums(float c) const {
     Stats s;
     s.m = m; s.s0 = s0; s.s1 = s1;
-    if (fabsf(m) <= kFar) {  // m c - fl(m c), exact
+    if (near() && m != -INFINITY) {  // m c - fl(m c), exact
       const float off = fmaf(m, c, -mc), f = fmaf(-off, kLn2, 1.f);
       s.s1 = f * fmaf(-off, s.s0, s.s1);
       s.s0 *= f;
@@ -114,16 +116,21 @@ template <bool ENTROPY> struct RunningT {
     m = most; mc = m * c;
     s0 = s.s0; s1 = s.s1;
   }
-  // sums of N elements about m, none below kClamp: pairs of partial sums (paired fp32 instructions)
-  template <int N> __device__ __forceinline__ void fold(const float (&v)[N], float c, float& x0, float& x1) const {
-    const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(-mc, -mc);
+  // sums of N elements about m, none above it: pairs of partial sums (paired fp32 instructions).  NEAR: by the fused
+  // product, which has to hold, and none below kClamp; otherwise by whichever holds, of any values
+  template <bool NEAR, int N> __device__ __forceinline__ void fold(const float (&v)[N], float c, float& x0, float& x1) const {
+    const float sub = NEAR || near() ? 0.f : -m, add = NEAR || near() ? -mc : 0.f;
+    const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(add, add), s2 = f2_pack(sub, sub);
     uint64_t a0[2] = {0, 0}, a1[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-      const uint64_t t = fma2(f2_pack(v[j], v[j + 1]), c2, n2);
+      uint64_t t = f2_pack(v[j], v[j + 1]);
+      if (!NEAR) t = add2(t, s2);
+      t = fma2(t, c2, n2);
       float t0, t1;
       f2_unpack(t, t0, t1);
       const uint64_t e = f2_pack(ex2(t0), ex2(t1));
+      if (!NEAR) t = f2_pack(fmaxf(t0, kFloor), fmaxf(t1, kFloor));
       a0[j / 2 & 1] = add2(a0[j / 2 & 1], e);
       if (ENTROPY) a1[j / 2 & 1] = fma2(e, t, a1[j / 2 & 1]);
     }
@@ -135,20 +142,20 @@ template <bool ENTROPY> struct RunningT {
       x1 = x + y;
     }
   }
-  // N elements, none above m and none below kClamp
-  template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
+  // N elements, none above m (NEAR: as for fold())
+  template <bool NEAR, int N> __device__ __forceinline__ void add(const float (&v)[N], float c) {
     float x0, x1 = 0.f;
-    fold(v, c, x0, x1);
+    fold<NEAR>(v, c, x0, x1);
     s0 += x0;
     s1 += x1;
   }
-  // N elements, none below kClamp, whose maximum is only looked for where their sum says that it lies well above m (by
-  // 3 at least, in powers of two): m need not be the maximum for the sums to be exact, only near enough to it that
-  // neither they nor ln S0 - S1 / S0 lose digits.
-  template <int N> __device__ __forceinline__ void add_near(float (&v)[N], float c) {
+  // N elements, whose maximum is only looked for where their sum says that it lies well above m (by 3 at least, in powers
+  // of two): m need not be the maximum for the sums to be exact, only near enough to it that neither they nor
+  // ln S0 - S1 / S0 lose digits.  (x1 is NaN beside -inf, which the fused product does not take.)
+  template <int N> __device__ __forceinline__ void add_near(const float (&v)[N], float c) {
     float x0 = INFINITY, x1 = 0.f;
-    if (fabsf(m) <= kFar) fold(v, c, x0, x1);
-    if (x0 <= 8.f * N) {
+    if (near() && m != -INFINITY) fold<true>(v, c, x0, x1);
+    if (x0 <= 8.f * N && x1 == x1) {
       s0 += x0;
       s1 += x1;
     } else {
@@ -158,24 +165,17 @@ template <bool ENTROPY> struct RunningT {
   // one element of any value
   __device__ __forceinline__ void add_one(float v, float c) {
     if (v > m) raise(v, c);
-    const float t = fabsf(m) <= kFar ? fmaf(v, c, -mc) : (v - (m == -INFINITY ? 0.f : m)) * c, e = ex2(t);
+    const float t = near() ? fmaf(v, c, -mc) : (v - m) * c, e = ex2(t);
     s0 += e;
     if (ENTROPY) s1 = fmaf(e, fmaxf(t, kFloor), s1);
   }
   // N elements of any values
-  template <int N> __device__ __forceinline__ void add_any(float (&v)[N], float c) {
+  template <int N> __device__ __forceinline__ void add_any(const float (&v)[N], float c) {
     float b = v[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
     if (b > m) raise(b, c);
-    if (far()) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) add_one(v[j], c);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = max_nan(v[j], kClamp);
-      add(v, c);
-    }
+    add<false>(v, c);
   }
 };
 using Running = RunningT<true>;
