@@ -6,8 +6,8 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_logprobs import (DT, L, NINF, U, call_head, check_logprobs, close, entropy64, softmax64,  # noqa: F401
-                                     strided, targets_for)
+from tests.test_gpu_logprobs import (DT, L, NINF, U, call_head, check_distill, check_logprobs, close, entropy64,  # noqa: F401
+                                     opts, softmax64, strided, targets_for)
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,48 @@ def check_exact_head(L, rows, dim, vocab, value):
         ok = (t >= 0) & (t < vocab)
         at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
         close(out["logp"], torch.where(ok, at, torch.zeros_like(at)), E + 4 * U * (lnv + at.abs()), "logp")
+
+
+# ------------------------------------------------------------------ distillation
+OPTIONS = [dict(), dict(scale=0.5), dict(scale=0.25), dict(scale=0.7), dict(scale=1.3, ce=0.0)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("layout", ["some", "few", "behind"])
+@pytest.mark.parametrize("value", MASKS)
+def test_distill_finite_masks(L, value, layout, dtype):
+    for i, (rows, vocab) in enumerate([(5, 900), (5, 6400), (200, 3001), (5, 40001), (3, 140000)]):
+        for o in (OPTIONS[i % 5], OPTIONS[(i + 2) % 5]):
+            x, left = finite_masks(rows, vocab, dtype, value, layout)
+            check_distill(L, x, dtype, min(12, left.numel()), opts(L, **o), columns=left)
+            x, _ = finite_masks(rows, vocab, dtype, value, layout)
+            check_distill(L, x, dtype, 12, opts(L, **o))          # alternatives the student has masked
+
+
+def test_distill_finite_masks_of_many_rows(L):
+    """More rows than run at once, so that a team's next row follows a wholly masked one."""
+    for value in (-1e4, -1e10):
+        x, left = finite_masks(4000, 1001, "bf16", value, "behind")
+        x[::3] = value
+        check_distill(L, x, "bf16", 8, opts(L, scale=0.5), columns=left)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("offset", [-1e9, -1e7, -1e5, 1e4, 1e5, 1e6, 1e7, 1e8, 1e9])
+def test_distill_far_from_zero(L, offset, dtype):
+    for o in OPTIONS:
+        for rows, vocab, dpad in [(5, 901, 0), (3, 50001, 3)]:
+            g = torch.Generator(device="cuda").manual_seed(vocab)
+            x, _ = strided(rows, vocab, dtype)
+            x.copy_(torch.randn(rows, vocab, device="cuda", generator=g, dtype=torch.float64) * 3 + offset)
+            check_distill(L, x, dtype, 5, opts(L, **o), dpad=dpad)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale,size", [(1e4, 30.0), (1e4, 1e-3), (1e3, 10.0), (300.0, 60.0), (1e-4, 3e4), (1e-4, 1e9)])
+def test_distill_extreme_scales(L, scale, size, dtype):
+    for rows, vocab in [(5, 901), (2, 50001)]:
+        g = torch.Generator(device="cuda").manual_seed(vocab + 1)
+        x, _ = strided(rows, vocab, dtype)
+        x.copy_(torch.randn(rows, vocab, device="cuda", generator=g) * size)
+        check_distill(L, x, dtype, 5, opts(L, scale=scale))

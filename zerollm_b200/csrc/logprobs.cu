@@ -14,6 +14,7 @@
 #include <cmath>
 #include <cstdint>
 #include <initializer_list>
+#include <type_traits>
 
 #include "logprobs.cuh"
 
@@ -272,17 +273,6 @@ template <typename T> __device__ __forceinline__ float max_vecs(const uint4 (&u)
       a = fmaxf(a, fmaxf(fmaxf(__uint_as_float(u[j].x), __uint_as_float(u[j].y)), fmaxf(__uint_as_float(u[j].z), __uint_as_float(u[j].w))));
     return a;
   }
-}
-
-// Element i of a lane's vectors (selected, not indexed: the vectors stay in registers).
-template <typename T> __device__ __forceinline__ float pick(const uint4 (&u)[kLaneVecs], int i) {
-  uint32_t word = 0;
-#pragma unroll
-  for (int j = 0; j < kLaneVecs * 4; ++j) {
-    const uint4& v = u[j / 4];
-    word = i * (int)sizeof(T) / 4 == j ? (j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w) : word;
-  }
-  return sizeof(T) == 4 ? __uint_as_float(word) : i % 2 ? hi_bf16(word) : lo_bf16(word);
 }
 
 // N of a lane's vectors, none of whose elements is above the running maximum.
@@ -889,27 +879,32 @@ struct Sums2 {
   }
 };
 
-constexpr float kFar = 0x1p90f;  // beyond it, logits only occur as masks (the type's lowest or highest value)
-// A thread's exponentials about a maximum m: x c - fl(m c), the rounding of m c taken out by settle() (as in RunningT);
-// beyond kFar (masks only) (x - m) c.
+// A thread's exponentials about a maximum m: x c - fl(m c), the rounding of m c taken out by settle() (as in RunningT)
+// while |m| times the larger of both factors is at most kNear (the fourth power's rounding is then four times 2^-14);
+// (x - m) c beyond it.
 template <int SECOND> struct Exponent {
-  float m, c, mc, mc1;
+  float m, c, sub, mc, mc1;  // sub: -m where the difference is formed first (mc and mc1 are 0 then), else 0
   __device__ __forceinline__ void at(float M, float scale_c) {
     m = M; c = scale_c;
-    mc = m == -INFINITY ? 0.f : m * c;
-    mc1 = m == -INFINITY ? 0.f : m * kLog2e;
+    const float most = SECOND == kNone ? c : fmaxf(c, kLog2e);
+    const bool near = fabsf(m) * most <= kNear;
+    sub = near || m == -INFINITY ? 0.f : -m;
+    mc = near ? m * c : 0.f;
+    mc1 = near ? m * kLog2e : 0.f;
   }
-  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar && m != -INFINITY; }
+  __device__ __forceinline__ bool far() const { return sub != 0.f; }
   // factors that make sums of e and e1 exact about m
   __device__ __forceinline__ void settle(float& f, float& f1) const {
     f = f1 = 1.f;
-    if (fabsf(m) <= kFar) {
+    if (!far() && m != -INFINITY) {
       const float off = fmaf(m, c, -mc) * kLn2;
       f = 1.f - off;
       f1 = SECOND == kSquare ? fmaf(-2.f, off, 1.f) : SECOND == kFourth ? fmaf(-4.f, off, 1.f)
            : SECOND == kOwn ? fmaf(-kLn2, fmaf(m, kLog2e, -mc1), 1.f) : 1.f;
     }
   }
+  // of a pair; its difference to m where that is formed first (FAR: it may be)
+  template <bool FAR> __device__ __forceinline__ uint64_t about(uint64_t x) const { return FAR ? add2(x, f2_pack(sub, sub)) : x; }
   __device__ __forceinline__ uint64_t first2(uint64_t x) const {
     float a, b;
     f2_unpack(fma2(x, f2_pack(c, c), f2_pack(-mc, -mc)), a, b);
@@ -924,14 +919,14 @@ template <int SECOND> struct Exponent {
   }
   // one element of any value
   __device__ __forceinline__ void one(float x, float& e, float& e1) const {
-    const bool dp = far();
-    e = ex2(dp ? (x - m) * c : fmaf(x, c, -mc));
+    if (far()) x += sub;
+    e = ex2(fmaf(x, c, -mc));
     if (SECOND == kSquare) e1 = e * e;
     else if (SECOND == kFourth) e1 = (e * e) * (e * e);
-    else if (SECOND == kOwn) e1 = ex2(dp ? (x - m) * kLog2e : fmaf(x, kLog2e, -mc1));
+    else if (SECOND == kOwn) e1 = ex2(fmaf(x, kLog2e, -mc1));
     else e1 = 0.f;
   }
-  // wf e + wc e1, of a pair (m not beyond kFar) and of one element, rounded alike
+  // wf e + wc e1, of a pair (m not far) and of one element, rounded alike
   __device__ __forceinline__ uint64_t grad2(uint64_t x, uint64_t wf, uint64_t wc) const {
     const uint64_t e = first2(x);
     if (SECOND == kNone) return mul2(e, wf);
@@ -992,24 +987,32 @@ __device__ __forceinline__ Sums2 distill_sums(Feed<T, NW>& feed, uint32_t& taken
     take_piece(feed, taken++, vecs, lane, u);
     const float most = max_vecs<T>(u);
     if (most > ex.m) raise(most);
-    if (__any_sync(0xffffffffu, ex.far())) {
-#pragma unroll 1
-      for (int i = 0; i < kLaneVecs * VEC; ++i) one(pick<T>(u, i));
-      continue;
-    }
     uint64_t b0[2] = {0, 0}, b1[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < kLaneVecs; ++j) {
+    auto add = [&](const uint4& w, auto far) {
       float f[VEC];
-      Elt<T>::unpack(u[j], f);
+      Elt<T>::unpack(w, f);
 #pragma unroll
       for (int l = 0; l < VEC; l += 2) {
-        const uint64_t x = f2_pack(f[l], f[l + 1]), e = ex.first2(x);
+        const uint64_t x = ex.template about<far.value>(f2_pack(f[l], f[l + 1])), e = ex.first2(x);
         b0[l / 2 & 1] = add2(b0[l / 2 & 1], e);
         if (SECOND == kSquare) b1[l / 2 & 1] = fma2(e, e, b1[l / 2 & 1]);
         else if (SECOND != kNone) b1[l / 2 & 1] = add2(b1[l / 2 & 1], ex.second2(x, e));
       }
-      if (vecs <= (j + 1) * 32) break;
+    };
+    if (__any_sync(0xffffffffu, ex.far())) {
+#pragma unroll 1
+      for (int j = 0; j < kLaneVecs; ++j) {  // (a short loop, as in add_piece())
+        uint4 w = u[0];
+#pragma unroll
+        for (int i = 1; i < kLaneVecs; ++i) w = i == j ? u[i] : w;
+        add(w, std::true_type());
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLaneVecs; ++j) {
+        add(u[j], std::false_type());
+        if (vecs <= (j + 1) * 32) break;
+      }
     }
     float p, q;
     f2_unpack(add2(b0[0], b0[1]), p, q);
