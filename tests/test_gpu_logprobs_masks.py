@@ -100,10 +100,32 @@ def test_token_logprobs_extreme_scales(L, scale, size, dtype):
         check_logprobs(L, x, dtype, scale, 5, targets_for(rows, vocab))
 
 
-@pytest.mark.parametrize("value", [1e4, 1e6, 1e9, 1e20])
-def test_linear_logprobs_of_large_exact_logits(L, value):
-    """One entry of hidden is not 0, so a logit is a single product, exact in fp32: tolerances without a product's."""
-    check_exact_head(L, 5, 264, 5003, value)
+@pytest.mark.parametrize("rows,dim", [(5, 264), (8, 4096), (9, 264), (300, 520), (40, 2048), (300, 4096), (20, 8200)])
+@pytest.mark.parametrize("value", [0.0, 1e4, 1e6, 1e9, 1e20])
+def test_linear_logprobs_of_exact_logits(L, rows, dim, value):
+    """One entry of hidden is not 0, so a logit is a single product, exact in fp32: tolerances without a product's, the
+    same for any number of rows."""
+    check_exact_head(L, rows, dim, 5003, value)
+
+
+@pytest.mark.parametrize("rows,dim,vocab", [(9, 1032, 777), (300, 2048, 1500), (40, 4096, 1001), (260, 8200, 515), (3, 8200, 300)])
+def test_linear_logprobs_of_long_reductions(L, rows, dim, vocab):
+    """Sums of at most 64 steps of 16 (each cut: 2u of its partial sum), joined by one rounding each: a logit is off by at
+    most (128 + chunks) u sum |h w|, lse and ln p by the row's largest such error, twice."""
+    g = torch.Generator(device="cuda").manual_seed(dim + vocab)
+    h = torch.randn(rows, dim, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(vocab, dim, device="cuda", generator=g) * (2.5 / math.sqrt(dim))).bfloat16()
+    t = targets_for(rows, vocab)
+    for a, b in [(h, w), (h.abs(), (w.abs() / 16).bfloat16())]:   # signs at random, and all alike
+        out = call_head(L, a, b, t, 1.0)
+        x = a.double() @ b.double().T
+        logp, lse = softmax64(x, 1.0)
+        off = (128 + math.ceil(dim / 1024)) * U * (a.double().abs() @ b.double().abs().T).amax(1)
+        E, lnv = (8 + math.ceil(vocab / 64) + 5 * 20) * U, math.log(vocab)
+        close(out["lse"], lse, off + E + 4 * U * (lnv + x.amax(1).abs()), "lse")
+        ok = (t >= 0) & (t < vocab)
+        at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
+        close(out["logp"], torch.where(ok, at, torch.zeros_like(at)), 2 * off + E + 4 * U * (lnv + at.abs()), "logp")
 
 
 def exact_head(rows, dim, vocab, value, seed=0):

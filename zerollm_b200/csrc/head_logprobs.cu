@@ -34,6 +34,13 @@ constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of 
 // A short reduction (up to kHeld blocks) keeps the row tile of hidden in shared memory from one vocabulary tile to the
 // next; its ring holds weight blocks.  A longer one streams both through a ring of pairs.
 constexpr int kHeld = 8;
+// Reduction blocks that the tensor core sums at once; a longer reduction's chunks are added in fp32 by the epilogue.
+// Each step of 16 products is cut to fp32 toward zero, so a sum comes out too small in magnitude by 0.1 to 0.9 of 2^-24 for
+// every step behind it, which like a temperature moves a row's entropy (of 512 x 4096 x 8000, random: 2.2e-6 of itself).
+// Chunks of 64 steps bound that for any length (8e-7), at the time of the undivided sum: 16384 x 2048 x 32000 1.27 ms in a
+// burst, 1.485 ms sustained; chunks of 32 steps (4e-7) took 1.33 and 1.57 ms.
+constexpr int kChunk = 16;
+static_assert(kHeld <= kChunk, "a reduction that is held is one chunk");
 template <bool HELD> struct Smem {
   static constexpr int STAGES = HELD ? 5 : 6;
   static constexpr int STAGE_BYTES = HELD ? kTileBytes : 2 * kTileBytes;
@@ -192,27 +199,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       while (ok && seg.next(a)) {
         for (int nt = seg.nt0; nt < seg.nt1 && ok; ++nt) {
-          // both CTAs' epilogues have drained accumulator `acc`
-          if (!__all_sync(0xffffffffu, bounded_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, DEV_TIMEOUT_ACC))) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-          for (int kb = 0; kb < a.k_blocks; ++kb) {
-            if (HELD && nt == seg.nt0 && !bounded_wait_warp(&h_full[kb], h_phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
-            if (!bounded_wait_warp(&full[stage], phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+          for (int k0 = 0; k0 < a.k_blocks && ok; k0 += kChunk) {
+            // both CTAs' epilogues have drained accumulator `acc`
+            if (!__all_sync(0xffffffffu, bounded_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, DEV_TIMEOUT_ACC))) { ok = false; break; }
             tc_fence_after();
-            const uint32_t w_base = smem_u32(smem + L::RING + stage * L::STAGE_BYTES);
-            const uint32_t h_base = HELD ? smem_u32(smem + kb * kTileBytes) : w_base + kTileBytes;
+            const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+            const int k1 = HELD ? a.k_blocks : min(a.k_blocks, k0 + kChunk);
+            for (int kb = k0; kb < k1; ++kb) {
+              if (HELD && nt == seg.nt0 && !bounded_wait_warp(&h_full[kb], h_phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+              if (!bounded_wait_warp(&full[stage], phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
+              tc_fence_after();
+              const uint32_t w_base = smem_u32(smem + L::RING + stage * L::STAGE_BYTES);
+              const uint32_t h_base = HELD ? smem_u32(smem + kb * kTileBytes) : w_base + kTileBytes;
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              umma_f16_pair_w(d_tmem, smem_desc_sw128(h_base + k * 32, 16, 1024), smem_desc_sw128(w_base + k * 32, 16, 1024),
-                              IDESC, (kb > 0 || k > 0) ? 1u : 0u);
-            umma_commit_pair_w(&empty[stage], 0x3);
-            if (HELD && nt + 1 == seg.nt1) umma_commit_pair_w(&h_empty[kb], 0x3);
-            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+              for (int k = 0; k < BK / 16; ++k)
+                umma_f16_pair_w(d_tmem, smem_desc_sw128(h_base + k * 32, 16, 1024), smem_desc_sw128(w_base + k * 32, 16, 1024),
+                                IDESC, (kb > k0 || k > 0) ? 1u : 0u);
+              umma_commit_pair_w(&empty[stage], 0x3);
+              if (HELD && nt + 1 == seg.nt1) umma_commit_pair_w(&h_empty[kb], 0x3);
+              if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (!ok) break;
+            umma_commit_pair_w(&acc_full[acc], 0x3);
+            if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
           }
-          if (!ok) break;
-          umma_commit_pair_w(&acc_full[acc], 0x3);
-          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
         h_phase ^= 1u;
       }
@@ -229,33 +239,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = (a.targets && row < a.rows) ? a.targets[row] : -1;
       Running run;
       float xt = 0.f;
-      for (int nt = seg.nt0; nt < seg.nt1; ++nt) {
-        if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
-#pragma unroll 1
-        for (int c = share * (BN / kShares); c < (share + 1) * (BN / kShares); c += 32) {
-          const int n = nt * BN + c;
-          if (n >= a.vocab) break;
-          uint32_t u[32];
-          tmem_ld32(t_row + (uint32_t)c, u);
-          tmem_ld_wait();
-          float v[32];
+      // 32 columns of the tile, from column n of the vocabulary on
+      auto fold = [&](float (&v)[32], int n) {
+        if (n >= a.vocab) return;
+        if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
-          if (n + 32 > a.vocab) {  // the last tile: entries past the vocabulary have p = 0
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
-          }
-          if (t >= n && t < n + 32 && t < a.vocab) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
-          }
-          run.add_near(v, a.c);
+          for (int j = 0; j < 32; ++j) v[j] = n + j < a.vocab ? v[j] : -INFINITY;
         }
+        if (t >= n && t < n + 32 && t < a.vocab) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) xt = t == n + j ? v[j] : xt;
+        }
+        run.add_near(v, a.c);
+      };
+      auto drained = [&] {
         tc_fence_before();
         mbar_arrive_cluster(acc_empty_leader[acc]);
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      };
+      constexpr int COLS = BN / kShares;  // this warp's columns of a tile
+      for (int nt = seg.nt0; nt < seg.nt1 && ok; ++nt) {
+        const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(share * COLS);
+        const int n0 = nt * BN + share * COLS;
+        if constexpr (HELD) {  // one chunk: from tensor memory
+          if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < COLS && n0 + c < a.vocab; c += 32) {
+            uint32_t u[32];
+            tmem_ld32(t_row + (uint32_t)(acc * BN + c), u);
+            tmem_ld_wait();
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
+            fold(v, n0 + c);
+          }
+          drained();
+        } else {  // the sum of the chunks in registers; the last accumulator is free before its logits are folded
+          float v[COLS / 32][32] = {};
+          for (int kb = 0; kb < a.k_blocks; kb += kChunk) {
+            if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < COLS; c += 16) {
+              uint32_t u[16];
+              tmem_ld16(t_row + (uint32_t)(acc * BN + c), u);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                v[c / 32][c % 32 + j] += __uint_as_float(u[j]);
+            }
+            drained();
+          }
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < COLS / 32; ++c) fold(v[c], n0 + c * 32);
+        }
       }
       if (ok && row < a.rows) {  // this pair's partial of the row
         const Stats st = run.sums(a.c);
@@ -312,13 +351,6 @@ int pair_slots() {
   }
   return n;
 }
-
-// The tensor core cuts each step of 16 products to fp32 toward zero, so a logit comes out too small in magnitude by a
-// part that grows with the number of steps: measured against 64-bit sums 1.1e-7 to 3.6e-7 of it at dim 256, 1.3e-6 to
-// 5.4e-6 at 2048, 3.1e-6 to 1.4e-5 at 4096 (signs at random, shifted, or all alike), which is 0.12 to 0.9 of 2^-24 a
-// step.  Like a temperature, that moves every row's entropy the same way.  The scale makes up for 0.2 of 2^-24 a step;
-// logits of random signs then keep their random part alone (entropy of 16384 x 2048 x 32000: 1.7e-6 off without it).
-float scale_of(float scale, int dim) { return (float)(scale * (1.0 + 0.2 * ((dim + 15) / 16) * 0x1p-24)); }
 
 // ------------------------------------------------------------------ few rows
 // Up to 8 rows: the weight is read once, at the rate of device memory, and tensor-core tiles of 256 rows would be
@@ -515,7 +547,6 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
     return st != ZL_OK ? st : launch_after(what, head_join_kernel, 1, 256, (cudaStream_t)stream, a, scale, logp, entropy, lse);
   }
   const Plan p = make_plan(rows, dim, vocab);
-  scale = scale_of(scale, dim);
   CUtensorMap mh, mw;
   if (!make_tma_map(&mh, hidden, false, dim, rows, BK, BM, 128, 0) ||
       !make_tma_map(&mw, weight, false, dim, vocab, BK, BN / 2, 128, 0))
