@@ -303,8 +303,9 @@ zl_status zl_token_logprobs_f32(const float *logits, int64_t row_stride, const i
                                 float scale, int top_k, float *logp, float *entropy, float *lse, float *top_logp,
                                 int32_t *top_ids, zl_stream stream);
 /* Their gradient: d_logits[r, j] = scale ( g_logp[r] (1[j = t] - p_j) - g_entropy[r] p_j (ln p_j + entropy[r]) )
- * with lse and entropy as the forward wrote them.  g_logp or g_entropy may be NULL (a zero gradient; entropy is
- * then not read); rows without a target take nothing from g_logp, and rows whose lse is beyond 1e30 either way
+ * with lse and entropy as the forward wrote them (p is e^{y_j - lse}, off by 2^-24 |lse| of itself at most; where
+ * |lse| > 256 it is formed anew from the row).  g_logp or g_entropy may be NULL (a zero gradient; entropy is then not
+ * read); rows without a target take nothing from g_logp, and rows whose lse is beyond 1e30 either way
  * (wholly masked, or with a token forced by the type's highest value) have none.  d_logits may be logits (with its row stride)
  * but may not overlap it in any other way. */
 zl_status zl_token_logprobs_backward_bf16(const zl_bf16 *logits, int64_t row_stride, const int32_t *targets,

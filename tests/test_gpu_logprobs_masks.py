@@ -6,8 +6,9 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_logprobs import (DT, L, NINF, U, call_head, check_distill, check_logprobs, close, entropy64,  # noqa: F401
-                                     opts, softmax64, strided, targets_for)
+from tests.test_gpu_logprobs import (DT, FLUSH, L, NINF, U, call_backward, call_head, call_logprobs,  # noqa: F401
+                                     check_distill, check_logprobs, close, entropy64, err, half_step, opts, softmax64, strided,
+                                     targets_for)
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +206,62 @@ def test_distill_extreme_scales(L, scale, size, dtype):
         x, _ = strided(rows, vocab, dtype)
         x.copy_(torch.randn(rows, vocab, device="cuda", generator=g) * size)
         check_distill(L, x, dtype, 5, opts(L, scale=scale))
+
+
+# ------------------------------------------------------------------ gradient
+def check_backward(L, x, dtype, scale, which, dpad=0):
+    """Against the fp64 formula on the logits themselves (not on the saved lse, which may round away all of ln vocab):
+    p is off by E + (4 + 4 |ln p|) u, its factors by a few u, as in the forward."""
+    rows, vocab = x.shape
+    scale = C.c_float(scale).value
+    t = targets_for(rows, vocab)
+    out, _, _ = call_logprobs(L, x, dtype, t, scale, 0)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    gl = torch.randn(rows, device="cuda", generator=g) if which != "entropy" else None
+    ge = torch.randn(rows, device="cuda", generator=g) if which != "logp" else None
+    ent = out["entropy"] if ge is not None else None
+    d, buf = strided(rows, vocab, dtype, dpad)
+    call_backward(L, x, dtype, t, out["lse"], ent, gl, ge, scale, d)
+    logp, _ = softmax64(x, scale)
+    p = logp.exp()
+    l0 = torch.where(p > 0, logp, torch.zeros_like(p))
+    ok = (t >= 0) & (t < vocab)
+    hot = torch.zeros_like(p).scatter_(1, t.clamp(0, vocab - 1).long()[:, None], 1.0) * ok[:, None]
+    gg = (torch.zeros(rows, device="cuda") if gl is None else gl).double() * ok
+    h = (torch.zeros(rows, device="cuda") if ge is None else ge).double()
+    H = (torch.zeros(rows, device="cuda") if ent is None else ent).double()
+    want = scale * (gg[:, None] * (hot - p) - h[:, None] * p * (l0 + H[:, None]))
+    size = scale * (gg.abs()[:, None] * (hot + p) + h.abs()[:, None] * p * (l0.abs() + H.abs()[:, None] + 1))
+    tol = size * (err(vocab, dtype) + (4 * l0.abs() + 20) * U) + FLUSH * scale * (gg.abs() + h.abs() * (88 + H))[:, None]
+    # below kFarLse the saved lse counts, half a step of it
+    tol = tol + size * torch.where(out["lse"].abs() <= 256, 2 * U * out["lse"].abs(), torch.zeros_like(out["lse"])).double()[:, None]
+    close(d, want, tol + half_step(dtype) * (want.abs() + tol) + FLUSH, "d_logits")
+    mask = torch.ones_like(buf, dtype=torch.bool)
+    torch.as_strided(mask, d.shape, d.stride(), 0).fill_(False)
+    assert bool((buf[mask] == 7.0).all()), "wrote outside its rows"
+    y = x.clone() if x.is_contiguous() else x
+    call_backward(L, y, dtype, t, out["lse"], ent, gl, ge, scale, y)   # in the logits' place
+    if dpad == 0 and x.is_contiguous() and x.data_ptr() % 16 == y.data_ptr() % 16:
+        assert torch.equal(y, d)
+    else:  # (at another place within 16 bytes: the same formula, sums in another order)
+        close(y, want, tol + half_step(dtype) * (want.abs() + tol) + FLUSH, "d_logits in place")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("which", ["logp", "entropy", "both"])
+@pytest.mark.parametrize("value", MASKS)
+def test_token_logprobs_backward_finite_masks(L, value, which, dtype):
+    for rows, vocab, dpad in [(3, 900, 0), (3, 6400, 0), (1300, 1001, 0), (5, 6401, 3), (3, 40001, 0)]:
+        x, _ = finite_masks(rows, vocab, dtype, value, "some")
+        check_backward(L, x, dtype, 0.7, which, dpad)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("offset,scale", [(-1e9, 1.0), (-1e5, 1.3), (-270.0, 1.0), (50.0, 1.0), (242.0, 1.0), (300.0, 1.0), (1e3, 0.7),
+                                          (1e6, 1.0), (1e8, 1.0), (0.0, 1e4), (0.0, 100.0)])
+def test_token_logprobs_backward_far_from_zero(L, offset, scale, dtype):
+    for rows, vocab, pad, at, dpad in [(3, 900, 0, 0, 0), (2000, 640, 0, 0, 0), (2, 50001, 0, 0, 0), (5, 1001, 13, 3, 2), (4, 6, 0, 1, 0)]:
+        g = torch.Generator(device="cuda").manual_seed(vocab)
+        x, _ = strided(rows, vocab, dtype, pad, at)
+        x.copy_(torch.randn(rows, vocab, device="cuda", generator=g, dtype=torch.float64) * 3 + offset)
+        check_backward(L, x, dtype, scale, "both", dpad)

@@ -747,11 +747,58 @@ struct LogprobBwdArgs {
   int64_t d_stride;
 };
 
+// A row whose lse is so far from 0 that its rounding shows in p (kFarLse on, 2^-17 of p below it; a row masked with -1e9,
+// whose lse holds nothing of ln V, at the far end): one block finds the row's maximum and sum again and has all of its
+// gradient, read a second time after the whole row was read once (it may lie in the logits' place).  32768 x 6400 bf16
+// of such rows 224 us, 135 us of others.
+constexpr float kFarLse = 256.f;
+template <typename T, int NT>
+__device__ __forceinline__ void far_row(const T* x, T* d, int V, float scale, int t, float g, float h, float gh, bool same) {
+  constexpr int VEC = Elt<T>::VEC;
+  __shared__ float3 red[NT / 32];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const float c = scale * kLog2e;
+  const Span<T> sp(x, V, 0, 1);
+  RunningT<false> run;
+  for (int v = tid; v < sp.hi; v += NT) {
+    float f[VEC];
+    Elt<T>::unpack(load16(x + sp.head + (int64_t)v * VEC), f);
+    run.add_any(f, c);
+  }
+  const int single = sp.single(V, 0, 1, tid);
+  if (single >= 0) run.add_one(Elt<T>::get(x + single), c);
+  Stats s = run.sums(c);
+  s.join_warp(c);
+  if (lane == 0) red[tid >> 5] = s.pack();
+  __syncthreads();
+  s = lane < NT / 32 ? Stats(red[lane]) : Stats();
+  s.join_warp(c);
+  const float ln_s0 = logf(s.s0);
+  auto grad = [&](float f, int i) {
+    if (s.s0 == 0.f) return 0.f;
+    const float l = fmaf(f - s.m, scale, -ln_s0), p = ex2(l * kLog2e);
+    return p * fmaf(-h, fmaxf(l, kFloor), -gh) + (i == t ? g : 0.f);
+  };
+  if (same) {
+    for (int v = tid; v < sp.hi; v += NT) {
+      const int i0 = sp.head + v * VEC;
+      float f[VEC];
+      Elt<T>::unpack(load16(x + i0), f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], i0 + j);
+      *reinterpret_cast<uint4*>(d + i0) = Elt<T>::pack(f);
+    }
+    if (single >= 0) Elt<T>::put(d + single, grad(Elt<T>::get(x + single), single));
+  } else {
+    for (int i = tid; i < V; i += NT) Elt<T>::put(d + i, grad(Elt<T>::get(x + i), i));
+  }
+}
+
 // d_j = scale [ g (1[j = t] - p_j) - h p_j (ln p_j + H) ], element by element from the row's saved statistics.  One
 // block per (row, slice of the vocabulary); a thread has four vectors on the way at once, or, where logits and gradient
 // rows do not share their place within 16 bytes, that many bytes' worth of single elements.
 // With l = scale x - lse: d = p (-scale h l - scale (g + h H)), one exponential and paired fp32 instructions.  Masked
-// logits are kept at -2^40 (l finite, p = 0) while lse is not itself a mask's size.
+// logits are kept at -2^40 (l finite, p = 0).
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a, int slices) {
   constexpr int VEC = Elt<T>::VEC, U = 4;
@@ -780,13 +827,18 @@ __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a
   const float g = t >= 0 ? a.g_logp[r] * scale : 0.f;
   const float h = a.g_entropy ? a.g_entropy[r] * scale : 0.f, H = a.g_entropy ? a.entropy[r] : 0.f;
   const float gh = fmaf(h, H, g);
+  const bool far = fabsf(lse) > kFarLse && !none;  // (asked about once this thread's first loads are on their way)
   auto grad = [&](float f, int i) {
     if (none) return 0.f;
     const float l = fmaf(f, scale, -lse), p = ex2(l * kLog2e);
     return p * fmaf(-h, fmaxf(l, kFloor), -gh) + (i == t ? g : 0.f);  // (ln p kept off -inf where p = 0)
   };
   if (same) {
-    const bool fast = fabsf(lse) <= 1e6f;
+    if (far) {
+      if (part == 0) far_row<T, NT>(x, d, V, scale, t, g, h, gh, true);
+      return;
+    }
+    const bool fast = fabsf(lse) <= kFarLse;  // (not NaN, not beyond 1e30)
     const uint64_t s2 = f2_pack(scale, scale), n2 = f2_pack(-lse, -lse), e2 = f2_pack(kLog2e, kLog2e), h2 = f2_pack(-h, -h),
                    g2 = f2_pack(-gh, -gh);
 #pragma unroll
@@ -831,10 +883,12 @@ __global__ void __launch_bounds__(NT) logprobs_bwd_kernel(const LogprobBwdArgs a
       float f[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) f[j] = i0 + j * NT < hi ? Elt<T>::get(x + i0 + j * NT) : 0.f;
+      if (far) break;
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (i0 + j * NT < hi) Elt<T>::put(d + i0 + j * NT, grad(f[j], i0 + j * NT));
     }
+    if (far && part == 0) far_row<T, NT>(x, d, V, scale, t, g, h, gh, false);
   }
 }
 
