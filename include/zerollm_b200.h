@@ -295,7 +295,8 @@ zl_status zl_cross_entropy_fused_bf16(zl_bf16 *logits, const int32_t *targets, i
  *   entropy[r] = -sum_j p_j ln p_j,
  *   top_ids / top_logp [rows, top_k]: the top_k largest logits, largest first (equal ones by the lower index,
  *   NaN last), and their log probabilities.
- * logp, entropy, lse, top_logp may be NULL; targets may be NULL without logp.  top_k in [0, min(vocab, 128)]. */
+ * logp, entropy, lse, top_logp may be NULL; targets may be NULL without logp.  top_k in [0, min(vocab, 128)], and 0 for
+ * rows of more than 5505015 (bf16) or 1376251 (fp32) logits (ZL_EUNSUPPORTED otherwise). */
 zl_status zl_token_logprobs_bf16(const zl_bf16 *logits, int64_t row_stride, const int32_t *targets, int rows,
                                  int vocab, float scale, int top_k, float *logp, float *entropy, float *lse,
                                  float *top_logp, int32_t *top_ids, zl_stream stream);

@@ -265,3 +265,15 @@ def test_token_logprobs_backward_far_from_zero(L, offset, scale, dtype):
         x, _ = strided(rows, vocab, dtype, pad, at)
         x.copy_(torch.randn(rows, vocab, device="cuda", generator=g, dtype=torch.float64) * 3 + offset)
         check_backward(L, x, dtype, scale, "both", dpad)
+
+
+# ------------------------------------------------------------------ the longest rows
+@pytest.mark.parametrize("dtype,vocab", [("bf16", 5505015), ("f32", 1376251)])
+def test_alternatives_of_the_longest_rows(L, dtype, vocab):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, _ = strided(2, vocab, dtype, 5, 1)
+    x.copy_(torch.randn(2, vocab, device="cuda", generator=g) * 3)
+    check_logprobs(L, x, dtype, 1.0, 128, targets_for(2, vocab))
+    y, _ = strided(2, vocab + 1, dtype)
+    y.copy_(torch.randn(2, vocab + 1, device="cuda", generator=g) * 3)
+    check_logprobs(L, y, dtype, 1.0, 0, targets_for(2, vocab + 1))

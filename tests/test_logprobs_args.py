@@ -142,3 +142,15 @@ def test_model_entries_refuse_null_arguments(L):
     o = L.DistillOptions(1.0, 1.0, 1, 0.5, 0.5, 1.0)
     refused(L, "zl_model_distill_step", L.ZL_EINVAL, "null", None, A, A, A, 4, A, None, C.byref(o), 1, 128, 0.0, 1, None, None)
     refused(L, "zl_model_score", L.ZL_EINVAL, "null", None, A, A, 1, 128, 1.0, 0, A, A, A, None, None, None)
+
+
+@pytest.mark.parametrize("t,most", [("bf16", 5505015), ("f32", 1376251)])
+def test_alternatives_of_very_long_rows(L, t, most):
+    """The longest row whose alternatives are found, and one more: refused before anything runs, with no rows too (as
+    a model's scoring asks before its forward)."""
+    n = "zl_token_logprobs_" + t
+    f = getattr(L.load(), n)
+    for rows in (0, 2):
+        refused(L, n, L.ZL_EUNSUPPORTED, "alternatives", A, most + 1, A, rows, most + 1, 1.0, 1, A, A, A, A, A, None)
+    assert f(A, most, A, 0, most, 1.0, 1, A, A, A, A, A, None) == L.ZL_OK
+    assert f(A, most + 1, A, 0, most + 1, 1.0, 0, A, A, A, None, None, None) == L.ZL_OK

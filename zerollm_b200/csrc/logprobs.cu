@@ -1384,6 +1384,13 @@ template <typename T, int SECOND> zl_status launch_distill(const char* what, int
 }
 
 constexpr int kVocabMax = 1 << 30;  // (column arithmetic is 32-bit)
+// Most logits of a row with alternatives: the maxima of kMaxParts parts beside the rings of eight warps.
+template <typename T> constexpr int top_vocab() {
+  constexpr int pieces = (int)((kMaxDynamic - 8 * kDepth * kPieceBytes) / (32 * sizeof(typename Maxima<T>::Store)));
+  constexpr int vecs = kMaxParts * (pieces * kPieceVecs - 1) + kMaxParts - 1;
+  return (vecs - 1) * Elt<T>::VEC + Elt<T>::VEC - 1;
+}
+static_assert(top_vocab<__nv_bfloat16>() == 5505015 && top_vocab<float>() == 1376251, "as the header says");
 bool off_words(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) & 3) return true;
@@ -1414,6 +1421,9 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   if (top_k > 0 && !top_ids) return set_error(ZL_EINVAL, "token_logprobs: null top_ids");
   if (off_words({targets, logp, entropy, lse, top_logp, top_ids}))
     return set_error(ZL_EINVAL, "token_logprobs: a target or output array off a 4-byte boundary");
+  // (the vectors' maxima of a row fit into the shared memory of a cluster)
+  if (top_k > 0 && vocab > top_vocab<T>())
+    return set_error(ZL_EUNSUPPORTED, "token_logprobs: top alternatives of at most %d logits", top_vocab<T>());
   if (rows == 0) return ZL_OK;
   LogprobArgs a{logits, stride, targets, rows, vocab, top_k, 1, 0, scale, logp, entropy, lse, top_logp, top_ids};
   const int vecs = vocab / Elt<T>::VEC + 1;
@@ -1427,10 +1437,9 @@ zl_status token_logprobs(const T* logits, int64_t stride, const int32_t* targets
   if (nw == 2) return launch_rows<T, 2, 1>("token_logprobs", rows, 1, s, a);
   if (nw == 4) return launch_rows<T, 4, 1>("token_logprobs", rows, 1, s, a);
   a.parts = team_parts(rows, a.pieces);
-  for (;; a.parts *= 2) {
+  for (;; a.parts *= 2) {  // (ends at kMaxParts at the latest)
     a.pieces = (vecs / a.parts + 1 + kPieceVecs - 1) / kPieceVecs;
     if (logprobs_smem<T, 8, 1>(a) <= kMaxDynamic) break;
-    if (a.parts == kMaxParts) return set_error(ZL_EUNSUPPORTED, "token_logprobs: vocab too large for top alternatives");
   }
   return launch_rows<T, 8, 1>("token_logprobs", rows, a.parts, s, a);
 }
