@@ -527,7 +527,8 @@ template <typename T, int NW, int TEAMS> size_t logprobs_smem(const LogprobArgs&
          (a.k ? (size_t)TEAMS * a.pieces * 32 * sizeof(typename Maxima<T>::Store) : 0);
 }
 
-// NW warps to a row (TEAMS rows to a block), or a cluster of `parts` blocks of NW warps.  Top alternatives: the
+// NW warps to a row (TEAMS rows to a block), or a cluster of `parts` blocks of NW warps.  A single warp goes on to further
+// rows; the grid has a block (or cluster) for every row of several warps.  Top alternatives: the
 // k-th largest of the maxima of 32 to 256 disjoint sets of elements is a bound that at least k elements reach, and
 // few more where values come in any order; the maxima of the single vectors, kept in shared memory, say which
 // vectors to read again (from L2).  The candidates' ranks are counted.
@@ -731,6 +732,7 @@ __global__ void __launch_bounds__(NW * TEAMS * 32, NW == 1 ? kRowBlocks : 24 / N
         team_sync<NW>();
       }
     }
+    if (NW > 1) break;  // one row: red, parts_st and the groups have no barrier between a row's reads and the next one's writes
   }
   if (!entered) cg::this_cluster().barrier_wait();
 }
