@@ -324,8 +324,8 @@ zl_status zl_token_logprobs_backward_f32(const float *logits, int64_t row_stride
  *   loss_rows[r] = row_weight[r] (distill_weight KD + target_weight CE),
  *   *loss_out = grad_scale * sum_r loss_rows[r],  d_logits = the gradient of *loss_out.
  * teacher_ids / teacher_logits [rows, top_k], top_k in [0, 128]; an id not in [0, vocab) is no alternative (short
- * lists end in -1), an id given twice counts twice.  targets may be NULL with target_weight 0; a target not in
- * [0, vocab) adds nothing.  row_weight may be NULL (all 1); a row of weight 0 has loss and gradient 0 whatever
+ * lists end in -1), an id given twice counts twice.  A weight of 0 leaves its term out: the record is not read with
+ * distill_weight 0, and targets may be NULL with target_weight 0; a target not in [0, vocab) adds nothing.  row_weight may be NULL (all 1); a row of weight 0 has loss and gradient 0 whatever
  * it holds, as has a student row with nothing left.  d_logits may be NULL (the loss alone) or logits (with its
  * row stride), but may not overlap it in any other way; loss_out may be NULL. */
 typedef struct {

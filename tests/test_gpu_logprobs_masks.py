@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from tests.test_gpu_logprobs import (DT, FLUSH, L, NINF, U, call_backward, call_head, call_logprobs,  # noqa: F401
-                                     check_distill, check_logprobs, close, entropy64, err, half_step, opts, softmax64, strided,
-                                     targets_for)
+                                     check_distill, check_logprobs, close, entropy64, err, half_step, opts, softmax64, stream,
+                                     strided, targets_for)
 
 pytestmark = pytest.mark.gpu
 
@@ -277,3 +277,27 @@ def test_alternatives_of_the_longest_rows(L, dtype, vocab):
     y, _ = strided(2, vocab + 1, dtype)
     y.copy_(torch.randn(2, vocab + 1, device="cuda", generator=g) * 3)
     check_logprobs(L, y, dtype, 1.0, 0, targets_for(2, vocab + 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [1.0, 0.5, 0.7])
+def test_distill_without_weight_reads_no_record(L, scale, dtype):
+    """distill_weight 0 beside a record of NaN, infinities and values beyond any probability: the cross-entropy's loss and
+    gradient, the same as without a record."""
+    rows, vocab, k = 6, 1001, 9
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(rows, vocab, device="cuda", generator=g) * 3).to(DT[dtype])
+    t = targets_for(rows, vocab)
+    ids = torch.randint(0, vocab, (rows, k), device="cuda", generator=g, dtype=torch.int32)
+    for bad in (math.nan, math.inf, 3e38):
+        v = torch.full((rows, k), bad, device="cuda")
+        for normalize in (0, 1):
+            o = opts(L, scale=scale, kd=0.0, ce=0.7, normalize=normalize)
+            got = []
+            for n in (k, 0):
+                lr, lo, d = torch.empty(rows, device="cuda"), torch.empty(1, device="cuda"), torch.empty_like(x)
+                L.call(f"zl_distill_topk_{dtype}", x.data_ptr(), vocab, ids.data_ptr(), v.data_ptr(), n, t.data_ptr(), None,
+                       C.byref(o), rows, vocab, d.data_ptr(), vocab, lr.data_ptr(), lo.data_ptr(), stream())
+                got.append((lr, lo, d))
+            for a, b in zip(*got):
+                assert torch.isfinite(a.float()).all() and torch.equal(a, b)

@@ -1493,7 +1493,9 @@ zl_status distill_topk(const T* logits, int64_t stride, const int32_t* ids, cons
   if (off_words({ids, values, targets, row_weight, loss_rows, loss_out}))
     return set_error(ZL_EINVAL, "%s: an array of 4-byte values off a 4-byte boundary", what);
   if (rows > 0) {
-    DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, k, 1, *opt, d, d_stride, loss_rows};
+    // (without weight the teacher's record is not read: whatever it holds, 0 times it is 0)
+    const int used = opt->distill_weight == 0.f ? 0 : k;
+    DistillArgs a{logits, stride, ids, values, targets, row_weight, rows, vocab, used, 1, *opt, d, d_stride, loss_rows};
     const int pieces = (vocab / Elt<T>::VEC + kPieceVecs) / kPieceVecs;
     const int nw = team_warps(rows, pieces);
     if (nw == 8) a.parts = team_parts(rows, pieces);
