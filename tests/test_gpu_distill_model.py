@@ -211,3 +211,23 @@ def test_numpy_front_end():
     want = np.where(has, -l1[np.arange(M), np.clip(t, 0, N - 1)], 0)
     assert np.abs(rows - want).max() < tol and abs(loss - 0.25 * want.sum()) < tol * M
     assert np.abs(dx.reshape(M, N) - 0.25 * has[:, None] * (np.exp(l1) - hot)).max() < tol
+
+
+def test_score_on_another_stream_has_memory_of_its_own():
+    """The outputs of a call on another stream do not lie in memory that a kernel of the current stream, still under way,
+    will write: memory freed there belongs to that stream."""
+    m, ids, tg = make()
+    want = m.score(ids, tg, 3, 128, top_k=5)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    m.score(ids, tg, 3, 128, top_k=5, stream=s)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        torch.cuda._sleep(20_000_000)                         # some 10 ms
+        old = [torch.full((384,), 7.0, device="cuda") for _ in range(8)] + [torch.full((384, 5), 7.0, device="cuda") for _ in range(4)]
+        del old                                               # freed, but written only when the sleep is over
+        got = m.score(ids, tg, 3, 128, top_k=5, stream=s)
+        torch.cuda.synchronize()
+        for k in want:
+            assert torch.equal(got[k], want[k]), k
+    m.close()

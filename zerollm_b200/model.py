@@ -155,14 +155,17 @@ class ZeroLLM:
     def score(self, ids: torch.Tensor, targets: torch.Tensor | None, B: int, S: int, scale: float = 1.0, top_k: int = 0,
               stream=None) -> dict:
         """Log probabilities of `targets` (where given), entropy and log-sum-exp of each of the B * S rows, and with
-        top_k > 0 the top alternatives' ids and log probabilities [B * S, top_k]."""
+        top_k > 0 the top alternatives' ids and log probabilities [B * S, top_k].  With alternatives all of them are of
+        the logits rounded to bf16, as the training step has them; without, of fp32 sums.  The outputs belong to
+        `stream` where one is given: another stream waits for it before it reads them."""
         n = B * S
-        out = {"entropy": torch.empty(n, device="cuda"), "lse": torch.empty(n, device="cuda")}
-        if targets is not None:
-            out["logp"] = torch.empty(n, device="cuda")
-        if top_k:
-            out["top_logp"] = torch.empty(n, top_k, device="cuda")
-            out["top_ids"] = torch.empty(n, top_k, dtype=torch.int32, device="cuda")
+        with torch.cuda.stream(stream):  # (memory that this stream may write now, whatever runs on the current one)
+            out = {"entropy": torch.empty(n, device="cuda"), "lse": torch.empty(n, device="cuda")}
+            if targets is not None:
+                out["logp"] = torch.empty(n, device="cuda")
+            if top_k:
+                out["top_logp"] = torch.empty(n, top_k, device="cuda")
+                out["top_ids"] = torch.empty(n, top_k, dtype=torch.int32, device="cuda")
         p = {k: v.data_ptr() for k, v in out.items()}
         L.call("zl_model_score", self.h, ids.data_ptr(), None if targets is None else targets.data_ptr(), B, S, scale, top_k,
                p.get("logp"), p["entropy"], p["lse"], p.get("top_logp"), p.get("top_ids"), _stream(stream))
