@@ -231,3 +231,25 @@ def test_score_on_another_stream_has_memory_of_its_own():
         for k in want:
             assert torch.equal(got[k], want[k]), k
     m.close()
+
+
+def test_tensors_of_another_kind_are_refused():
+    """Ids as topk() gives them (64 bits), transposed records, other types, counts and devices are no arrays that the
+    library may read by their address."""
+    m, ids, tg = make()
+    n, k = 384, 4
+    t_ids = torch.zeros(n, k, device="cuda", dtype=torch.int32)
+    t_val = torch.zeros(n, k, device="cuda")
+    w = torch.ones(n, device="cuda")
+    before = m.grads()
+    for args, kw in [((t_ids.long(), t_val, tg), {}), ((t_ids, t_val.bfloat16(), tg), {}), ((t_ids, t_val.T.contiguous().T, tg), {}),
+                     ((t_ids[:200], t_val[:200], tg), {}), ((t_ids.cpu(), t_val, tg), {}), ((t_ids, t_val, tg.long()), {}),
+                     ((t_ids, t_val, tg[:100]), {}), ((t_ids, t_val, tg), dict(row_weight=w[:5])),
+                     ((t_ids, t_val, tg), dict(row_weight=w.double()))]:
+        with pytest.raises(AssertionError):
+            m.distill_step(ids, *args, 3, 128, 0.0, **kw)
+    for bad in (tg.long(), tg[:100], tg.cpu()):
+        with pytest.raises(AssertionError):
+            m.score(ids, bad, 3, 128)
+    assert np.array_equal(before, m.grads())
+    m.close()

@@ -79,6 +79,12 @@ def _stream(stream):
     return C.c_void_p(stream.cuda_stream)
 
 
+def _packed(name: str, t: torch.Tensor, dtype: torch.dtype, n: int):
+    """What the library takes by its address: at least `n` packed elements of `dtype` on the GPU."""
+    assert t.dtype == dtype and t.is_cuda and t.is_contiguous() and t.numel() >= n, \
+        f"{name}: {n} packed elements of {dtype} on the GPU, not {t.dtype} {tuple(t.shape)} on {t.device}"
+
+
 class ZeroLLM:
     def __init__(self, cfg: Config, max_tokens: int, seed: int = 0, init_std: float = 0.02):
         L.load()
@@ -144,9 +150,15 @@ class ZeroLLM:
                      row_weight: torch.Tensor | None = None, update: bool = True, stream=None) -> torch.Tensor:
         """train_step with the distillation loss on a teacher's record ([B * S, k] ids and logits, as `score` of the
         teacher returns them), averaged over the rows.  Returns the device loss."""
-        k = teacher_ids.shape[-1]
-        assert teacher_ids.numel() == teacher_logits.numel() == B * S * k
-        opt = L.DistillOptions(scale, 1.0, int(normalize), distill_weight, target_weight, 1.0 / (B * S))
+        n, k = B * S, teacher_ids.shape[-1]
+        assert teacher_ids.numel() == teacher_logits.numel() == n * k
+        _packed("teacher_ids", teacher_ids, torch.int32, n * k)
+        _packed("teacher_logits", teacher_logits, torch.float32, n * k)
+        if targets is not None:
+            _packed("targets", targets, torch.int32, n)
+        if row_weight is not None:
+            _packed("row_weight", row_weight, torch.float32, n)
+        opt = L.DistillOptions(scale, 1.0, int(normalize), distill_weight, target_weight, 1.0 / n)
         L.call("zl_model_distill_step", self.h, ids.data_ptr(), teacher_ids.data_ptr(), teacher_logits.data_ptr(), k,
                None if targets is None else targets.data_ptr(), None if row_weight is None else row_weight.data_ptr(),
                C.byref(opt), B, S, lr, int(update), self.loss_dev.data_ptr(), _stream(stream))
@@ -159,6 +171,8 @@ class ZeroLLM:
         the logits rounded to bf16, as the training step has them; without, of fp32 sums.  The outputs belong to
         `stream` where one is given: another stream waits for it before it reads them."""
         n = B * S
+        if targets is not None and n <= self.max_tokens:  # (the library refuses more)
+            _packed("targets", targets, torch.int32, n)
         with torch.cuda.stream(stream):  # (memory that this stream may write now, whatever runs on the current one)
             out = {"entropy": torch.empty(n, device="cuda"), "lse": torch.empty(n, device="cuda")}
             if targets is not None:
