@@ -45,3 +45,15 @@ def test_trainer_cli_runs(tmp_path):
     assert rc == 0
     assert (tmp_path / "ck" / "config.bin").exists()
     assert (tmp_path / "ck" / "optimizer" / "adamw_m.bin").exists()
+
+
+def test_teacher_arguments_are_refused():
+    """Before anything is read or run."""
+    from zerollm_b200.model import Config
+    from zerollm_b200.trainer import Trainer
+
+    cfg = Config(vocab_size=100)
+    for bad in (dict(teacher_top_k=0), dict(teacher_top_k=-3), dict(teacher_top_k=101), dict(temperature=0.0),
+                dict(temperature=float("nan")), dict(temperature=-1.0), dict(teacher_weight=float("inf"))):
+        with pytest.raises(ValueError):
+            Trainer(cfg, None, None, batch=4, seq=128, lr=1e-3, teacher="nowhere", **bad)

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import os
 import sys
 import time
@@ -48,8 +49,16 @@ class Trainer:
                  teacher: str | None = None, teacher_top_k: int = 16, teacher_weight: float = 0.5,
                  temperature: float = 1.0):
         """teacher: a checkpoint directory (of the same configuration) to distill from; epochs then train on
-        teacher_weight * T^2 * KL(teacher's top k || student), both at temperature T, plus (1 - teacher_weight) *
-        cross-entropy."""
+        teacher_weight * T^2 * KL(teacher's top k, renormalised || student), both at temperature T, plus
+        (1 - teacher_weight) * cross-entropy."""
+        if teacher is not None:
+            most = min(128, cfg.vocab_size)
+            if not 1 <= teacher_top_k <= most:
+                raise ValueError(f"teacher_top_k must be in [1, {most}], not {teacher_top_k}")
+            if not 1e-4 <= temperature <= 1e4:
+                raise ValueError(f"temperature must be in [1e-4, 1e4], not {temperature}")
+            if not math.isfinite(teacher_weight):
+                raise ValueError(f"teacher_weight must be finite, not {teacher_weight}")
         self.rank, self.world = rank, world
         self.batch, self.seq, self.lr = batch, seq, lr
         torch.cuda.set_device(local_rank)
