@@ -253,3 +253,48 @@ def test_tensors_of_another_kind_are_refused():
             m.score(ids, bad, 3, 128)
     assert np.array_equal(before, m.grads())
     m.close()
+
+
+@pytest.mark.parametrize("T,weight,k", [(2.0, 0.75, 8), (1.0, 0.3, 3), (4.0, 1.0, 20)])
+def test_trainer_step_is_the_distillation_step(tmp_path, T, weight, k):
+    """A step of the trainer with a teacher: loss and gradients of the explicit calls on a model of the same weights, and
+    the loss by its formula from both models' fp32 logits.  The step's logits are bf16: a student's ln p is off by twice
+    2^-9 of the largest logit at scale 1 / T, a teacher's q by twice that of itself, so q (ln q - ln p) by four of them
+    times (1 + |ln q - ln p|)."""
+    from zerollm_b200 import Config, ZeroLLM, trainer
+    cfg = Config(vocab_size=256, embed_dim=128, num_layers=2, num_heads=2, ff_hidden_dim=256, max_seq_len=128)
+    B, S, V = 4, 128, 256
+    t = ZeroLLM(cfg, B * S, seed=11, init_std=0.1)
+    t.save(str(tmp_path / "teacher"))
+    tokens, offsets = trainer.synthetic_stories(60, 150, 64, seed=4)
+    tr = trainer.Trainer(cfg, tokens, offsets, batch=B, seq=S, lr=1e-3, seed=1, teacher=str(tmp_path / "teacher"),
+                         teacher_top_k=k, teacher_weight=weight, temperature=T)
+    m = ZeroLLM(cfg, B * S, seed=5, init_std=0.1)
+    m.set_optimizer()
+    tr.model.set_params(m.params())
+    g = torch.Generator(device="cuda").manual_seed(2)
+    tr.d_ids.copy_(torch.randint(0, V, (B * S,), device="cuda", generator=g))
+    tr.d_tg.copy_(torch.randint(0, V, (B * S,), device="cuda", generator=g))
+    ls, lt = torch.empty(B * S, V, device="cuda"), torch.empty(B * S, V, device="cuda")
+    m.forward(tr.d_ids, B, S, ls)
+    t.forward(tr.d_ids, B, S, lt)
+    rec = t.score(tr.d_ids, None, B, S, 1.0 / T, k)
+    at = rec["top_ids"].long()
+    lq = torch.log_softmax(lt.double().gather(1, at) / T, 1)
+    lp = torch.log_softmax(ls.double() / T, 1).gather(1, at)
+    ce = -torch.log_softmax(ls.double(), 1).gather(1, tr.d_tg.long()[:, None]).mean()
+    want = weight * T * T * (lq.exp() * (lq - lp)).sum(1).mean() + (1 - weight) * ce
+    loss = float(tr.train_step())
+    got = tr.model.grads()
+    other = float(m.distill_step(tr.d_ids, rec["top_ids"], rec["top_logp"], tr.d_tg, B, S, 1e-3, scale=1.0 / T,
+                                 distill_weight=weight * T * T, target_weight=1.0 - weight))
+    assert abs(loss - other) <= 1e-5 * abs(other) and rel(got, m.grads()) < GRAD_TOL
+    step = 2.0 ** -9 * float(torch.maximum(ls.abs().amax(), lt.abs().amax()))
+    slack = weight * T * T * 4 * step / T * (1 + float((lq - lp).abs().max())) + (1 - weight) * 2 * step
+    assert abs(loss - float(want)) < slack
+    # a step on the cross-entropy alone would fail: its loss is within 2 step of ce, and slack >= step (4 weight T + 2 - 2
+    # weight) >= 2 step for T >= 1/2, so it is more than 2 slack - slack from the loss wanted
+    assert abs(float(want) - float(ce)) > 2 * slack
+    tr.close()
+    t.close()
+    m.close()
