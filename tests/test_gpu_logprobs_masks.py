@@ -301,3 +301,55 @@ def test_distill_without_weight_reads_no_record(L, scale, dtype):
                 got.append((lr, lo, d))
             for a, b in zip(*got):
                 assert torch.isfinite(a.float()).all() and torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ maxima that rise
+def rising(rows, vocab, dtype, offset):
+    """Ascending rows of ordinary spread about `offset`: every piece of a row raises the running maximum."""
+    g = torch.Generator(device="cuda").manual_seed(vocab + 7)
+    x, _ = strided(rows, vocab, dtype)
+    v = torch.randn(rows, vocab, device="cuda", generator=g, dtype=torch.float64).sort(dim=1).values
+    x.copy_(v + offset)
+    return x
+
+
+OFFSETS = [-3e5, -5e3, 100.0, 1e3, 3e3, 5e3, 2e4, 9e4, 1.7e5, 3e5]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("offset", OFFSETS)
+def test_token_logprobs_of_rising_rows(L, offset, dtype):
+    for rows, vocab in [(3, 900), (1300, 3001), (3, 20000), (2, 140000)]:
+        for scale in (1.0, 0.7):
+            check_logprobs(L, rising(rows, vocab, dtype, offset), dtype, scale, 5, targets_for(rows, vocab))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("offset", OFFSETS)
+def test_distill_of_rising_rows(L, offset, dtype):
+    for rows, vocab in [(5, 901), (400, 3001), (3, 20000), (2, 140000)]:
+        for o in OPTIONS:
+            check_distill(L, rising(rows, vocab, dtype, offset), dtype, 5, opts(L, **o))
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("offset", [1e3, 3e3, 5e3, 9e4])
+def test_linear_logprobs_of_rising_exact_logits(L, offset, rows):
+    """Logits of a single product each, ascending over the vocabulary in steps of bf16."""
+    dim, vocab = 136, 3000
+    h = torch.zeros(rows, dim, device="cuda")
+    h[:, 3] = 1.0
+    w = torch.zeros(vocab, dim, device="cuda")
+    step = 2.0 ** (math.floor(math.log2(offset)) - 7)
+    w[:, 3] = offset + step * torch.arange(vocab, device="cuda").div(200, rounding_mode="floor")
+    h, w = h.bfloat16(), w.bfloat16()
+    t = targets_for(rows, vocab)
+    scale = C.c_float(0.3 / step).value                       # (neighbours 0.3 apart)
+    out = call_head(L, h, w, t, scale)
+    logp, lse = softmax64(h.double() @ w.double().T, scale)
+    E, lnv = (8 + math.ceil(vocab / 64) + 5 * 20) * U, math.log(vocab)
+    close(out["lse"], lse, E + 4 * U * (lnv + scale * offset * 1.2), "lse")
+    close(out["entropy"], entropy64(logp), E * (2 + lnv) + 4 * U * (lnv + 1), "entropy")
+    ok = (t >= 0) & (t < vocab)
+    at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
+    close(out["logp"], torch.where(ok, at, torch.zeros_like(at)), E + 4 * U * (lnv + at.abs()), "logp")

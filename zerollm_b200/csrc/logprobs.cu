@@ -949,14 +949,14 @@ template <int SECOND> struct Exponent {
     mc1 = near ? m * kLog2e : 0.f;
   }
   __device__ __forceinline__ bool far() const { return sub != 0.f; }
-  // factors that make sums of e and e1 exact about m
-  __device__ __forceinline__ void settle(float& f, float& f1) const {
+  // factors that make sums of e and e1 exact about m (SIGN 1; -1: the other way)
+  template <int SIGN = 1> __device__ __forceinline__ void settle(float& f, float& f1) const {
     f = f1 = 1.f;
     if (!far() && m != -INFINITY) {
-      const float off = fmaf(m, c, -mc) * kLn2;
-      f = 1.f - off;
-      f1 = SECOND == kSquare ? fmaf(-2.f, off, 1.f) : SECOND == kFourth ? fmaf(-4.f, off, 1.f)
-           : SECOND == kOwn ? fmaf(-kLn2, fmaf(m, kLog2e, -mc1), 1.f) : 1.f;
+      const float off = SIGN * fmaf(m, c, -mc);
+      f = take_out(off);
+      f1 = SECOND == kSquare ? take_out(2.f * off) : SECOND == kFourth ? take_out(4.f * off)
+           : SECOND == kOwn ? take_out(SIGN * fmaf(m, kLog2e, -mc1)) : 1.f;
     }
   }
   // of a pair; its difference to m where that is formed first (FAR: it may be)
@@ -1023,12 +1023,21 @@ __device__ __forceinline__ Sums2 distill_sums(Feed<T, NW>& feed, uint32_t& taken
   ex.at(-INFINITY, c);
   float s = 0.f, h = 0.f;  // about ex
   auto raise = [&](float most) {
-    float f, f1;
-    ex.settle(f, f1);
-    t.m = ex.m; t.s = s * f; t.h = h * f1;
-    t.rebase(most, c);
-    s = t.s; h = t.h;
+    const Exponent<SECOND> was = ex;
     ex.at(most, c);
+    float f, f1;
+    if (!was.far() && was.m != -INFINITY && !ex.far()) {  // from one fl(m c) to the other
+      f = ex2(was.mc - ex.mc);
+      f1 = SECOND == kSquare ? f * f : SECOND == kFourth ? (f * f) * (f * f) : SECOND == kOwn ? ex2(was.mc1 - ex.mc1) : 1.f;
+      s *= f;
+      h *= f1;
+    } else {
+      was.settle(f, f1);
+      t.m = was.m; t.s = s * f; t.h = h * f1;
+      t.rebase(most, c);
+      ex.template settle<-1>(f, f1);
+      s = t.s * f; h = t.h * f1;
+    }
   };
   auto one = [&](float x) {
     if (x > ex.m) raise(x);

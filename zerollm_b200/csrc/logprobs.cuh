@@ -45,11 +45,15 @@ __device__ __forceinline__ float ex2(float t) {
 // ------------------------------------------------------------------ running softmax statistics
 // c = scale * log2(e).  Sums of e = 2^((x - m) c) and e (x - m) c about the running maximum m.  A masked logit
 // (-inf) has e = 0; it is kept off -inf before anything is multiplied with e.  A NaN or +inf logit makes s0 and
-// s1 NaN.  While |m c| <= kNear the exponent is one fused product x c - fl(m c); the rounding of m c, at most 2^-12
-// there, is taken out of the sums again, to first order (the rest is below 2^-25), when they leave the thread or m
-// rises.  Beyond it (large logits, masks of finite values) the exponent is (x - m) c, of a difference that is exact
-// where x is near m.
+// s1 NaN.  While |m c| <= kNear the exponent is one fused product x c - fl(m c): the running sums are about fl(m c), whose
+// rounding off = m c - fl(m c), at most 2^-12 there, is taken out of them when they leave the thread.  Beyond it (large
+// logits, masks of finite values) the exponent is (x - m) c, of a difference that is exact where x is near m.
 constexpr float kNear = 0x1p13f;
+// 2^-off of such a rounding, to second order
+__device__ __forceinline__ float take_out(float off) {
+  const float x = off * kLn2;
+  return fmaf(x, fmaf(x, 0.5f, -1.f), 1.f);
+}
 constexpr float kClamp = -0x1p96f;   // masked logits in fused products: e = 0 beside any |m c| <= kNear
 constexpr uint32_t kClampBf16 = 0xef80ef80u;
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -103,7 +107,7 @@ template <bool ENTROPY> struct RunningT {
     Stats s;
     s.m = m; s.s0 = s0; s.s1 = s1;
     if (near() && m != -INFINITY) {  // m c - fl(m c), exact
-      const float off = fmaf(m, c, -mc), f = fmaf(-off, kLn2, 1.f);
+      const float off = fmaf(m, c, -mc), f = take_out(off);
       s.s1 = f * fmaf(-off, s.s0, s.s1);
       s.s0 *= f;
     }
@@ -111,10 +115,22 @@ template <bool ENTROPY> struct RunningT {
   }
   // a maximum above m of elements to come
   __device__ __forceinline__ void raise(float most, float c) {
-    Stats s = sums(c);
-    s.rebase(most, c);
-    m = most; mc = m * c;
-    s0 = s.s0; s1 = s.s1;
+    const float most_c = most * c;
+    if (near() && m != -INFINITY && fabsf(most_c) <= kNear) {  // from fl(m c) to fl(most c)
+      const float d = mc - most_c, f = ex2(d);
+      s1 = f * fmaf(d, s0, s1);
+      s0 *= f;
+    } else {
+      Stats s = sums(c);
+      s.rebase(most, c);
+      s0 = s.s0; s1 = s.s1;
+      if (fabsf(most_c) <= kNear) {  // from most c to fl(most c)
+        const float off = fmaf(most, c, -most_c), f = take_out(-off);
+        s1 = f * fmaf(off, s0, s1);
+        s0 *= f;
+      }
+    }
+    m = most; mc = most_c;
   }
   // sums of N elements about m, none above it: pairs of partial sums (paired fp32 instructions).  NEAR: by the fused
   // product, which has to hold, and none below kClamp; otherwise by whichever holds, of any values
