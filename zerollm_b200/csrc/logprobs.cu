@@ -302,13 +302,14 @@ __device__ __forceinline__ void add_piece(RunningT<E>& s, const uint4 (&u)[kLane
   if (most > s.m) s.raise(most, c);
   if (__any_sync(0xffffffffu, !s.near())) {
 #pragma unroll 1
-    for (int j = 0; j < kLaneVecs; ++j) {  // (a short loop: unrolled it cost the rows that never come here 3%)
+    for (int j = 0; j < kLaneVecs; ++j) {  // (by elements, in a short loop: in pairs, or unrolled, it cost other rows 2%, 3%)
       uint4 w = u[0];
 #pragma unroll
       for (int i = 1; i < kLaneVecs; ++i) w = i == j ? u[i] : w;
       float f[VEC];
       Elt<T>::unpack(w, f);
-      s.template add<false>(f, c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s.add_one(f[i], c);
     }
   } else if (vecs >= kPieceVecs) {
     add_vecs<T, kLaneVecs>(s, u, c);
@@ -936,7 +937,7 @@ struct Sums2 {
 };
 
 // A thread's exponentials about a maximum m: x c - fl(m c), the rounding of m c taken out by settle() (as in RunningT)
-// while |m| times the larger of both factors is at most kNear (the fourth power's rounding is then four times 2^-14);
+// while |m| times the larger of both factors is at most kNear (the fourth power's rounding is then four times 2^-9);
 // (x - m) c beyond it.
 template <int SECOND> struct Exponent {
   float m, c, sub, mc, mc1;  // sub: -m where the difference is formed first (mc and mc1 are 0 then), else 0
@@ -949,15 +950,25 @@ template <int SECOND> struct Exponent {
     mc1 = near ? m * kLog2e : 0.f;
   }
   __device__ __forceinline__ bool far() const { return sub != 0.f; }
-  // factors that make sums of e and e1 exact about m (SIGN 1; -1: the other way)
-  template <int SIGN = 1> __device__ __forceinline__ void settle(float& f, float& f1) const {
+  // what m c and m log2 e lost to rounding where they are used
+  __device__ __forceinline__ float off() const { return far() ? 0.f : fmaf(m, c, -mc); }
+  __device__ __forceinline__ float off1() const { return far() ? 0.f : fmaf(m, kLog2e, -mc1); }
+  // factors that make sums of e and e1 exact about m
+  __device__ __forceinline__ void settle(float& f, float& f1) const {
     f = f1 = 1.f;
-    if (!far() && m != -INFINITY) {
-      const float off = SIGN * fmaf(m, c, -mc);
-      f = take_out(off);
-      f1 = SECOND == kSquare ? take_out(2.f * off) : SECOND == kFourth ? take_out(4.f * off)
-           : SECOND == kOwn ? take_out(SIGN * fmaf(m, kLog2e, -mc1)) : 1.f;
+    if (m != -INFINITY) {
+      f = take_out(off());
+      f1 = SECOND == kSquare ? take_out(2.f * off()) : SECOND == kFourth ? take_out(4.f * off())
+           : SECOND == kOwn ? take_out(off1()) : 1.f;
     }
+  }
+  // a larger maximum M, and the factors that take sums of e and e1 there
+  __device__ __forceinline__ void raise(float M, float& f, float& f1) {
+    const Exponent was = *this;
+    at(M, c);
+    f = ex2(fmaxf((was.m - M) * c + (off() - was.off()), kFloor));  // (also where m was -inf)
+    f1 = SECOND == kSquare ? f * f : SECOND == kFourth ? (f * f) * (f * f)
+         : SECOND == kOwn ? ex2(fmaxf((was.m - M) * kLog2e + (off1() - was.off1()), kFloor)) : 1.f;
   }
   // of a pair; its difference to m where that is formed first (FAR: it may be)
   template <bool FAR> __device__ __forceinline__ uint64_t about(uint64_t x) const { return FAR ? add2(x, f2_pack(sub, sub)) : x; }
@@ -1023,21 +1034,10 @@ __device__ __forceinline__ Sums2 distill_sums(Feed<T, NW>& feed, uint32_t& taken
   ex.at(-INFINITY, c);
   float s = 0.f, h = 0.f;  // about ex
   auto raise = [&](float most) {
-    const Exponent<SECOND> was = ex;
-    ex.at(most, c);
     float f, f1;
-    if (!was.far() && was.m != -INFINITY && !ex.far()) {  // from one fl(m c) to the other
-      f = ex2(was.mc - ex.mc);
-      f1 = SECOND == kSquare ? f * f : SECOND == kFourth ? (f * f) * (f * f) : SECOND == kOwn ? ex2(was.mc1 - ex.mc1) : 1.f;
-      s *= f;
-      h *= f1;
-    } else {
-      was.settle(f, f1);
-      t.m = was.m; t.s = s * f; t.h = h * f1;
-      t.rebase(most, c);
-      ex.template settle<-1>(f, f1);
-      s = t.s * f; h = t.h * f1;
-    }
+    ex.raise(most, f, f1);
+    s *= f;
+    h *= f1;
   };
   auto one = [&](float x) {
     if (x > ex.m) raise(x);

@@ -46,10 +46,10 @@ __device__ __forceinline__ float ex2(float t) {
 // c = scale * log2(e).  Sums of e = 2^((x - m) c) and e (x - m) c about the running maximum m.  A masked logit
 // (-inf) has e = 0; it is kept off -inf before anything is multiplied with e.  A NaN or +inf logit makes s0 and
 // s1 NaN.  While |m c| <= kNear the exponent is one fused product x c - fl(m c): the running sums are about fl(m c), whose
-// rounding off = m c - fl(m c), at most 2^-12 there, is taken out of them when they leave the thread.  Beyond it (large
+// rounding off = m c - fl(m c), at most 2^-7 there, is taken out of them when they leave the thread.  Beyond it (large
 // logits, masks of finite values) the exponent is (x - m) c, of a difference that is exact where x is near m.
-constexpr float kNear = 0x1p13f;
-// 2^-off of such a rounding, to second order
+constexpr float kNear = 0x1p18f;  // (rows about -1e5, or masked with it, at the full rate)
+// 2^-off of such a rounding, to second order (the third is below 2^-25)
 __device__ __forceinline__ float take_out(float off) {
   const float x = off * kLn2;
   return fmaf(x, fmaf(x, 0.5f, -1.f), 1.f);
@@ -113,23 +113,16 @@ template <bool ENTROPY> struct RunningT {
     }
     return s;
   }
-  // a maximum above m of elements to come
+  // a maximum above m of elements to come: the sums go from fl(m c) (or m c) to fl(most c) (or most c)
   __device__ __forceinline__ void raise(float most, float c) {
     const float most_c = most * c;
-    if (near() && m != -INFINITY && fabsf(most_c) <= kNear) {  // from fl(m c) to fl(most c)
-      const float d = mc - most_c, f = ex2(d);
-      s1 = f * fmaf(d, s0, s1);
-      s0 *= f;
-    } else {
-      Stats s = sums(c);
-      s.rebase(most, c);
-      s0 = s.s0; s1 = s.s1;
-      if (fabsf(most_c) <= kNear) {  // from most c to fl(most c)
-        const float off = fmaf(most, c, -most_c), f = take_out(-off);
-        s1 = f * fmaf(off, s0, s1);
-        s0 *= f;
-      }
-    }
+    float d = (m - most) * c;
+    if (near()) d -= fmaf(m, c, -mc);
+    if (fabsf(most_c) <= kNear) d += fmaf(most, c, -most_c);
+    d = fmaxf(d, kFloor);  // (also where m = -inf)
+    const float f = ex2(d);
+    s1 = f * fmaf(d, s0, s1);
+    s0 *= f;
     m = most; mc = most_c;
   }
   // sums of N elements about m, none above it: pairs of partial sums (paired fp32 instructions).  NEAR: by the fused
