@@ -353,3 +353,44 @@ def test_linear_logprobs_of_rising_exact_logits(L, offset, rows):
     ok = (t >= 0) & (t < vocab)
     at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
     close(out["logp"], torch.where(ok, at, torch.zeros_like(at)), E + 4 * U * (lnv + at.abs()), "logp")
+
+
+@pytest.mark.parametrize("rows,dim,vocab", [(3, 72, 1000), (8, 72, 17), (9, 72, 1000), (300, 136, 700), (20, 1032, 513)])
+def test_linear_logprobs_of_infinite_and_nan_logits(L, rows, dim, vocab):
+    """A logit of -inf is masked; one of +inf or NaN makes the statistics NaN; as on stored logits."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    h = torch.zeros(rows, dim, device="cuda").bfloat16()
+    h[:, 5] = 1
+    h[rows // 2] = 0
+    h[rows // 2, 6] = 1                                       # (another row: column 6 stays finite)
+    w = (torch.randn(vocab, dim, device="cuda", generator=g) * 3).bfloat16()
+    other = w.clone()
+    gone = torch.rand(vocab, device="cuda", generator=g) < 0.5
+    gone[vocab // 2] = False
+    t = targets_for(rows, vocab)
+    E, lnv = (8 + math.ceil(vocab / 64) + 5 * 20) * U, math.log(vocab)
+    for last in (False, True):                                # masks in the last tile, and everywhere
+        z = gone if last else gone & (torch.arange(vocab, device="cuda") >= vocab - 9)
+        x = torch.where(z, torch.full((), NINF, device="cuda", dtype=torch.float64), w[:, 5].double())[None].repeat(rows, 1)
+        x[rows // 2] = w[:, 6].double()
+        # (the rows with column 5 alone: 0 times -inf would be NaN)
+        v = other.clone()
+        v[z, 5] = NINF
+        keep = torch.arange(rows, device="cuda") != rows // 2
+        out = call_head(L, h, v, t, 1.0)
+        logp, lse = softmax64(x, 1.0)
+        close(out["lse"][keep], lse[keep], E + 4 * U * (lnv + 20), "lse")
+        close(out["entropy"][keep], entropy64(logp)[keep], E * (2 + lnv) + 4 * U * (lnv + 1), "entropy")
+        ok = (t >= 0) & (t < vocab)
+        at = logp.gather(1, t.clamp(0, vocab - 1).long()[:, None])[:, 0]
+        want = torch.where(ok, at, torch.zeros_like(at))
+        close(out["logp"][keep], want[keep], E + 4 * U * (lnv + 20), "logp")
+    for bad in (math.inf, math.nan):
+        v = other.clone()
+        v[vocab // 3, 5] = bad
+        out = call_head(L, h, v, t, 1.0)
+        assert torch.isnan(out["lse"][keep]).all() and torch.isnan(out["entropy"][keep]).all()
+    v = other.clone()
+    v[:, 5] = NINF
+    out = call_head(L, h, v, t, 1.0)                          # nothing left
+    assert bool((out["lse"][keep] == NINF).all()) and bool((out["entropy"][keep] == 0).all())
