@@ -258,9 +258,9 @@ def test_tensors_of_another_kind_are_refused():
 @pytest.mark.parametrize("T,weight,k", [(2.0, 0.75, 8), (1.0, 0.3, 3), (4.0, 1.0, 20)])
 def test_trainer_step_is_the_distillation_step(tmp_path, T, weight, k):
     """A step of the trainer with a teacher: loss and gradients of the explicit calls on a model of the same weights, and
-    the loss by its formula from both models' fp32 logits.  The step's logits are bf16: a student's ln p is off by twice
-    2^-9 of the largest logit at scale 1 / T, a teacher's q by twice that of itself, so q (ln q - ln p) by four of them
-    times (1 + |ln q - ln p|)."""
+    the loss by its formula from both models' fp32 logits.  The step's logits are bf16: each is off by at most half a step
+    of the largest one (2^-8 of its power of two), a student's ln p by twice that at scale 1 / T, a teacher's q by twice
+    that of itself, so q (ln q - ln p) by four of them times (1 + |ln q - ln p|)."""
     from zerollm_b200 import Config, ZeroLLM, trainer
     cfg = Config(vocab_size=256, embed_dim=128, num_layers=2, num_heads=2, ff_hidden_dim=256, max_seq_len=128)
     B, S, V = 4, 128, 256
@@ -289,7 +289,7 @@ def test_trainer_step_is_the_distillation_step(tmp_path, T, weight, k):
     other = float(m.distill_step(tr.d_ids, rec["top_ids"], rec["top_logp"], tr.d_tg, B, S, 1e-3, scale=1.0 / T,
                                  distill_weight=weight * T * T, target_weight=1.0 - weight))
     assert abs(loss - other) <= 1e-5 * abs(other) and rel(got, m.grads()) < GRAD_TOL
-    step = 2.0 ** -9 * float(torch.maximum(ls.abs().amax(), lt.abs().amax()))
+    step = 2.0 ** (math.floor(math.log2(float(torch.maximum(ls.abs().amax(), lt.abs().amax())))) - 8)
     slack = weight * T * T * 4 * step / T * (1 + float((lq - lp).abs().max())) + (1 - weight) * 2 * step
     assert abs(loss - float(want)) < slack
     # a step on the cross-entropy alone would fail: its loss is within 2 step of ce, and slack >= step (4 weight T + 2 - 2
