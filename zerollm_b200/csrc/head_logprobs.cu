@@ -11,10 +11,11 @@
 // partial; a second small kernel joins a row's partials in a fixed order.
 //
 // Measured (2 T V d flops at the measured 1.63 PFLOP/s burst / 1.39 PFLOP/s sustained rates): 16384 x 2048 x 32000
-// 1.34 ms in a burst, 1.51 ms sustained (floor 1.32 / 1.54 ms): the tensor cores bind.  32768 x 512 x 6400 158 / 183 us
-// (floor 133 / 154 us); without the epilogue's arithmetic 136 us, so there the epilogue's exponentials cost the rest;
-// sixteen epilogue warps in place of eight gained 1 % there and lost 4 % on the long reduction.  With the weight and
-// hidden both streamed and a row tile's vocabulary walked by one pair the same took 2.60 ms and 209 us.
+// 1.27 to 1.38 ms in a burst of 30 passes, 1.48 to 1.54 ms over seconds (floor 1.32 / 1.54 ms): the tensor cores bind.
+// 32768 x 512 x 6400 154 to 158 / 177 to 184 us (floor 133 / 154 us); without the epilogue's arithmetic 136 us, so there
+// the epilogue's exponentials cost the rest; sixteen epilogue warps in place of eight gained 1 % there and lost 4 % on the
+// long reduction.  With the weight and hidden both streamed and a row tile's vocabulary walked by one pair the same took
+// 2.60 ms and 209 us.
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
@@ -36,7 +37,7 @@ constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of 
 constexpr int kHeld = 8;
 // Reduction blocks that the tensor core sums at once; a longer reduction's chunks are added in fp32 by the epilogue.
 // Each step of 16 products is cut to fp32 toward zero, so a sum comes out too small in magnitude by 0.1 to 0.9 of 2^-24 for
-// every step behind it, which like a temperature moves a row's entropy (of 512 x 4096 x 8000, random: 2.2e-6 of itself).
+// every step behind it, which like a temperature moves a row's entropy (of 16384 x 2048 x 32000, undivided: 1.7e-6 of it).
 // Chunks of 64 steps bound that for any length (8e-7), at the time of the undivided sum: 16384 x 2048 x 32000 1.27 ms in a
 // burst, 1.485 ms sustained; chunks of 32 steps (4e-7) took 1.33 and 1.57 ms.
 constexpr int kChunk = 16;
@@ -358,8 +359,8 @@ int pair_slots() {
 // device memory to registers, and the rows of hidden as B, from shared memory.  The order of the reduction index is
 // free as long as both operands use the same one, so a lane's 16-byte load of 8 consecutive elements of one weight row
 // serves as its A registers of two products.  A lane has the logits of 2 entries x 2 rows and folds them into the
-// statistics of these rows; a block leaves one partial per row.  Measured: one row of 2048 x 32000 28.6 us with the
-// join (131 MB, 20 us at the copy rate), of 2048 x 128000 84 us (95 % of it); on the tensor-core tiles 47 us.  Eight
+// statistics of these rows; a block leaves one partial per row.  Measured: one row of 2048 x 32000 28.7 us with the
+// join (131 MB, 20 us at the copy rate), of 2048 x 128000 84 to 87 us (92 to 95 % of it); on the tensor-core tiles 47 us.  Eight
 // loads of a weight row in flight per lane; four of them with 3 or 4 blocks an SM took 34 / 37 us.
 constexpr int kFewRows = 8, kFewWarps = 8, kFewBlocks = 2, kFewDim = 8192;  // (hidden: up to 128 KB of shared memory)
 

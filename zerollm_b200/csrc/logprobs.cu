@@ -533,10 +533,11 @@ template <typename T, int NW, int TEAMS> size_t logprobs_smem(const LogprobArgs&
 // k-th largest of the maxima of 32 to 256 disjoint sets of elements is a bound that at least k elements reach, and
 // few more where values come in any order; the maxima of the single vectors, kept in shared memory, say which
 // vectors to read again (from L2).  The candidates' ranks are counted.
-// Measured: 32768 x 6400 bf16 118 us with 16 alternatives, 92 us without (419 MB, 64 us at the copy rate; the ring
+// Measured: 32768 x 6400 bf16 118 us with 16 alternatives, 91 us without (419 MB, 64 us at the copy rate; the ring
 // alone, without arithmetic, takes 64 us).  Bound by instructions: about 270 for a lane's 32 logits of a piece
 // (unpacking, maxima, clamp, exponential, two sums) and 700 for a row's alternatives fill 2/3 of the issue slots and
-// half of the exponential units.  1021 x 50001 39 us, 1 x 32000 with 20 about 9 us (8 of them the host's call).
+// half of the exponential units.  With 7/8 of each row masked 115 us by -inf or -1e4, 176 us by -1e9, whose pieces are
+// added element by element.  1021 x 50001 38 us, 1 x 32000 with 20 about 8.5 us (8 of them the host's call).
 //
 // LOOSE (one warp to a row): a short row with too few vectors for its groups to bound anything, or a large k with
 // fewer than 256 groups.  All of its elements are ranked, or where those are too many none is found by a bound and
@@ -750,7 +751,7 @@ struct LogprobBwdArgs {
   int64_t d_stride;
 };
 
-// A row whose lse is so far from 0 that its rounding shows in p (kFarLse on, 2^-17 of p below it; a row masked with -1e9,
+// A row whose lse is so far from 0 that its rounding shows in p (kFarLse on, at most 2^-17 of p below it; a row masked with -1e9,
 // whose lse holds nothing of ln V, at the far end): one block finds the row's maximum and sum again and has all of its
 // gradient, read a second time after the whole row was read once (it may lie in the logits' place).  32768 x 6400 bf16
 // of such rows 224 us, 135 us of others.
@@ -911,7 +912,8 @@ struct DistillArgs {
 };
 
 // How the second exponential, e1 = 2^((x - m) log2 e) beside e = 2^((x - m) s log2 e), is had: not at all (no
-// hard targets, or s = 1), as the square of the first (s = 1/2), as the fourth power (s = 1/4), or by itself.
+// hard targets, or s = 1), as the square of the first (s = 1/2), as the fourth power (s = 1/4), or by itself.  A power has
+// twice or four times the first one's relative error (2^-22 of the instruction): 1e-6 at most.
 enum Second { kNone, kSquare, kFourth, kOwn };
 
 // Sums of both exponentials about a maximum.
@@ -1132,9 +1134,10 @@ __device__ __forceinline__ void distill_gradient(Feed<T, NW>& feed, uint32_t& ta
 // exponentials from one reading of the row, the dense part of the gradient from a second one (out of L2, and already
 // under way while the sums are joined), then the at most k + 1 elements with a teacher's or target's share.  An element
 // is read for the last time before its gradient is written, so the gradient may take its place.
-// Measured: 32768 x 6400 bf16 with 16 alternatives and hard targets at scale 1/2 199 us, 195 us at scale 1 without
-// targets, 277 us at scale 0.7 with them (839 MB, 128 us at the copy rate); 2048 x 32000 63 us (262 MB), 64 x 262139
-// fp32 39 us (134 MB).  Bound by instructions (two exponentials a logit, about 1000 instructions a row beside them).
+// Measured, in a burst of 30 passes: 32768 x 6400 bf16 with 16 alternatives and hard targets at scale 1/2 198 us (209 us
+// over seconds, under the power cap), 188 us at scale 1 without targets, 282 us at scale 0.7 with them (839 MB, 128 us at
+// the copy rate); 2048 x 32000 63 us (262 MB), 64 x 262139 fp32 39 us (134 MB).  Bound by instructions (two
+// exponentials a logit, about 1000 instructions a row beside them).
 // Rows kept in shared memory from their sums to their gradient ran at 233 us: fewer warps fit.
 template <typename T, int NW, int TEAMS, int SECOND>
 __global__ void __launch_bounds__(NW * TEAMS * 32, 24 / (NW * TEAMS)) distill_kernel(const DistillArgs a) {
@@ -1471,7 +1474,8 @@ zl_status token_logprobs_backward(const T* logits, int64_t stride, const int32_t
   if (g_entropy && !entropy) return set_error(ZL_EINVAL, "%s: a gradient of entropies needs the entropies", what);
   if ((const void*)d == (const void*)logits && d_stride != stride)
     return set_error(ZL_EINVAL, "%s: a gradient in the logits' place has their row stride", what);
-  // (128 threads to a block: 32768 x 6400 bf16 146 us, 161 / 195 us with 256 / 512; 839 MB, 88 % of the copy rate)
+  // (128 threads to a block: 32768 x 6400 bf16 135 to 138 us in a burst, 143 / 236 us with 256 / 512; 839 MB, 128 us at the
+  // copy rate; 145 us over seconds)
   constexpr int NT = 128;
   constexpr int per = NT * Elt<T>::VEC * 4;
   const int slices = (int)(((int64_t)vocab + per - 1) / per);
