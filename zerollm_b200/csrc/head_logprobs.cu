@@ -360,7 +360,7 @@ int pair_slots() {
 // free as long as both operands use the same one, so a lane's 16-byte load of 8 consecutive elements of one weight row
 // serves as its A registers of two products.  A lane has the logits of 2 entries x 2 rows and folds them into the
 // statistics of these rows; a block leaves one partial per row.  Measured: one row of 2048 x 32000 28.7 us with the
-// join (131 MB, 20 us at the copy rate), of 2048 x 128000 84 to 87 us (92 to 95 % of it); on the tensor-core tiles 47 us.  Eight
+// join (131 MB, 20 us at the copy rate), of 2048 x 128000 84 to 87 us (92 to 95 % of it); nine rows, on the tensor-core tiles, 39 us.  Eight
 // loads of a weight row in flight per lane; four of them with 3 or 4 blocks an SM took 34 / 37 us.
 constexpr int kFewRows = 8, kFewWarps = 8, kFewBlocks = 2, kFewDim = 8192;  // (hidden: up to 128 KB of shared memory)
 
