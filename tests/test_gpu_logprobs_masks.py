@@ -394,3 +394,26 @@ def test_linear_logprobs_of_infinite_and_nan_logits(L, rows, dim, vocab):
     v[:, 5] = NINF
     out = call_head(L, h, v, t, 1.0)                          # nothing left
     assert bool((out["lse"][keep] == NINF).all()) and bool((out["entropy"][keep] == 0).all())
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 2048), (4, 4096), (8, 8192), (3, 8192)])
+def test_linear_logprobs_of_few_rows_is_as_exact_as_fp32(L, rows, dim):
+    """Up to eight rows a logit is a sum of joins of four chains of at most four steps of 16 products (dim a multiple of
+    256): off by at most (2 * 4 + dim / 256 + 3) u sum |h w|.  A chain's steps, cut toward zero, shrink it by less than u
+    each, which moves the entropy by 4 u times the variance of ln p (2.5^2) over itself (above 6): 5 u; its own sums'
+    roundings, at random, add a few u."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    vocab = 8000
+    worst = 0.0
+    for _ in range(6):
+        h = torch.randn(rows, dim, device="cuda", generator=g).bfloat16()
+        w = (torch.randn(vocab, dim, device="cuda", generator=g) * (2.5 / math.sqrt(dim))).bfloat16()
+        t = targets_for(rows, vocab)
+        out = call_head(L, h, w, t, 1.0)
+        x = h.double() @ w.double().T
+        logp, lse = softmax64(x, 1.0)
+        off = (8 + dim / 256 + 3) * U * (h.double().abs() @ w.double().abs().T).amax(1)
+        E, lnv = (8 + math.ceil(vocab / 64) + 5 * 20) * U, math.log(vocab)
+        close(out["lse"], lse, off + E + 4 * U * (lnv + x.amax(1).abs()), "lse")
+        worst = max(worst, float((out["entropy"].double() - entropy64(logp)).norm() / entropy64(logp).norm()))
+    assert worst < 16 * U

@@ -393,7 +393,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
     const int n0 = tile * 16 + g, n1 = n0 + 8;  // this lane's weight rows (the last one again past the end)
     const uint4* w0 = reinterpret_cast<const uint4*>(weight + (int64_t)min(n0, a.vocab - 1) * dim) + q;
     const uint4* w1 = reinterpret_cast<const uint4*>(weight + (int64_t)min(n1, a.vocab - 1) * dim) + q;
-    float d[4][4] = {};  // (four sums of a quarter of the products each: a quarter of the steps that cut one)
+    float d[4][4] = {}, sum[4] = {};  // (sums of a few products each, joined in fp32: few steps that cut one)
+    auto join = [&] {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sum[j] += (d[0][j] + d[1][j]) + (d[2][j] + d[3][j]);
+        d[0][j] = d[1][j] = d[2][j] = d[3][j] = 0.f;
+      }
+    };
     auto product = [&](const uint4& u0, const uint4& u1, int b, int half) {
       const uint4 x = h[(b * 8 + g) * 4 + q];
       mma_16816(d[half], u0.x, u1.x, u0.y, u1.y, x.x, x.y);
@@ -411,14 +418,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewBlocks)
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) product(u0[i], u1[i], b + i, i % 2 * 2);
+      join();
     }
     for (; b < blocks; ++b) {
       const bool in = b * 4 + q < vecs;
       product(in ? __ldg(w0 + b * 4) : make_uint4(0, 0, 0, 0), in ? __ldg(w1 + b * 4) : make_uint4(0, 0, 0, 0), b, 0);
     }
+    join();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float x0 = (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]), x1 = (d[0][2 + i] + d[1][2 + i]) + (d[2][2 + i] + d[3][2 + i]);
+      const float x0 = sum[i], x1 = sum[2 + i];
       if (n0 < a.vocab) {
         run[i].add_one(x0, a.c);
         if (t[i] == n0) xt[i] = x0;
