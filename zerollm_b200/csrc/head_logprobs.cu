@@ -27,6 +27,7 @@ int sm_count_current();  // gemm.cu
 bool make_tma_map(CUtensorMap* map, const void* ptr, bool is_f32, uint64_t inner, uint64_t rows, uint32_t box_inner,
                   uint32_t box_rows, int swizzle_bytes, uint64_t row_stride);
 
+
 namespace {
 constexpr int BM = 128, BN = 256, BK = 64;   // rows of a CTA, vocabulary entries of a tile, reduction block
 constexpr int kEpiWarps = 8, kShares = kEpiWarps / 4;  // epilogue warps; those that share a row, each its columns of a tile
@@ -35,12 +36,14 @@ constexpr int kTileBytes = BM * BK * 2;      // a CTA's share of hidden, and of 
 // A short reduction (up to kHeld blocks) keeps the row tile of hidden in shared memory from one vocabulary tile to the
 // next; its ring holds weight blocks.  A longer one streams both through a ring of pairs.
 constexpr int kHeld = 8;
-// Reduction blocks that the tensor core sums at once; a longer reduction's chunks are added in fp32 by the epilogue.
-// Each step of 16 products is cut to fp32 toward zero, so a sum comes out too small in magnitude by 0.1 to 0.9 of 2^-24 for
-// every step behind it, which like a temperature moves a row's entropy (of 16384 x 2048 x 32000, undivided: 1.7e-6 of it).
-// Chunks of 64 steps bound that for any length (8e-7), at the time of the undivided sum: 16384 x 2048 x 32000 1.27 ms in a
-// burst, 1.485 ms sustained; chunks of 32 steps (4e-7) took 1.33 and 1.57 ms.
-constexpr int kChunk = 16;
+// Most reduction blocks that the tensor core sums at once; a longer reduction is cut into chunks alike, added in fp32 by
+// the epilogue.  Each step of 16 products is cut to fp32 toward zero, so a sum comes out too small in magnitude by 0.1 to
+// 0.9 of 2^-24 for every step behind it, which like a temperature moves a row's entropy (of 16384 x 2048 x 32000,
+// undivided: 1.7e-6 of it).  Chunks of up to 48 steps bound that for any length (6e-7 there).  Reading an accumulator takes
+// 1800 cycles, about what tensor memory gives beside the products, and a tile's statistics 3200; the products of two chunks
+// have to last as long: undivided, or in three chunks of 11, 1.31 ms there, in four of 8 1.36 ms, in seven of 5 a third
+// more; 8192 x 1024 x 16000 171 us undivided, 176 us in two chunks.
+constexpr int kChunk = 12;
 static_assert(kHeld <= kChunk, "a reduction that is held is one chunk");
 template <bool HELD> struct Smem {
   static constexpr int STAGES = HELD ? 5 : 6;
@@ -89,7 +92,8 @@ struct HeadArgs {
   int rows, vocab, k_blocks, row_tiles, n_tiles, slots, group;
   int64_t steps, per;
   float c;  // scale * log2(e)
-  int few;           // few rows: partials of a row, one of each block
+  int chunk;  // reduction blocks of a chunk (at most kChunk, alike)
+  int few;    // few rows: partials of a row, one of each block
   float4* partials;  // [row][slot][share] (m, S0, S1, target logit)
 };
 
@@ -200,12 +204,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       while (ok && seg.next(a)) {
         for (int nt = seg.nt0; nt < seg.nt1 && ok; ++nt) {
-          for (int k0 = 0; k0 < a.k_blocks && ok; k0 += kChunk) {
+          for (int k0 = 0; k0 < a.k_blocks && ok; k0 += a.chunk) {
             // both CTAs' epilogues have drained accumulator `acc`
             if (!__all_sync(0xffffffffu, bounded_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, DEV_TIMEOUT_ACC))) { ok = false; break; }
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-            const int k1 = HELD ? a.k_blocks : min(a.k_blocks, k0 + kChunk);
+            const int k1 = HELD ? a.k_blocks : min(a.k_blocks, k0 + a.chunk);
             for (int kb = k0; kb < k1; ++kb) {
               if (HELD && nt == seg.nt0 && !bounded_wait_warp(&h_full[kb], h_phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
               if (!bounded_wait_warp(&full[stage], phase, DEV_TIMEOUT_FULL)) { ok = false; break; }
@@ -277,24 +281,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           drained();
         } else {  // the sum of the chunks in registers; the last accumulator is free before its logits are folded
-          float v[COLS / 32][32] = {};
-          for (int kb = 0; kb < a.k_blocks; kb += kChunk) {
+          uint32_t v[COLS / 8][8];  // (the first chunk comes straight into them)
+          if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < COLS / 8; ++c) tmem_ld8(t_row + (uint32_t)(acc * BN + c * 8), v[c]);
+          tmem_ld_wait();
+          drained();
+          for (int kb = a.chunk; kb < a.k_blocks; kb += a.chunk) {
             if (!bounded_wait_warp(&acc_full[acc], acc_phase, DEV_TIMEOUT_ACC)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < COLS; c += 16) {
-              uint32_t u[16];
-              tmem_ld16(t_row + (uint32_t)(acc * BN + c), u);
+            for (int c = 0; c < COLS / 8; c += 2) {
+              uint32_t u[2][8];
+#pragma unroll
+              for (int p = 0; p < 2; ++p) tmem_ld8(t_row + (uint32_t)(acc * BN + (c + p) * 8), u[p]);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                v[c / 32][c % 32 + j] += __uint_as_float(u[j]);
+              for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c + p][j] = __float_as_uint(__uint_as_float(v[c + p][j]) + __uint_as_float(u[p][j]));
             }
             drained();
           }
           if (!ok) break;
 #pragma unroll
-          for (int c = 0; c < COLS / 32; ++c) fold(v[c], n0 + c * 32);
+          for (int c = 0; c < COLS / 32; ++c) {
+            float x[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[(c * 32 + j) / 8][j % 8]);
+            fold(x, n0 + c * 32);
+          }
         }
       }
       if (ok && row < a.rows) {  // this pair's partial of the row
@@ -547,7 +564,7 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
        reinterpret_cast<uintptr_t>(lse)) & 3)
     return set_error(ZL_EINVAL, "%s: a target or output array off a 4-byte boundary", what);
   if (rows <= kFewRows && dim <= kFewDim) {
-    HeadArgs a{targets, rows, vocab, 0, 0, 0, 0, 0, 0, 0, scale * kLog2e, few_blocks(vocab), reinterpret_cast<float4*>(workspace)};
+    HeadArgs a{targets, rows, vocab, 0, 0, 0, 0, 0, 0, 0, scale * kLog2e, 0, few_blocks(vocab), reinterpret_cast<float4*>(workspace)};
     const size_t smem = (size_t)(dim + 31) / 32 * 512;
     cudaError_t e = cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewDim / 32 * 512);
     if (e != cudaSuccess) return launched(what, e);
@@ -562,7 +579,9 @@ extern "C" zl_status zl_linear_logprobs_bf16(const zl_bf16* hidden, const zl_bf1
       !make_tma_map(&mw, weight, false, dim, vocab, BK, BN / 2, 128, 0))
     return set_error(ZL_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
   HeadArgs a{targets, rows, vocab, (dim + BK - 1) / BK, p.row_tiles, p.n_tiles, p.slots, p.group, p.steps, p.per,
-             scale * kLog2e, 0, reinterpret_cast<float4*>(workspace)};
+             scale * kLog2e, 0, 0, reinterpret_cast<float4*>(workspace)};
+  const int chunks = (a.k_blocks + kChunk - 1) / kChunk;
+  a.chunk = (a.k_blocks + chunks - 1) / chunks;
   const bool held = a.k_blocks <= kHeld;
   cudaLaunchAttribute attr;
   const cudaLaunchConfig_t cfg = pair_config(p.pairs, held ? Smem<true>::TOTAL : Smem<false>::TOTAL, (cudaStream_t)stream, &attr);
