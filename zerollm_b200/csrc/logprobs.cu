@@ -1079,7 +1079,14 @@ __device__ __forceinline__ Sums2 distill_sums(Feed<T, NW>& feed, uint32_t& taken
         uint4 w = u[0];
 #pragma unroll
         for (int i = 1; i < kLaneVecs; ++i) w = i == j ? u[i] : w;
-        add(w, std::true_type());
+        if constexpr (SECOND == kOwn) {  // (by elements: in pairs it cost other rows 281 instead of 277 us at 32768 x 6400)
+          float f[VEC];
+          Elt<T>::unpack(w, f);
+#pragma unroll
+          for (int l = 0; l < VEC; ++l) one(f[l]);
+        } else {
+          add(w, std::true_type());
+        }
       }
     } else {
 #pragma unroll
@@ -1142,7 +1149,7 @@ __device__ __forceinline__ void distill_gradient(Feed<T, NW>& feed, uint32_t& ta
 // under way while the sums are joined), then the at most k + 1 elements with a teacher's or target's share.  An element
 // is read for the last time before its gradient is written, so the gradient may take its place.
 // Measured, in a burst of 30 passes: 32768 x 6400 bf16 with 16 alternatives and hard targets at scale 1/2 198 us (209 us
-// over seconds, under the power cap), 188 us at scale 1 without targets, 282 us at scale 0.7 with them (839 MB, 128 us at
+// over seconds, under the power cap), 188 us at scale 1 without targets, 277 us at scale 0.7 with them (839 MB, 128 us at
 // the copy rate); 2048 x 32000 63 us (262 MB), 64 x 262139 fp32 39 us (134 MB).  Bound by instructions (two
 // exponentials a logit, about 1000 instructions a row beside them).
 // Rows kept in shared memory from their sums to their gradient ran at 233 us: fewer warps fit.
